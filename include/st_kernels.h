@@ -431,6 +431,63 @@ long long st_format_attack_log(const char* vocab_bytes, const int64_t* vocab_off
                                const int32_t* n_iter, const uint8_t* changed, const int32_t* rows, char* out,
                                long long out_cap);
 
+/* ---------------------------------------------------------------------------------------------
+ * (10) Products with 4-bit weights and group scales.  NO COUNTERPART IN THE REFERENCE: a decode step of few rows is bound by
+ * reading the generator matrix (9339 x 256 f32 = 9.6 MB), in 4 bits an eighth of it.
+ *   y[m, n] = sum_k x[m, k] * scale[n, k / group] * (code[n, k] - zero[n, k / group]) + bias[n]
+ *   codes   u8 [N, ceil(K / 2)]: two a byte, the even column in the low four bits (an odd K's last high bits are ignored)
+ *   scales  f16 [N, ceil(K / group)]       zeros  u8 [N, ceil(K / group)] (0..15; the upper bits are ignored) or NULL: 8
+ *   group   32, 64 or 128; the last group of a row may be short
+ * st_quantize_weight_q4 makes codes, scales (and zeros, when not NULL) of an f32 matrix [N, K]: scale = max |w| / 7, or
+ * (max - min) / 15 with 0 in the range, rounded to f16; a code is the nearest one under the rounded scale.
+ * st_pack_weight_q4 lays them out for the product (once per weight); the image takes st_q4_packed_bytes and must lie on 16
+ * bytes.  st_gemm_q4: x [M, K] and y [M, N] of `type` (ST_TYPE_*), rows ldx and ldy values apart (any alignment of whole
+ * values); bias f32 [N] or NULL.  Sums are held in f32, one rounding to y's type at the end; the codes enter the product as they
+ * are, an f32 x with 22 significant bits and more.  A row of x with an infinity or a NaN gives values that are not finite.
+ * M = 0 is a no-op.  Asynchronous, needs no workspace, may be captured into a graph.                                       */
+#define ST_TYPE_F32 0
+#define ST_TYPE_BF16 1
+#define ST_TYPE_F16 2
+typedef struct StQ4Weight {
+  const void* image;                 /* st_pack_weight_q4                                                             */
+  int32_t N, K, group, has_zeros;    /* as packed                                                                     */
+} StQ4Weight;
+size_t st_q4_packed_bytes(int N, int K, int group, int has_zeros);
+int st_quantize_weight_q4(const float* W, int N, int K, int group, uint8_t* codes, void* scales, uint8_t* zeros, void* stream);
+int st_pack_weight_q4(const uint8_t* codes, const void* scales, const uint8_t* zeros, int N, int K, int group, void* out_packed,
+                      void* stream);
+int st_gemm_q4(const void* x, int type, int64_t ldx, int M, const StQ4Weight* w, const float* bias, void* y, int64_t ldy,
+               void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * (11) A token drawn from every row of logits [B, V] (f32, bf16 or f16; rows ld values apart, any alignment of whole values),
+ * from given uniform numbers u [B] in [0, 1).  NO COUNTERPART IN THE REFERENCE, whose decoder is greedy (model.py:289-292).
+ *   w_i = exp((l_i - max l) / temperature); entries are ranked by logit, equal ones by index.  Kept are the first top_k (0: all),
+ *   of those the shortest prefix with top_p of their mass (1: all), of those the ones with w >= min_p (0: all); the first entry
+ *   always.  ids[b] = the first kept entry at which the cumulative mass exceeds u * (kept mass);
+ *   logp[b] (may be NULL) = log of its share of the kept mass.
+ *   temperature 0: the largest logit, lowest index first, logp 0.  Logits of -inf or NaN are never drawn; a row with nothing else
+ *   gives id -1 and logp -inf.  Equal infinities of the largest logit share the mass.
+ * Masses are summed in whole numbers of 2^-44: the result depends on the row alone, not on the launch, and entries of less than
+ * 2^-45 of the largest are not drawn.
+ * Settings: one for all rows, or device arrays [B] (those not NULL).  Scalars are checked (ST_EINVAL: temperature < 0 or not
+ * finite, top_k < 0, top_p outside (0, 1], min_p outside [0, 1]); array values act as written above, with temperature <= 0 or
+ * NaN greedy, top_k <= 0 off, top_p <= 0 the first entry alone, top_p >= 1 or NaN off, min_p <= 0 or NaN off, min_p > 1 the first alone.
+ * u is clamped to [0, 1]; a NaN counts as 0.  V <= ST_SAMPLE_MAX_VOCAB.  B = 0 is a no-op.  Asynchronous, may be captured into
+ * a graph; calls that overlap need workspaces of their own (nothing in one has to be cleared).                              */
+#define ST_SAMPLE_MAX_VOCAB 524288
+typedef struct StSampleSettings {
+  float temperature;
+  int32_t top_k;
+  float top_p, min_p;
+  const float* temperature_rows;     /* NULL: the scalar above                                                        */
+  const int32_t* top_k_rows;
+  const float *top_p_rows, *min_p_rows;
+} StSampleSettings;
+size_t st_sample_workspace_bytes(int B, int V);
+int st_sample_logits(const void* logits, int type, int64_t ld, int B, int V, const float* u, const StSampleSettings* settings,
+                     int32_t* ids, float* logp, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

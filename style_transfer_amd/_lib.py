@@ -20,7 +20,9 @@ ST_DEC_NO_L0_TABLE = 4
 ST_PROF_OFF, ST_PROF_GENERATOR, ST_PROF_HALF_LAYER = 0, 1, 2
 ST_GEMM_F32, ST_GEMM_F16X3 = 0, 1
 GEMM_FORMATS = {"f32": ST_GEMM_F32, "f16x3": ST_GEMM_F16X3}
-ABI_VERSION = 8
+ST_TYPE_F32, ST_TYPE_BF16, ST_TYPE_F16 = 0, 1, 2
+ST_SAMPLE_MAX_VOCAB = 524288
+ABI_VERSION = 9
 
 fp = C.c_void_p  # device pointers travel as integers
 
@@ -77,6 +79,15 @@ class StClassifierWeights(C.Structure):
     _fields_ = [(n, fp) for n in ("w1", "b1", "w2", "b2", "w3", "b3")]
 
 
+class StQ4Weight(C.Structure):
+    _fields_ = [("image", fp)] + [(n, C.c_int32) for n in ("N", "K", "group", "has_zeros")]
+
+
+class StSampleSettings(C.Structure):
+    _fields_ = [("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float),
+                ("temperature_rows", fp), ("top_k_rows", fp), ("top_p_rows", fp), ("min_p_rows", fp)]
+
+
 EXPORTS = {
     # name: (restype, argtypes)
     "st_fgim_perturb": (C.c_int, [C.POINTER(StClassifierWeights), fp, fp, fp, C.c_int, C.c_int, fp, fp, fp, fp]),
@@ -119,6 +130,12 @@ EXPORTS = {
     "st_format_attack_log": (C.c_longlong, [C.c_char_p, fp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_char_p, C.c_int, C.c_int,
                                             C.c_int, C.c_longlong, fp, fp, fp, fp, C.c_int, fp, C.c_int, fp, fp, fp, fp,
                                             C.c_longlong]),
+    "st_q4_packed_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int]),
+    "st_quantize_weight_q4": (C.c_int, [fp, C.c_int, C.c_int, C.c_int, fp, fp, fp, fp]),
+    "st_pack_weight_q4": (C.c_int, [fp, fp, fp, C.c_int, C.c_int, C.c_int, fp, fp]),
+    "st_gemm_q4": (C.c_int, [fp, C.c_int, C.c_int64, C.c_int, C.POINTER(StQ4Weight), fp, fp, C.c_int64, fp]),
+    "st_sample_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "st_sample_logits": (C.c_int, [fp, C.c_int, C.c_int64, C.c_int, C.c_int, fp, C.POINTER(StSampleSettings), fp, fp, fp, C.c_size_t, fp]),
     "st_encode_latent": (C.c_int, [C.POINTER(StEncoderWeights), fp, fp, fp, C.c_int, C.c_int, C.c_int, fp, fp, C.c_size_t, fp]),
 }
 

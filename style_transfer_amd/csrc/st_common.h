@@ -18,6 +18,27 @@ bool sl_small_views_ok(int B);
 int sl_small_views(const float* ori, const float* like0, int n_views, int B, float tau, float* loss_rows, float* lse, const float* g,
                    float* d_ori_parts, float* d_like0, hipStream_t st);
 
+// internal: a draw from rows of logits (csrc/st_sample.hip; used by csrc/st_decode.hip).  Row r of the logits belongs to sentence
+// s = idx ? idx[r] : r, whose uniform number is u[s * u_stride] and whose settings are the s-th of the *_rows; ids and logp are
+// written at r; rows from *n_dev on (n_dev given) are left alone.
+struct SampleArgs {
+  const void* logits;
+  int type;
+  long ld;
+  int B, V;
+  const float* u;
+  long u_stride;
+  StSampleSettings set;
+  const int* idx;
+  const int* n_dev;
+  int32_t* ids;
+  float* logp;
+  void* ws;
+};
+int sample_check(const StSampleSettings* s);
+size_t sample_workspace(int B, int V);
+int sample_launch(const SampleArgs& a, hipStream_t st);
+
 #define ST_CHECK_ARG(cond, ...)   \
   do {                            \
     if (!(cond)) {                \
@@ -36,6 +57,12 @@ int sl_small_views(const float* ori, const float* like0, int n_views, int B, flo
   } while (0)
 
 #define ST_LAUNCH_CHECK() ST_HIP(hipGetLastError())
+
+#define ST_TRY(x)            \
+  do {                       \
+    int rc_ = (x);           \
+    if (rc_ != ST_OK) return rc_; \
+  } while (0)
 
 // Kernels that need more than 64 KiB of dynamic LDS must opt in once PER DEVICE (hipFuncSetAttribute acts on the
 // current device).  `done` is a per-kernel static array indexed by device ordinal.

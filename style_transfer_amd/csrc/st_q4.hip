@@ -1,0 +1,319 @@
+// Products with 4-bit weights and group scales: y[m, n] = sum_k x[m, k] * s[n, k / g] * (c[n, k] - z[n, k / g]) + b[n].
+//
+// A weight is read as a code c in 0..15; c - z is a whole number in -15..15, which f16 holds exactly, so the matrix cores
+// multiply f16 images of x with f16 whole numbers (v_mfma_f32_16x16x32_f16, sums in f32) and the scale is applied in f32 once a
+// group: no weight is rounded.  x in f16 goes in as it is.  x in bf16 or f32 is first multiplied, row by row, with a power of
+// two that brings the row's largest value to [2^14, 2^15): a bf16 value then is an f16 value (8 significant bits of 11; what is
+// 2^-29 of the largest and less becomes an f16 subnormal, an error below 2^-39 of the largest), an f32 value is split into
+// hi + lo as in the f16x3 format (about 2^-22 of the value) and costs two products.
+#include "st_common.h"
+
+namespace {
+
+constexpr int KB = 128;   // columns k of a block: 64 lanes x 16 bytes hold 16 rows n x 128 codes
+
+struct Q4Layout {
+  int nb, kb, gpb;         // blocks of 16 n, of 128 k; groups a block
+  size_t scales, zeros, total;   // byte offsets
+};
+
+size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
+Q4Layout q4_layout(int N, int K, int group, int has_zeros) {
+  Q4Layout y;
+  y.nb = (N + 15) / 16;
+  y.kb = (K + KB - 1) / KB;
+  y.gpb = KB / group;
+  const size_t blocks = (size_t)y.nb * y.kb;
+  y.scales = blocks * 1024;
+  y.zeros = y.scales + up256(blocks * 16 * y.gpb * 2);
+  y.total = y.zeros + (has_zeros ? up256(blocks * 16 * y.gpb) : 0);
+  return y;
+}
+
+int check_q4_shape(int N, int K, int group) {
+  ST_CHECK_ARG(N > 0 && K > 0, "N=%d K=%d must be positive", N, K);
+  ST_CHECK_ARG(N <= (1 << 24) && K <= (1 << 24), "N=%d K=%d: at most 2^24", N, K);
+  ST_CHECK_ARG(group == 32 || group == 64 || group == 128, "group=%d unsupported (32, 64, 128)", group);
+  return ST_OK;
+}
+
+// ---- image ---------------------------------------------------------------------------------------------------------------
+// Block (nb, kb) is 1 KB: lane l's 16 bytes are the codes of row n = 16 nb + (l & 15); its word j holds
+// k = 128 kb + 32 j + 8 (l >> 4) + 0..7, the operand of one 16x16x32 product.  In the word, k's pair p (2p, 2p + 1) lies in the
+// nibbles p and p + 4: one and-or makes a pair of f16 out of it.  Scales (f16) and zero codes (bytes) lie block by block,
+// [16 n][groups of the block]: a lane reads those of its row at once.  Rows from N on and groups from K on have scale 0.
+__global__ __launch_bounds__(256) void q4_pack_kernel(const uint8_t* __restrict__ codes, const uint16_t* __restrict__ scales,
+                                                      const uint8_t* __restrict__ zeros, int N, int K, int group, int nb_n, int kb_n,
+                                                      uint32_t* __restrict__ out, uint16_t* __restrict__ out_s, uint8_t* __restrict__ out_z) {
+  const size_t t = (size_t)blockIdx.x * 256 + threadIdx.x;
+  const size_t blocks = (size_t)nb_n * kb_n;
+  const int row_bytes = (K + 1) / 2, groups = (K + group - 1) / group, gpb = KB / group;
+  if (t < blocks * 256) {
+    const int j = (int)(t & 3), lane = (int)((t >> 2) & 63);
+    const size_t b = t >> 8;
+    const int kb = (int)(b % kb_n), n = (int)(b / kb_n) * 16 + (lane & 15);
+    const int k0 = kb * KB + 32 * j + 8 * (lane >> 4);
+    uint32_t w = 0;
+    if (n < N)
+      for (int i = 0; i < 8; ++i) {
+        const int k = k0 + i;
+        if (k < K) {
+          const uint32_t c = (codes[(size_t)n * row_bytes + (k >> 1)] >> (4 * (k & 1))) & 15u;
+          w |= c << (4 * ((i >> 1) + 4 * (i & 1)));
+        }
+      }
+    out[t] = w;
+  }
+  if (t < blocks * 16 * gpb) {
+    const int i = (int)(t % gpb), r = (int)((t / gpb) & 15);
+    const size_t b = t / (16 * gpb);
+    const int n = (int)(b / kb_n) * 16 + r, g = (int)(b % kb_n) * gpb + i;
+    const bool in = n < N && g < groups;
+    out_s[t] = in ? scales[(size_t)n * groups + g] : (uint16_t)0;
+    if (out_z) out_z[t] = in ? (uint8_t)(zeros[(size_t)n * groups + g] & 15) : (uint8_t)0;
+  }
+}
+
+// ---- codes of an f32 matrix ------------------------------------------------------------------------------------------------
+// One wave a (row, group).  Without zero codes: s = max |w| / 7 and z = 8; with them the range [min(w, 0), max(w, 0)] is cut into
+// 15 steps and z is 0's place in it.  s is rounded to f16 first, the codes go by the rounded one.
+__global__ __launch_bounds__(256) void q4_quantize_kernel(const float* __restrict__ W, int N, int K, int group, uint8_t* __restrict__ codes,
+                                                          _Float16* __restrict__ scales, uint8_t* __restrict__ zeros) {
+  const int groups = (K + group - 1) / group, lane = threadIdx.x & 63;
+  const size_t wv = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (wv >= (size_t)N * groups) return;
+  const int n = (int)(wv / groups), g = (int)(wv % groups);
+  const int k = g * group + 2 * lane;                 // lanes 0 .. group / 2 - 1 have two columns each
+  const bool in0 = 2 * lane < group && k < K, in1 = 2 * lane < group && k + 1 < K;
+  const float a = in0 ? W[(size_t)n * K + k] : 0.0f, b = in1 ? W[(size_t)n * K + k + 1] : 0.0f;
+  const float hi = wave_max(fmaxf(fmaxf(a, b), 0.0f)), lo = -wave_max(fmaxf(fmaxf(-a, -b), 0.0f));
+  const float step = zeros ? (hi - lo) / 15.0f : fmaxf(hi, -lo) / 7.0f;
+  const _Float16 s16 = (_Float16)fminf(step, 65504.0f);
+  const float s = (float)s16;
+  const int z = zeros ? (s > 0.0f ? min(15, max(0, (int)rintf(-lo / s))) : 0) : 8;
+  const int c0 = s > 0.0f ? min(15, max(0, (int)fminf(fmaxf(rintf(a / s), -16.0f), 16.0f) + z)) : z;
+  const int c1 = s > 0.0f ? min(15, max(0, (int)fminf(fmaxf(rintf(b / s), -16.0f), 16.0f) + z)) : z;
+  if (in0) codes[(size_t)n * ((K + 1) / 2) + (k >> 1)] = (uint8_t)(c0 | (in1 ? c1 << 4 : 0));
+  if (lane == 0) {
+    scales[wv] = s16;
+    if (zeros) zeros[wv] = (uint8_t)z;
+  }
+}
+
+// ---- product ---------------------------------------------------------------------------------------------------------------
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// 8 codes -> 8 f16 values c - z.  0x6400 | c is the f16 1024 + c; with c in the second nibble it is 1024 + 16 c, a sixteenth of
+// which is 64 + c: both corrections are exact.
+__device__ __forceinline__ h8 q4_open(uint32_t w, h2 z_low, h2 z_high) {
+  const h2 sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
+  const h2 a = __builtin_bit_cast(h2, (w & 0x000f000fu) | 0x64006400u) + z_low;
+  const h2 b = __builtin_bit_cast(h2, (w & 0x00f000f0u) | 0x64006400u) * sixteenth + z_high;
+  const uint32_t v = w >> 8;
+  const h2 c = __builtin_bit_cast(h2, (v & 0x000f000fu) | 0x64006400u) + z_low;
+  const h2 d = __builtin_bit_cast(h2, (v & 0x00f000f0u) | 0x64006400u) * sixteenth + z_high;
+  return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+template <int TYPE> struct XOf;
+template <> struct XOf<ST_TYPE_F32> { typedef float t; };
+template <> struct XOf<ST_TYPE_BF16> { typedef uint16_t t; };
+template <> struct XOf<ST_TYPE_F16> { typedef _Float16 t; };
+
+template <int TYPE> __device__ __forceinline__ float x_value(typename XOf<TYPE>::t v) {
+  if constexpr (TYPE == ST_TYPE_BF16) return __uint_as_float((uint32_t)v << 16);
+  else return (float)v;
+}
+__device__ __forceinline__ uint16_t bf16_of(float v) {   // nearest, ties to even; NaN stays NaN
+  const uint32_t u = __float_as_uint(v);
+  if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40);
+  return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1)) >> 16);
+}
+
+struct Q4Args {
+  const void* x;
+  long ldx;
+  int M, N, K, nb, kb;
+  const u32x4* codes;
+  const uint16_t* scales;
+  const uint8_t* zeros;
+  const float* bias;
+  void* y;
+  long ldy;
+  int vec;   // x's rows may be read 8 values at a time
+};
+
+// 8 values of row `row` from column k on as f32; columns from K on and absent rows are 0
+template <int TYPE> __device__ __forceinline__ void load_x8(const Q4Args& a, int row, int k, float (&v)[8]) {
+  typedef typename XOf<TYPE>::t T;
+  const T* p = (const T*)a.x + (size_t)row * a.ldx + k;
+  if (row < a.M && k + 8 <= a.K && a.vec) {
+    T t[8];
+    if constexpr (TYPE == ST_TYPE_F32) {
+      *(f32x4*)&t[0] = *(const f32x4*)p;
+      *(f32x4*)&t[4] = *(const f32x4*)(p + 4);
+    } else {
+      *(f32x4*)&t[0] = *(const f32x4*)p;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = x_value<TYPE>(t[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = row < a.M && k + i < a.K ? x_value<TYPE>(p[i]) : 0.0f;
+  }
+}
+
+// One workgroup: 16 rows m x 16 NT columns n; its waves take the k blocks in turn and are joined through shared memory.
+template <int TYPE, int GPB, int NT>
+__global__ __launch_bounds__(512) void q4_rows_kernel(Q4Args a) {
+  extern __shared__ float red[];   // [waves][NT][4][64]
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  const int m = blockIdx.y * 16 + (lane & 15), kq = 8 * (lane >> 4);
+  const int nb0 = blockIdx.x * NT;
+  float shift = 1.0f, unshift = 1.0f;
+  if constexpr (TYPE != ST_TYPE_F16) {
+    float big = 0.0f;
+    for (int b = wv; b < a.kb; b += nw)
+      for (int j = 0; j < 4; ++j) {
+        float v[8];
+        load_x8<TYPE>(a, m, b * KB + 32 * j + kq, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(v[i]));
+      }
+    big = fmaxf(big, __shfl_xor(big, 16, 64));
+    big = fmaxf(big, __shfl_xor(big, 32, 64));
+    if (big > 0.0f && big < INFINITY) {
+      const int e = min(126, max(-112, 14 - (int)((__float_as_uint(big) >> 23) & 255) + 127));
+      shift = __uint_as_float((uint32_t)(e + 127) << 23);
+      unshift = __uint_as_float((uint32_t)(127 - e) << 23);
+    }
+  }
+  f32x4 acc[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) acc[t] = f32x4{0, 0, 0, 0};
+  for (int b = wv; b < a.kb; b += nw) {
+    h8 xh[4], xl[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float v[8];
+      load_x8<TYPE>(a, m, b * KB + 32 * j + kq, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float s = v[i] * shift;
+        xh[j][i] = (_Float16)s;
+        if constexpr (TYPE == ST_TYPE_F32) xl[j][i] = (_Float16)fmaxf(s - (float)xh[j][i], -65504.0f);   // an infinite value: inf - inf
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      if (nb0 + t >= a.nb) continue;
+      const size_t blk = (size_t)(nb0 + t) * a.kb + b;
+      const u32x4 w = a.codes[blk * 64 + lane];
+#pragma unroll
+      for (int g = 0; g < GPB; ++g) {
+        const size_t at = (blk * 16 + (lane & 15)) * GPB + g;
+        const float s = (float)__builtin_bit_cast(_Float16, a.scales[at]);
+        const float z = a.zeros ? (float)a.zeros[at] : 8.0f;
+        const _Float16 zl = (_Float16)(-1024.0f - z), zh = (_Float16)(-64.0f - z);
+        f32x4 part = {0, 0, 0, 0};
+#pragma unroll
+        for (int j = g * (4 / GPB); j < (g + 1) * (4 / GPB); ++j) {
+          const h8 wj = q4_open(w[j], h2{zl, zl}, h2{zh, zh});
+          part = mfma16x32h(xh[j], wj, part);
+          if constexpr (TYPE == ST_TYPE_F32) part = mfma16x32h(xl[j], wj, part);
+        }
+        acc[t] += part * s;
+      }
+    }
+  }
+  // the product's rows m are 4 (lane >> 4) + i, its columns n are lane & 15: every row's power of two is taken back here
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float f = __shfl(unshift, 4 * (lane >> 4) + i, 64);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) red[((wv * NT + t) * 4 + i) * 64 + lane] = acc[t][i] * f;
+  }
+  __syncthreads();
+  typedef typename XOf<TYPE>::t T;
+  for (int o = threadIdx.x; o < NT * 256; o += blockDim.x) {
+    const int row = blockIdx.y * 16 + o / (16 * NT), col = o % (16 * NT), n = nb0 * 16 + col;
+    const int src = ((col >> 4) * 4 + ((o / (16 * NT)) & 3)) * 64 + 16 * ((o / (16 * NT)) >> 2) + (col & 15);
+    if (row >= a.M || n >= a.N) continue;
+    float s = 0.0f;
+    for (int q = 0; q < nw; ++q) s += red[q * NT * 256 + src];
+    if (a.bias) s += a.bias[n];
+    T* y = (T*)a.y + (size_t)row * a.ldy + n;
+    if constexpr (TYPE == ST_TYPE_BF16) *y = bf16_of(s);
+    else *y = (T)s;
+  }
+}
+
+template <int TYPE, int GPB> int q4_launch(const Q4Args& a, hipStream_t st) {
+  const int nw = a.kb < 8 ? a.kb : 8, nt = 4;
+  hipLaunchKernelGGL((q4_rows_kernel<TYPE, GPB, 4>), dim3((a.nb + nt - 1) / nt, (a.M + 15) / 16), dim3(64 * nw), (size_t)nw * nt * 1024, st, a);
+  ST_LAUNCH_CHECK();
+  return ST_OK;
+}
+template <int TYPE> int q4_launch_group(const Q4Args& a, int group, hipStream_t st) {
+  return group == 32 ? q4_launch<TYPE, 4>(a, st) : group == 64 ? q4_launch<TYPE, 2>(a, st) : q4_launch<TYPE, 1>(a, st);
+}
+
+}  // namespace
+
+extern "C" size_t st_q4_packed_bytes(int N, int K, int group, int has_zeros) {
+  if (N <= 0 || K <= 0 || N > (1 << 24) || K > (1 << 24) || (group != 32 && group != 64 && group != 128)) return 0;
+  return q4_layout(N, K, group, has_zeros).total;
+}
+
+extern "C" int st_pack_weight_q4(const uint8_t* codes, const void* scales, const uint8_t* zeros, int N, int K, int group, void* out_packed,
+                                 void* stream) {
+  ST_TRY(check_q4_shape(N, K, group));
+  ST_CHECK_ARG(codes && scales && out_packed, "NULL buffer");
+  ST_CHECK_ARG(((size_t)out_packed & 15) == 0, "the packed image must lie on 16 bytes");
+  const Q4Layout y = q4_layout(N, K, group, zeros != nullptr);
+  const size_t threads = (size_t)y.nb * y.kb * 256;
+  ST_CHECK_ARG(threads / 256 < (1ull << 31), "N=%d K=%d: too large for one launch", N, K);
+  char* out = (char*)out_packed;
+  hipLaunchKernelGGL(q4_pack_kernel, dim3((unsigned)((size_t)y.nb * y.kb)), dim3(256), 0, (hipStream_t)stream, codes, (const uint16_t*)scales,
+                     zeros, N, K, group, y.nb, y.kb, (uint32_t*)out, (uint16_t*)(out + y.scales), zeros ? (uint8_t*)(out + y.zeros) : nullptr);
+  ST_LAUNCH_CHECK();
+  return ST_OK;
+}
+
+extern "C" int st_quantize_weight_q4(const float* W, int N, int K, int group, uint8_t* codes, void* scales, uint8_t* zeros, void* stream) {
+  ST_TRY(check_q4_shape(N, K, group));
+  ST_CHECK_ARG(W && codes && scales, "NULL buffer");
+  const size_t waves = (size_t)N * ((K + group - 1) / group);
+  ST_CHECK_ARG(waves / 4 < (1ull << 31) - 1, "N=%d K=%d: too large for one launch", N, K);
+  hipLaunchKernelGGL(q4_quantize_kernel, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, (hipStream_t)stream, W, N, K, group, codes,
+                     (_Float16*)scales, zeros);
+  ST_LAUNCH_CHECK();
+  return ST_OK;
+}
+
+extern "C" int st_gemm_q4(const void* x, int type, int64_t ldx, int M, const StQ4Weight* w, const float* bias, void* y, int64_t ldy,
+                          void* stream) {
+  ST_CHECK_ARG(w != nullptr, "weights struct is NULL");
+  ST_TRY(check_q4_shape(w->N, w->K, w->group));
+  ST_CHECK_ARG(type == ST_TYPE_F32 || type == ST_TYPE_BF16 || type == ST_TYPE_F16, "type=%d unknown", type);
+  ST_CHECK_ARG(M >= 0 && M <= 65535 * 16, "M=%d (0 .. %d)", M, 65535 * 16);
+  if (M == 0) return ST_OK;
+  ST_CHECK_ARG(x && w->image && y, "NULL buffer");
+  ST_CHECK_ARG(((size_t)w->image & 15) == 0, "the packed image must lie on 16 bytes");
+  const size_t size = type == ST_TYPE_F32 ? 4 : 2;
+  ST_CHECK_ARG(((size_t)x & (size - 1)) == 0 && ((size_t)y & (size - 1)) == 0, "x and y must lie on their type's size");
+  ST_CHECK_ARG(ldx >= 0 && (M == 1 || ldy >= w->N), "ldx=%lld ldy=%lld: negative, or rows of y (%d values) overlap", (long long)ldx, (long long)ldy, w->N);
+  const Q4Layout l = q4_layout(w->N, w->K, w->group, w->has_zeros);
+  Q4Args a;
+  a.x = x; a.ldx = M == 1 ? w->K : ldx; a.M = M; a.N = w->N; a.K = w->K; a.nb = l.nb; a.kb = l.kb;
+  a.codes = (const u32x4*)w->image;
+  a.scales = (const uint16_t*)((const char*)w->image + l.scales);
+  a.zeros = w->has_zeros ? (const uint8_t*)w->image + l.zeros : nullptr;
+  a.bias = bias; a.y = y; a.ldy = M == 1 ? w->N : ldy;
+  a.vec = ((size_t)x & 15) == 0 && (M == 1 || (size_t)a.ldx * size % 16 == 0);
+  hipStream_t st = (hipStream_t)stream;
+  return type == ST_TYPE_F32 ? q4_launch_group<ST_TYPE_F32>(a, w->group, st)
+         : type == ST_TYPE_BF16 ? q4_launch_group<ST_TYPE_BF16>(a, w->group, st) : q4_launch_group<ST_TYPE_F16>(a, w->group, st);
+}

@@ -230,3 +230,145 @@ def fgim_perturb(cw, latent, target, eps, want_grad=False):
     check(lib().st_fgim_perturb(C.byref(cw.c), latent.data_ptr(), target.data_ptr(), e.data_ptr(), e.numel(), B,
                                 pred.data_ptr(), _p(grad), out.data_ptr(), _stream()), "st_fgim_perturb")
     return pred, grad, out
+
+
+# ---- products with 4-bit weights, and a draw from the logits (no counterpart in the reference) -----------------------
+
+_TYPES = {torch.float32: _lib.ST_TYPE_F32, torch.bfloat16: _lib.ST_TYPE_BF16, torch.float16: _lib.ST_TYPE_F16}
+
+
+def _on(t, name, dtype, shape, device=None):
+    """a contiguous GPU tensor of this type and shape, or a ValueError that names it"""
+    if not (torch.is_tensor(t) and t.is_cuda and t.dtype == dtype and tuple(t.shape) == tuple(shape) and t.is_contiguous()):
+        raise ValueError("%s: expected a contiguous %s GPU tensor of shape %s, got %s" % (
+            name, dtype, tuple(shape), "%s %s on %s" % (t.dtype, tuple(t.shape), t.device) if torch.is_tensor(t) else type(t).__name__))
+    if device is not None and t.device != device:
+        raise ValueError("%s is on %s, not on %s" % (name, t.device, device))
+    return t
+
+
+def _rows_of(t, name):
+    """-> (type, values between rows) of a 2-d GPU tensor whose rows are contiguous"""
+    if not (torch.is_tensor(t) and t.is_cuda and t.dim() == 2 and t.dtype in _TYPES):
+        raise ValueError("%s: expected a 2-d float32, bfloat16 or float16 GPU tensor" % name)
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError("%s: the values of a row must be contiguous (stride %s)" % (name, t.stride()))
+    return _TYPES[t.dtype], t.stride(0)
+
+
+def _call(device, name, *args):
+    """one call of the library on `device`'s current stream, whichever device is current"""
+    fn = getattr(lib(), name)
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if rc != 0:
+        check(rc, name)
+
+
+class Q4Weight:
+    """A packed [N, K] weight of 4-bit codes with a scale (and a zero code) per group of columns: st_pack_weight_q4's image
+    and the struct that st_gemm_q4 takes."""
+
+    def __init__(self, image, N, K, group, has_zeros):
+        self.image, self.N, self.K, self.group = image, N, K, group
+        self.c = _lib.StQ4Weight(image.data_ptr(), N, K, group, 1 if has_zeros else 0)
+        self.ref = C.byref(self.c)
+
+
+def quantize_weight_q4(W, group=128, zero_points=False):
+    """nn.Linear weight [N, K] (f32) -> (codes u8 [N, ceil(K/2)], scales f16 [N, ceil(K/group)], zeros u8 or None):
+    scale = max |w| / 7 of the group, with zero_points (max - min) / 15; W ~ scale * (code - zero), zero = 8 when None."""
+    if not (torch.is_tensor(W) and W.is_cuda and W.dim() == 2 and W.dtype == torch.float32 and W.is_contiguous() and W.numel()):
+        raise ValueError("W: expected a contiguous 2-d float32 GPU tensor")
+    if group not in (32, 64, 128):
+        raise ValueError("group %r: expected 32, 64 or 128" % (group,))
+    N, K = W.shape
+    g = -(-K // group)
+    codes = torch.empty(N, (K + 1) // 2, dtype=torch.uint8, device=W.device)
+    scales = torch.empty(N, g, dtype=torch.float16, device=W.device)
+    zeros = torch.empty(N, g, dtype=torch.uint8, device=W.device) if zero_points else None
+    _call(W.device, "st_quantize_weight_q4", W.data_ptr(), N, K, group, codes.data_ptr(), scales.data_ptr(), _p(zeros))
+    return codes, scales, zeros
+
+
+def pack_weight_q4(codes, scales, zeros=None, k=None, group=128):
+    """4-bit codes (two a byte, even columns low), f16 group scales and zero codes of a [N, k] weight -> Q4Weight
+    (st_pack_weight_q4).  k defaults to twice the bytes of a row (give it where it is odd)."""
+    if not (torch.is_tensor(codes) and codes.is_cuda and codes.dim() == 2 and codes.dtype == torch.uint8 and codes.is_contiguous()):
+        raise ValueError("codes: expected a contiguous 2-d uint8 GPU tensor")
+    if group not in (32, 64, 128):
+        raise ValueError("group %r: expected 32, 64 or 128" % (group,))
+    N = codes.shape[0]
+    K = 2 * codes.shape[1] if k is None else int(k)
+    if K < 1 or (K + 1) // 2 != codes.shape[1]:
+        raise ValueError("codes: %d bytes a row do not hold k = %d columns" % (codes.shape[1], K))
+    shape = (N, -(-K // group))
+    _on(scales, "scales", torch.float16, shape, codes.device)
+    if zeros is not None:
+        _on(zeros, "zeros", torch.uint8, shape, codes.device)
+    nbytes = lib().st_q4_packed_bytes(N, K, group, 0 if zeros is None else 1)
+    image = torch.empty(nbytes, dtype=torch.uint8, device=codes.device)
+    _call(codes.device, "st_pack_weight_q4", codes.data_ptr(), scales.data_ptr(), _p(zeros), N, K, group, image.data_ptr())
+    return Q4Weight(image, N, K, group, zeros is not None)
+
+
+def gemm_q4(x, weight, bias=None, out=None):
+    """x [M, K] (f32, bf16 or f16; rows may be strided) times a Q4Weight's transpose, plus bias f32 [N] -> [M, N] of x's type
+    (written into `out` when given: same type, rows may be strided)."""
+    kind, ldx = _rows_of(x, "x")
+    M, dev = x.shape[0], x.device
+    if x.shape[1] != weight.K:
+        raise ValueError("x has %d columns, the weight %d" % (x.shape[1], weight.K))
+    if weight.image.device != dev:
+        raise ValueError("the weight is on %s, x on %s" % (weight.image.device, dev))
+    if bias is not None:
+        _on(bias, "bias", torch.float32, (weight.N,), dev)
+    if out is None:
+        out, ldy = torch.empty(M, weight.N, dtype=x.dtype, device=dev), weight.N
+    else:
+        ldy = _rows_of(out, "out")[1]
+        if out.dtype != x.dtype or tuple(out.shape) != (M, weight.N) or out.device != dev:
+            raise ValueError("out: expected %s of shape %s on %s" % (x.dtype, (M, weight.N), dev))
+    _call(dev, "st_gemm_q4", x.data_ptr(), kind, ldx, M, weight.ref, _p(bias), out.data_ptr(), ldy)
+    return out
+
+
+def _sample_settings(B, dev, temperature, top_k, top_p, min_p):
+    """-> (StSampleSettings, what it points to); a setting is a number, or a tensor [B] (f32, top_k int32) on the GPU"""
+    s = _lib.StSampleSettings(1.0, 0, 1.0, 0.0)
+    for name, v, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if torch.is_tensor(v):
+            setattr(s, name + "_rows", _on(v, name, dtype, (B,), dev).data_ptr())
+        elif name == "top_k":
+            if int(v) != v or not 0 <= v < 1 << 31:
+                raise ValueError("top_k %r: expected a whole number, 0 for off" % (v,))
+            s.top_k = int(v)
+        else:
+            v = float(v)
+            if not (0.0 <= v < float("inf") if name == "temperature" else 0.0 < v <= 1.0 if name == "top_p" else 0.0 <= v <= 1.0):
+                raise ValueError("%s %r is out of range" % (name, v))
+            setattr(s, name, v)
+    return s
+
+
+def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, want_logp=True, ws: DecodeWorkspace = None):
+    """One token per row of logits [B, V] (f32, bf16 or f16; rows may be strided) from the uniform numbers u [B] (f32, in
+    [0, 1)) -> (ids int32 [B], logp f32 [B] or None).  Filters in the order temperature, top_k (0: off), top_p (1: off),
+    min_p (0: off); each is a number or a tensor [B].  temperature 0: argmax.  A row of -inf / NaN alone: id -1, logp -inf."""
+    kind, ld = _rows_of(logits, "logits")
+    B, V = logits.shape
+    dev = logits.device
+    if V < 1 or V > _lib.ST_SAMPLE_MAX_VOCAB:
+        raise ValueError("logits: rows of %d values (1 .. %d)" % (V, _lib.ST_SAMPLE_MAX_VOCAB))
+    _on(u, "u", torch.float32, (B,), dev)
+    s = _sample_settings(B, dev, temperature, top_k, top_p, min_p)
+    ids = torch.empty(B, dtype=torch.int32, device=dev)
+    logp = torch.empty(B, dtype=torch.float32, device=dev) if want_logp else None
+    nbytes = lib().st_sample_workspace_bytes(B, V)
+    buf = None if nbytes == 0 else ws.get(nbytes) if ws is not None else torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _call(dev, "st_sample_logits", logits.data_ptr(), kind, ld, B, V, u.data_ptr(), C.byref(s), ids.data_ptr(), _p(logp), _p(buf), nbytes)
+    return ids, logp

@@ -1,0 +1,436 @@
+"""GPU: the draw from logits (st_sample_logits) and the product with 4-bit weights (st_gemm_q4) against plain 64-bit
+implementations, one by one and in a row.
+
+Tolerances.  Token ids are exact: masks and draws are whole-number sums, and no test puts a border within 2^-40 of a draw by
+chance.  logp is one rounding to f32 (2^-24 of the value) of a logarithm whose argument is good to 1e-12.  A product is
+y (1 + r) + d: r the one rounding to y's type (half a step: 2^-24, 2^-8, 2^-11), |d| <= ((K + 64) 2^-24 + 2^-22) A + 2^-39 K max|x| max|w|
+with A = sum |x| |w|: f32 additions of K terms and of the joins, the 22 bits that an f32 x keeps, and what its row's power of
+two takes from values far below the row's largest."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+HALF_STEP = {"f32": 2.0 ** -24, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available(), "GPU tests need a visible MI355X"
+    return torch.device("cuda", 0)
+
+
+# ---- the draw ---------------------------------------------------------------------------------------------------------
+
+def plain_sample(row, u, temperature, top_k, top_p, min_p):
+    """the definition, on one row in 64 bits (settings as the 32 bits that the kernel is given)"""
+    row = row.astype(np.float64)
+    row = np.where(np.isnan(row), -np.inf, row)
+    order = np.argsort(-row, kind="stable")
+    order = order[:int((row > -np.inf).sum())]
+    if len(order) == 0:
+        return -1, -np.inf
+    top = row[order[0]]
+    if not temperature > 0:
+        return int(order[0]), 0.0
+    if top_k > 0:
+        order = order[:top_k]
+    with np.errstate(invalid="ignore"):
+        w = np.where(row[order] == top, 1.0, np.exp((row[order] - top) / np.float64(np.float32(temperature))))
+    c = np.cumsum(w)
+    keep = len(order)
+    if top_p < 1:
+        keep = int(np.searchsorted(np.concatenate(([0.0], c))[:-1], np.float64(np.float32(top_p)) * c[-1], side="left"))
+    if min_p > 0:
+        keep = min(keep, int((w >= np.float64(np.float32(min_p))).sum()))
+    keep = max(keep, 1)
+    at = min(int(np.searchsorted(c[:keep], np.float64(u) * c[keep - 1], side="right")), keep - 1)
+    return int(order[at]), math.log(w[at] / c[keep - 1])
+
+
+def check_sample(logits, u, ids, logp, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    rows, us = logits.float().cpu().numpy(), u.cpu().numpy()
+    ids, logp = ids.cpu().numpy(), None if logp is None else logp.cpu().numpy()
+    each = lambda v: v.cpu().numpy() if torch.is_tensor(v) else [v] * len(rows)  # noqa: E731
+    t, k, p, q = each(temperature), each(top_k), each(top_p), each(min_p)
+    for i, row in enumerate(rows):
+        want, lw = plain_sample(row, us[i], float(t[i]), int(k[i]), float(p[i]), float(q[i]))
+        assert ids[i] == want, "row %d of %s: id %d, want %d (u=%r, logp %r, want %r)" % (
+            i, rows.shape, ids[i], want, us[i], None if logp is None else logp[i], lw)
+        if logp is not None:
+            assert (logp[i] == lw) if math.isinf(lw) else abs(logp[i] - lw) <= 2.0 ** -24 * abs(lw) + 1e-11, (i, logp[i], lw)
+
+
+def some_logits(dev, b, v, kind, seed, spread=2.5):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    x = torch.randn(b, v, generator=g, device=dev) * (0.3 + spread * torch.rand(b, 1, generator=g, device=dev))
+    return x.to(TYPES[kind]), torch.rand(b, generator=g, device=dev), g
+
+
+SETTINGS = [dict(), dict(temperature=0.0), dict(top_k=1), dict(top_k=50), dict(top_k=1000, temperature=1.5), dict(top_p=0.9),
+            dict(top_p=0.999, temperature=0.4), dict(top_p=1e-6), dict(min_p=0.05), dict(min_p=1.0),
+            dict(temperature=0.8, top_k=40, top_p=0.95, min_p=0.02), dict(temperature=50.0, top_k=700, top_p=0.5),
+            dict(temperature=0.7, top_k=3000, top_p=0.97, min_p=1e-4), dict(temperature=1e-3, top_p=0.9)]
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("b,v", [(1, 1), (3, 2), (5, 63), (2, 64), (4, 257), (300, 100), (33, 1000), (17, 9339), (2, 19724), (3, 50001), (2, 131072)])
+def test_sample_sizes_and_settings(dev, b, v, kind):
+    from style_transfer_amd import ops
+    logits, u, _ = some_logits(dev, b, v, kind, 1000 * b + v)
+    for s in SETTINGS:
+        ids, logp = ops.sample_logits(logits, u, **s)
+        check_sample(logits, u, ids, logp, **s)
+
+
+def test_sample_many_rows(dev):
+    from style_transfer_amd import ops
+    logits, u, _ = some_logits(dev, 2100, 777, "bf16", 5)
+    for s in (dict(top_k=20, top_p=0.9), dict(top_p=0.8), dict()):
+        ids, logp = ops.sample_logits(logits, u, **s)
+        check_sample(logits, u, ids, logp, **s)
+
+
+@pytest.mark.parametrize("v", [524288, 262147])
+def test_sample_largest_vocabulary(dev, v):
+    from style_transfer_amd import ops
+    logits, u, _ = some_logits(dev, 2, v, "f32", v)
+    for s in (dict(), dict(top_k=50, top_p=0.9), dict(top_p=0.95, temperature=3.0)):
+        ids, logp = ops.sample_logits(logits, u, **s)
+        check_sample(logits, u, ids, logp, **s)
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("v", [100, 9339, 70001])
+def test_sample_ties_and_masks(dev, v, kind):
+    """rows of one value, of few values, of masked entries (-inf, the type's lowest, NaN), empty rows, infinities, -0 and 0"""
+    from style_transfer_amd import ops
+    t = TYPES[kind]
+    g = torch.Generator(device=dev).manual_seed(v)
+    rows = torch.randn(13, v, generator=g, device=dev)
+    rows[0] = 0.0
+    rows[1] = torch.randint(0, 3, (v,), generator=g, device=dev).float() * 0.5
+    rows[2, torch.rand(v, generator=g, device=dev) < 0.7] = -math.inf
+    rows[3, torch.rand(v, generator=g, device=dev) < 0.7] = float("nan")
+    rows[4] = -math.inf
+    rows[5] = float("nan")
+    rows[6] = torch.finfo(t).min
+    rows[7, 1:] = torch.finfo(t).min
+    rows[8, :] = -math.inf
+    rows[8, v - 1] = -3.0
+    rows[9, torch.rand(v, generator=g, device=dev) < 0.2] = math.inf
+    rows[10] = torch.where(torch.rand(v, generator=g, device=dev) < 0.5, -0.0, 0.0)
+    rows[11] = torch.finfo(t).max
+    rows[11, ::2] = torch.finfo(t).min
+    rows[12] = 40 * rows[12]
+    logits = rows.to(t)
+    u = torch.rand(13, generator=g, device=dev)
+    for s in SETTINGS:
+        for uu in (u, torch.zeros_like(u), torch.full_like(u, 1 - 2.0 ** -24)):
+            ids, logp = ops.sample_logits(logits, uu, **s)
+            check_sample(logits, uu, ids, logp, **s)
+
+
+def test_sample_settings_by_row(dev):
+    from style_transfer_amd import ops
+    b, v = 96, 5003
+    logits, u, g = some_logits(dev, b, v, "f32", 3)
+    pick = lambda vals, dt: torch.tensor(vals, dtype=dt, device=dev)[torch.randint(0, len(vals), (b,), generator=g, device=dev)]  # noqa: E731
+    s = dict(temperature=pick([0.0, 0.3, 1.0, 2.0], torch.float32), top_k=pick([0, 1, 7, 50, 900, 5003, 100000], torch.int32),
+             top_p=pick([0.1, 0.5, 0.9, 1.0], torch.float32), min_p=pick([0.0, 0.01, 0.3], torch.float32))
+    ids, logp = ops.sample_logits(logits, u, **s)
+    check_sample(logits, u, ids, logp, **s)
+    # values that scalars are refused for: as documented for arrays
+    odd = dict(temperature=torch.tensor([-1.0, float("nan"), 1.0, 1.0, 1.0, 1.0], device=dev),
+               top_k=torch.tensor([0, 0, -5, 0, 0, 0], dtype=torch.int32, device=dev),
+               top_p=torch.tensor([1.0, 1.0, float("nan"), 0.0, 2.0, 1.0], device=dev),
+               min_p=torch.tensor([0.0, 0.0, float("nan"), 0.0, -1.0, 2.0], device=dev))
+    plain = dict(temperature=torch.tensor([0.0, 0.0, 1.0, 1.0, 1.0, 1.0]), top_k=torch.tensor([0, 0, 0, 1, 0, 1]),
+                 top_p=torch.ones(6), min_p=torch.zeros(6))
+    ids, logp = ops.sample_logits(logits[:6], u[:6], **odd)
+    check_sample(logits[:6], u[:6], ids, logp, **plain)
+
+
+def test_sample_strides_and_alignment(dev):
+    from style_transfer_amd import ops
+    for kind in sorted(TYPES):
+        wide, u, _ = some_logits(dev, 9, 4000, kind, 11)
+        for view in (wide[:, 1:3001], wide[:, 3:3002], wide[::2, 5:], wide[:1].expand(9, 4000), wide.t().contiguous().t()[:, :1]):
+            ids, logp = ops.sample_logits(view, u[:view.shape[0]].contiguous(), top_k=30, top_p=0.9)
+            check_sample(view, u, ids, logp, top_k=30, top_p=0.9)
+            ids, logp = ops.sample_logits(view, u[:view.shape[0]].contiguous(), temperature=1.3)
+            check_sample(view, u, ids, logp, temperature=1.3)
+
+
+def test_sample_far_rows(dev):
+    """a row that begins past 2^32 bytes"""
+    from style_transfer_amd import ops
+    v, b = 65536, 20000
+    big = torch.zeros(b * v, dtype=torch.bfloat16, device=dev).view(b, v)
+    big[b - 1] = torch.randn(v, device=dev).to(torch.bfloat16)
+    u = torch.rand(3, device=dev)
+    rows = big[[0]].expand(1, v)
+    ids, logp = ops.sample_logits(big[b - 3:], u, top_p=0.9)
+    check_sample(big[b - 3:], u, ids, logp, top_p=0.9)
+    far = big[::b - 1]
+    ids, logp = ops.sample_logits(far, u[:2].contiguous(), top_k=10)
+    check_sample(far, u[:2], ids, logp, top_k=10)
+    del rows
+
+
+def test_sample_repeats_and_streams(dev):
+    """the same answer on every run, on another stream, captured and replayed between eager calls on other inputs"""
+    from style_transfer_amd import ops
+    sets = [some_logits(dev, 40, 30001, "f32", s)[:2] for s in (1, 2, 3)]
+    s = dict(temperature=1.1, top_k=0, top_p=0.95)
+    want = [ops.sample_logits(l, u, **s) for l, u in sets]
+    for l, u in sets:
+        check_sample(l, u, *ops.sample_logits(l, u, **s), **s)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [ops.sample_logits(l, u, **s) for l, u in sets]
+    torch.cuda.current_stream().wait_stream(side)
+    for (a, b), (c, d) in zip(want, got):
+        assert torch.equal(a, c) and torch.equal(b, d)
+    l0, u0 = sets[0][0].clone(), sets[0][1].clone()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.sample_logits(l0, u0, **s)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.sample_logits(l0, u0, **s)
+    for i in (0, 1, 2, 1, 0):
+        l0.copy_(sets[i][0]), u0.copy_(sets[i][1])
+        graph.replay()
+        eager = ops.sample_logits(sets[(i + 1) % 3][0], sets[(i + 1) % 3][1], **s)
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], want[i][0]) and torch.equal(out[1], want[i][1])
+        assert torch.equal(eager[0], want[(i + 1) % 3][0])
+
+
+def test_sample_refusals(dev):
+    from style_transfer_amd import ops
+    logits, u, _ = some_logits(dev, 4, 100, "f32", 1)
+    for bad in (dict(temperature=-0.1), dict(temperature=float("inf")), dict(temperature=float("nan")), dict(top_k=-1), dict(top_k=2.5),
+                dict(top_p=0.0), dict(top_p=1.1), dict(min_p=-0.1), dict(min_p=1.5), dict(top_k=torch.ones(4, device=dev)),
+                dict(top_p=torch.ones(3, device=dev)), dict(min_p=torch.ones(4))):
+        with pytest.raises(ValueError):
+            ops.sample_logits(logits, u, **bad)
+    for l, uu in ((logits.double(), u), (logits.t(), u), (logits[0], u), (logits, u[:3]), (logits, u.half()), (logits.cpu(), u),
+                  (logits, u.cpu()), (logits[:, :0], u)):
+        with pytest.raises(ValueError):
+            ops.sample_logits(l, uu)
+    ids, logp = ops.sample_logits(logits[:0], u[:0])
+    assert ids.shape == (0,) and logp.shape == (0,)
+    assert ops.sample_logits(logits, u, want_logp=False)[1] is None
+
+
+# ---- the product ------------------------------------------------------------------------------------------------------
+
+def codes_of(packed, k):
+    c = packed.cpu().numpy()
+    return np.stack((c & 15, c >> 4), 2).reshape(c.shape[0], -1)[:, :k].astype(np.float64)
+
+
+def weight_of(codes, scales, zeros, k, group):
+    full = lambda a: np.repeat(a.cpu().numpy().astype(np.float64), group, 1)[:, :k]  # noqa: E731
+    return (codes_of(codes, k) - (8.0 if zeros is None else full(zeros))) * full(scales)
+
+
+def some_weight(dev, n, k, group, zeros, seed):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    groups = -(-k // group)
+    codes = torch.randint(0, 256, (n, (k + 1) // 2), generator=g, device=dev, dtype=torch.uint8)
+    scales = (0.01 * (0.1 + torch.rand(n, groups, generator=g, device=dev))).half()
+    z = torch.randint(0, 16, (n, groups), generator=g, device=dev, dtype=torch.uint8) if zeros else None
+    return codes, scales, z, g
+
+
+def check_product(x, w, bias, y, kind):
+    x64, y = x.float().cpu().numpy().astype(np.float64), y.float().cpu().numpy().astype(np.float64)
+    b64 = 0.0 if bias is None else bias.cpu().numpy().astype(np.float64)
+    want = x64 @ w.T + b64
+    A = np.abs(x64) @ np.abs(w).T + np.abs(b64)
+    k = x64.shape[1]
+    tol = ((k + 64) * 2.0 ** -24 + 2.0 ** -22) * A + 2.0 ** -39 * k * np.abs(x64).max(1, keepdims=True) * np.abs(w).max() + 1e-37
+    tol = HALF_STEP[kind] * (np.abs(want) + tol) + tol + (2.0 ** -25 if kind == "f16" else 0.0)   # f16's subnormal step, halved
+    far = np.abs(y - want) - tol
+    at = np.unravel_index(np.argmax(far), far.shape)
+    assert far[at] <= 0, "%s: %r, want %r, may differ by %.3g" % (at, y[at], want[at], tol[at])
+    if kind == "f32":
+        # and as a whole: K / 32 partial products are added one by one, each addition at random up to 2^-24 of the sum so far, which
+        # is of the size sqrt(sum x^2 w^2) where signs are mixed and grows up to |y| where they are not (a row of one sign: 301
+        # values of 1.2 make 364, whose own rounding is 2^-25 of 364 and 2^-20 of its sqrt(sum x^2 w^2)): sqrt(K / 32) 2^-24 of
+        # both, 2^-20 for K up to 8192
+        size = np.linalg.norm(np.sqrt((x64 ** 2) @ (w ** 2).T) + np.abs(b64) + np.abs(want))
+        off = np.linalg.norm(y - want)
+        assert off <= 2.0 ** -20 * size, "norm of the error %.3g at a size of %.3g" % (off, size)
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("m,n,k,group,zeros,bias", [
+    (1, 1, 1, 32, False, False), (1, 16, 128, 128, True, True), (2, 17, 33, 32, True, False), (3, 100, 200, 64, False, True),
+    (16, 256, 256, 64, True, True), (17, 250, 257, 128, True, True), (31, 64, 1024, 128, False, False), (33, 129, 777, 64, True, True),
+    (64, 1000, 96, 32, False, True), (65, 333, 640, 32, True, False), (128, 257, 2049, 128, False, True), (200, 1040, 500, 64, True, True),
+    (1, 9339, 256, 32, False, True), (5, 2050, 4096, 128, True, False), (300, 515, 130, 32, False, True), (257, 4100, 1030, 128, True, True)])
+def test_gemm_q4(dev, m, n, k, group, zeros, bias, kind):
+    from style_transfer_amd import ops
+    codes, scales, z, g = some_weight(dev, n, k, group, zeros, m + n + k)
+    x = torch.randn(m, k, generator=g, device=dev).to(TYPES[kind])
+    b = torch.randn(n, generator=g, device=dev) if bias else None
+    q = ops.pack_weight_q4(codes, scales, z, k=k, group=group)
+    y = ops.gemm_q4(x, q, b)
+    assert y.dtype == x.dtype and y.shape == (m, n)
+    check_product(x, weight_of(codes, scales, z, k, group), b, y, kind)
+    assert torch.equal(y, ops.gemm_q4(x, q, b))
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("m", [1, 7, 70, 300])
+def test_gemm_q4_strides(dev, m, kind):
+    """rows of x and y that are apart, that begin off 16 bytes, one row for all; what lies between y's rows stays"""
+    from style_transfer_amd import ops
+    n, k = 333, 200
+    codes, scales, z, g = some_weight(dev, n, k, 64, True, 5)
+    q, w = ops.pack_weight_q4(codes, scales, z, group=64), weight_of(codes, scales, z, k, 64)
+    wide = torch.randn(m, 408, generator=g, device=dev).to(TYPES[kind])
+    for x in (wide[:, :200], wide[:, 8:208], wide[:, 1:201], wide[:1, 4:204].expand(m, 200)):
+        check_product(x, w, None, ops.gemm_q4(x, q), kind)
+        store = torch.full((m + 1, 350), 7.0, device=dev, dtype=x.dtype)
+        assert ops.gemm_q4(x, q, out=store[:m, 3:336]) is not None
+        check_product(x, w, None, store[:m, 3:336], kind)
+        assert bool((store[:, :3] == 7).all()) and bool((store[:, 336:] == 7).all()) and bool((store[m] == 7).all())
+
+
+@pytest.mark.parametrize("m", [2, 40, 130])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_gemm_q4_range(dev, m, kind):
+    """rows of very small, very large and very unequal values; a row of zeros; infinities and NaN stay in their row"""
+    from style_transfer_amd import ops
+    n, k = 96, 640
+    codes, scales, z, g = some_weight(dev, n, k, 128, False, 9)
+    q, w = ops.pack_weight_q4(codes, scales, z), weight_of(codes, scales, z, k, 128)
+    x = torch.randn(m, k, generator=g, device=dev)
+    for scale in (1e-30, 1e-12, 1e6, 1e30):
+        y = (x * scale).to(TYPES[kind])
+        check_product(y, w, None, ops.gemm_q4(y, q), kind)
+    y = x * torch.exp(8 * torch.randn(m, k, generator=g, device=dev))
+    y[1] = 0
+    y = y.to(TYPES[kind])
+    check_product(y, w, None, ops.gemm_q4(y, q), kind)
+    bad = x.clone()
+    bad[0, 3], bad[1, 500] = math.inf, float("nan")
+    y = ops.gemm_q4(bad.to(TYPES[kind]), q)
+    assert not bool(torch.isfinite(y[:2].float()).any()) and bool(torch.isfinite(y[2:].float()).all())
+    if m > 2:
+        check_product(bad[2:].to(TYPES[kind]), w, None, y[2:], kind)
+
+
+def test_gemm_q4_far_weights(dev):
+    """an image of more than 2^32 codes' bytes is out of reach here, one whose codes pass 2^31 in number is not"""
+    from style_transfer_amd import ops
+    n, k, m = 131072 + 5, 16384 + 64, 2
+    codes, scales, z, g = some_weight(dev, n, k, 128, False, 2)
+    x = torch.randn(m, k, generator=g, device=dev).to(torch.bfloat16)
+    y = ops.gemm_q4(x, ops.pack_weight_q4(codes, scales, z, k=k))
+    for part in (slice(0, 40), slice(n - 40, n)):
+        check_product(x, weight_of(codes[part], scales[part], None, k, 128), None, y[:, part], "bf16")
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_quantize_weight_q4(dev, group, zeros):
+    """every weight within half a step of its code's value (a step: the scale), plus the scale's own rounding to f16 times the
+    largest code; exact codes against the definition"""
+    from style_transfer_amd import ops
+    n, k = 37, 301
+    g = torch.Generator(device=dev).manual_seed(group)
+    W = torch.randn(n, k, generator=g, device=dev) * 0.1
+    W[3] = 0
+    W[4, :group] = 0.7
+    W[5] = W[5].abs() + 1.0
+    codes, scales, z = ops.quantize_weight_q4(W, group, zeros)
+    assert (z is not None) == zeros
+    w, want = weight_of(codes, scales, z, k, group), W.cpu().numpy().astype(np.float64)
+    s = np.repeat(scales.cpu().numpy().astype(np.float64), group, 1)[:, :k]
+    assert (np.abs(w - want) <= 0.5 * s * (1 + 2.0 ** -20) + 15 * s * 2.0 ** -11 + (0.5 * s if zeros else 0)).all()
+    assert (w[3] == 0).all()
+    if not zeros:
+        a = np.abs(want)
+        for i in range(0, k, group):
+            step = (a[:, i:i + group].max(1).astype(np.float32) / np.float32(7)).astype(np.float16)
+            assert np.array_equal(step, scales[:, i // group].cpu().numpy())
+    y = ops.gemm_q4(W[:9].contiguous(), ops.pack_weight_q4(codes, scales, z, k=k, group=group))
+    check_product(W[:9], w, None, y, "f32")
+
+
+def test_gemm_q4_graph_and_stream(dev):
+    from style_transfer_amd import ops
+    codes, scales, z, g = some_weight(dev, 1000, 512, 64, True, 4)
+    q = ops.pack_weight_q4(codes, scales, z, group=64)
+    for m in (3, 150):
+        xs = [torch.randn(m, 512, generator=g, device=dev) for _ in range(3)]
+        want = [ops.gemm_q4(x, q) for x in xs]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = [ops.gemm_q4(x, q) for x in xs]
+        torch.cuda.current_stream().wait_stream(side)
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+        x0 = xs[0].clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = ops.gemm_q4(x0, q)
+        for i in (0, 2, 1, 0):
+            x0.copy_(xs[i])
+            graph.replay()
+            again = ops.gemm_q4(xs[(i + 1) % 3], q)
+            torch.cuda.synchronize()
+            assert torch.equal(y, want[i]) and torch.equal(again, want[(i + 1) % 3])
+
+
+def test_q4_refusals(dev):
+    from style_transfer_amd import ops
+    codes, scales, z, g = some_weight(dev, 40, 128, 64, True, 1)
+    q = ops.pack_weight_q4(codes, scales, z, group=64)
+    x = torch.randn(4, 128, device=dev)
+    for args, kw in (((codes, scales), dict(group=48)), ((codes, scales), dict(group=128)), ((codes, scales.float()), dict(group=64)),
+                     ((codes, scales, z[:, :1]), dict(group=64)), ((codes.cpu(), scales), dict(group=64)), ((codes, scales), dict(group=64, k=200)),
+                     ((codes.t(), scales), dict(group=64)), ((codes, scales, z.cpu()), dict(group=64))):
+        with pytest.raises(ValueError):
+            ops.pack_weight_q4(*args, **kw)
+    for a, kw in ((x[:, :100], {}), (x.double(), {}), (x.t(), {}), (x[0], {}), (x.cpu(), {}), (x, dict(bias=torch.zeros(39, device=dev))),
+                  (x, dict(bias=torch.zeros(40, device=dev).half())), (x, dict(out=torch.empty(4, 41, device=dev))),
+                  (x, dict(out=torch.empty(4, 40, device=dev).half())), (x, dict(out=torch.empty(40, 4, device=dev).t()))):
+        with pytest.raises(ValueError):
+            ops.gemm_q4(a, q, **kw)
+    for W, kw in ((x.half(), {}), (x.t(), {}), (x, dict(group=16)), (x[:0], {})):
+        with pytest.raises(ValueError):
+            ops.quantize_weight_q4(W, **kw)
+    assert ops.gemm_q4(x[:0], q).shape == (0, 40)
+
+
+# ---- in a row ---------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows", [1, 64, 200])
+def test_head_and_draw(dev, rows):
+    """quantised head -> logits -> tokens, as a decode step uses them: the draw of the very logits that the product gave"""
+    from style_transfer_amd import ops
+    V, g = 9339, torch.Generator(device=dev).manual_seed(rows)
+    W, b = torch.randn(V, 256, generator=g, device=dev) * 0.2, torch.randn(V, generator=g, device=dev) * 0.1
+    codes, scales, z = ops.quantize_weight_q4(W, 64)
+    q = ops.pack_weight_q4(codes, scales, z, group=64)
+    h, u = torch.randn(rows, 256, generator=g, device=dev), torch.rand(rows, generator=g, device=dev)
+    logits = ops.gemm_q4(h, q, b)
+    check_product(h, weight_of(codes, scales, z, 256, 64), b, logits, "f32")
+    s = dict(temperature=0.9, top_k=60, top_p=0.95)
+    ids, logp = ops.sample_logits(logits, u, **s)
+    check_sample(logits, u, ids, logp, **s)
+    ids0, _ = ops.sample_logits(logits, u, temperature=0.0)
+    assert torch.equal(ids0.long(), logits.argmax(1))
