@@ -136,6 +136,23 @@ struct Shared {
   uint32_t found_count, found_bin, n;
 };
 
+// one wave's choice among n <= 64 elements (lane i: `place`, `m`; elements of shared memory at places[] and masses[])
+template <bool BY_COUNT>
+__device__ __forceinline__ void pick_of_64(Shared& sh, const u64* places, const u64* masses, int n, u64 target, u64 before_mass, uint32_t before_count) {
+  const int lane = threadIdx.x & 63;
+  const u64 mine = lane < n ? places[lane] : ~0ull, m = lane < n ? masses[lane] : 0;
+  uint32_t c = before_count;
+  u64 b = before_mass;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const bool earlier = places[i] < mine;
+    c += earlier;
+    b += earlier ? masses[i] : 0;
+  }
+  const bool here = lane < n && (BY_COUNT ? c == target : b <= target && target < b + m);
+  if (here) sh.found_place = mine, sh.found_count = c, sh.found_mass = b;
+}
+
 __device__ __forceinline__ u64 wave_scan(u64 v, int lane) {   // inclusive
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -207,18 +224,7 @@ template <bool BY_COUNT, class E> __device__ void select(Shared& sh, u64 target,
         }
       });
       __syncthreads();
-      if (wv == 0) {
-        const u64 mine = lane < (int)n ? sh.small[lane] : ~0ull, m = lane < (int)n ? sh.digit_mass[lane] : 0;
-        uint32_t c = before_count;
-        u64 b = before_mass;
-        for (int i = 0; i < (int)n; ++i) {
-          const bool earlier = sh.small[i] < mine;
-          c += earlier;
-          b += earlier ? sh.digit_mass[i] : 0;
-        }
-        const bool here = lane < (int)n && (BY_COUNT ? c == target : b <= target && target < b + m);
-        if (here) sh.found_place = mine, sh.found_count = c, sh.found_mass = b;
-      }
+      if (wv == 0) pick_of_64<BY_COUNT>(sh, sh.small, sh.digit_mass, (int)n, target, before_mass, before_count);
       __syncthreads();
       return;
     }
@@ -306,7 +312,11 @@ __device__ void find_entry(const Row<TYPE>& r, const Bins& b, const Scale& sc, u
   const uint32_t n = sh.n;
   __syncthreads();
   const u64 rest = target - (BY_COUNT ? before_count : before_mass);
-  if (n <= room) {
+  if (n <= 64) {
+    if (threadIdx.x < n) sh.digit_mass[threadIdx.x] = mass_of(weight(sc, of_key((uint32_t)(b.list[threadIdx.x] >> 32))));
+    if (threadIdx.x < 64) pick_of_64<BY_COUNT>(sh, b.list, sh.digit_mass, (int)n, rest, 0, 0);   // one wave's own writes
+    __syncthreads();
+  } else if (n <= room) {
     select<BY_COUNT>(sh, rest, [&](auto f) {
       for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
         const u64 place = b.list[i];
@@ -353,6 +363,130 @@ __device__ __forceinline__ void answer(const SampleArgs& a, int b, int id, doubl
 __device__ __forceinline__ void answer_none(const SampleArgs& a, int b) {
   a.ids[b] = -1;
   if (a.logp) a.logp[b] = -INFINITY;
+}
+
+// list[0 .. n) in ascending order; room: its size, a power of two.  All pairs up to 256 entries, a bitonic network beyond.
+__device__ void sort_places(u64* list, int n, int room, Shared& sh) {
+  const int tid = threadIdx.x, nt = blockDim.x;
+  if (n <= 256) {
+    const int e = tid & 255, parts = nt >> 8, part = tid >> 8;
+    const u64 mine = e < n ? list[e] : 0;
+    if (tid < 256) sh.digit_count[tid] = 0;
+    __syncthreads();
+    if (e < n) {
+      uint32_t c = 0;
+#pragma unroll 4
+      for (int j = part; j < n; j += parts) c += list[j] < mine;
+      if (parts > 1) atomicAdd(&sh.digit_count[e], c);
+      else sh.digit_count[e] = c;
+    }
+    __syncthreads();
+    if (tid < n) list[sh.digit_count[tid]] = mine;
+    __syncthreads();
+    return;
+  }
+  int size = 512;
+  while (size < n) size *= 2;   // n <= room
+  for (int i = n + tid; i < size; i += nt) list[i] = ~0ull;
+  __syncthreads();
+  for (int k = 2; k <= size; k *= 2)
+    for (int j = k / 2; j > 0; j /= 2) {
+      for (int i = tid; i < size / 2; i += nt) {
+        const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
+        const u64 x = list[lo], y = list[hi];
+        if ((x > y) == ((lo & k) == 0)) list[lo] = y, list[hi] = x;
+      }
+      __syncthreads();
+    }
+}
+
+// The answer from a sorted list of the row's first n entries of the walk, where nothing after them can be kept (they are all
+// there is, or the first top_k).  cum: room for n masses; n <= 4 workgroups' threads.
+__device__ void draw_from_sorted(const SampleArgs& a, int b, const u64* list, int n, u64* cum, const Scale& sc, const Settings& o, Shared& sh) {
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, per = (n + blockDim.x - 1) / blockDim.x;
+  u64 sum = 0, over = 0;
+  for (int i = 0; i < per; ++i) {
+    const int e = tid * per + i;
+    if (e < n) {
+      const double w = weight(sc, of_key((uint32_t)(list[e] >> 32)));
+      const u64 m = mass_of(w);
+      sum += m;
+      if (w >= (double)o.min_p) over += m;
+      cum[e] = sum;
+    }
+  }
+  u64 base = wave_scan(sum, lane);
+  if (lane == 63) sh.wave_u64[wv] = base;
+  base -= sum;
+  __syncthreads();
+  u64 S = 0;
+  for (int i = 0; i < (int)(blockDim.x >> 6); ++i) {
+    if (i < wv) base += sh.wave_u64[i];
+    S += sh.wave_u64[i];
+  }
+  auto at_mass = [&](u64 t, auto f) {   // f(entry, mass up to and with it) for the entry at which the mass exceeds t
+    u64 before = base;
+    for (int i = 0; i < per; ++i) {
+      const int e = tid * per + i;
+      if (e < n) {
+        const u64 upto = base + cum[e];
+        if (before <= t && t < upto) f(e, upto);
+        before = upto;
+      }
+    }
+  };
+  if (o.top_p < 1.0f) {
+    at_mass(nucleus_target(o.top_p, S), [&](int, u64 upto) { sh.found_mass = upto; });
+    __syncthreads();
+    S = sh.found_mass;
+  }
+  if (o.min_p > 0.0f) {
+    over = block_sum(over, sh);
+    if (over < S) S = over;
+  }
+  if (S < ONE_MASS) S = ONE_MASS;   // the largest entry stays whatever is asked
+  at_mass(draw_target(o.u, S), [&](int e, u64) { answer(a, b, (int)(uint32_t)list[e], weight(sc, of_key((uint32_t)(list[e] >> 32))), S); });
+}
+
+// The entries that can be among the k largest: every thread has its largest entry, and the k-th largest of those is no larger
+// than the k-th largest of all.  256 bins over the threads' largest find it; entries of its bin and of those above it go to the
+// list, unsorted.  -> how many (more than `room`: the list is not complete, or fewer than k threads have an entry)
+template <int TYPE, bool LOCAL>
+__device__ uint32_t gather_top(const Row<TYPE>& r, int k, float top, float own_max, u64* list, uint32_t room, int index0, Shared& sh) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  float lowest = own_max > -INFINITY ? -own_max : -INFINITY, unused = 0.0f;
+  block_max2(lowest, unused, sh);
+  const float per_unit = 255.0f / fmaxf(top + lowest, 1e-30f);
+  auto bin = [&](float l) { return l == top ? 0 : (int)fminf((top - l) * per_unit, 255.0f); };
+  for (int i = tid; i < 256; i += blockDim.x) sh.digit_count[i] = 0;
+  if (tid == 0) sh.n = 0, sh.found_bin = 256;
+  __syncthreads();
+  if (own_max > -INFINITY) atomicAdd(&sh.digit_count[bin(own_max)], 1u);
+  __syncthreads();
+  if (tid < 64) {
+    uint32_t c[4], before = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = sh.digit_count[4 * lane + i], before += c[i];
+    before = wave_scan(before, lane) - before;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (before < (uint32_t)k && (uint32_t)k <= before + c[i]) sh.found_bin = 4 * lane + i;
+      before += c[i];
+    }
+  }
+  __syncthreads();
+  const int cut = (int)sh.found_bin;
+  if (cut >= 256) return room + 1;
+  each_entry<TYPE, LOCAL>(r, [&](float l, int i) {
+    if (bin(l) <= cut) {
+      const uint32_t at = atomicAdd(&sh.n, 1u);
+      if (at < room) list[at] = place_of(l, index0 + i);
+    }
+  });
+  __syncthreads();
+  const uint32_t n = sh.n;
+  __syncthreads();
+  return n;
 }
 
 // Any settings: masses (and counts, where a rank is asked for) of the bins in one pass over the row, then each question goes to
@@ -453,6 +587,7 @@ template <int TYPE, bool LOCAL> __global__ __launch_bounds__(1024) void sample_r
     }
   }
   r.local = local;
+  const float own_max = top;
   block_max2(top, low, sh);   // its barriers make the copy visible
   if (top == -INFINITY) {
     if (tid == 0) answer_none(a, b);
@@ -471,6 +606,26 @@ template <int TYPE, bool LOCAL> __global__ __launch_bounds__(1024) void sample_r
   }
   const float temp = fminf(o.temp, 3.4e38f);
   const Scale sc = {top, 1.4426950408889634 / (double)temp};
+  // few entries, or few that can be kept: sort them
+  const int room = nbin / 2;
+  if (a.V <= room || (o.top_k > 0 && o.top_k <= (int)blockDim.x / 2)) {
+    uint32_t n;
+    if (a.V <= room) {
+      if (tid == 0) sh.n = 0;
+      __syncthreads();
+      each_entry<TYPE, LOCAL>(r, [&](float l, int i) { bins.list[atomicAdd(&sh.n, 1u)] = place_of(l, i); });
+      __syncthreads();
+      n = sh.n;
+      __syncthreads();
+    } else {
+      n = gather_top<TYPE, LOCAL>(r, o.top_k, top, own_max, bins.list, room, 0, sh);
+    }
+    if (n <= (uint32_t)room) {
+      sort_places(bins.list, (int)n, room, sh);
+      draw_from_sorted(a, b, bins.list, o.top_k > 0 ? min((int)n, o.top_k) : (int)n, bins.mass, sc, o, sh);
+      return;
+    }
+  }
   // bins down to 32 temperatures under the top (e^-32 < 2^-45: no mass beyond), or to the lowest logit if that is nearer
   bins.top = top;
   bins.per_unit = (float)nbin / fmaxf(fminf(32.0f * temp, top + low), 1e-30f);
@@ -485,7 +640,7 @@ template <int TYPE, bool LOCAL> int launch_rows(const SampleArgs& a, int nbin, i
 }
 template <int TYPE> int launch_type(const SampleArgs& a, hipStream_t st) {
   const size_t row = ((size_t)a.V * sizeof(typename LOf<TYPE>::t) + 31) / 16 * 16;
-  const int nbin = a.V <= 16384 ? 1024 : a.V <= 65536 ? 2048 : 4096;
+  const int nbin = a.V <= 1024 ? 2048 : a.V <= 16384 ? 1024 : a.V <= 65536 ? 2048 : 4096;
   const int threads = a.V <= 2048 ? 256 : a.B >= 1024 && a.V <= 16384 ? 512 : 1024;
   const size_t lds = (size_t)nbin * 12;
   if (lds + row <= 128 * 1024) return launch_rows<TYPE, true>(a, nbin, threads, lds + row, st);
