@@ -13,6 +13,10 @@
 
 namespace {
 
+// Everything below is inlined into its kernel and shared memory is reached by its own instructions: passing it to functions by
+// reference makes flat accesses of it, and code of many times the size.
+#define SM_INLINE __attribute__((always_inline))
+
 typedef unsigned long long u64;
 
 constexpr double ONE = 17592186044416.0;   // 2^44
@@ -23,10 +27,12 @@ template <int TYPE> struct LOf;
 template <> struct LOf<ST_TYPE_F32> { typedef float t; };
 template <> struct LOf<ST_TYPE_BF16> { typedef uint16_t t; };
 template <> struct LOf<ST_TYPE_F16> { typedef _Float16 t; };
+template <int TYPE> __device__ __forceinline__ float raw_logit(typename LOf<TYPE>::t v) {
+  if constexpr (TYPE == ST_TYPE_BF16) return __uint_as_float((uint32_t)v << 16);
+  else return (float)v;
+}
 template <int TYPE> __device__ __forceinline__ float logit(typename LOf<TYPE>::t v) {   // -inf: no entry (a NaN is none either)
-  float f;
-  if constexpr (TYPE == ST_TYPE_BF16) f = __uint_as_float((uint32_t)v << 16);
-  else f = (float)v;
+  const float f = raw_logit<TYPE>(v);
   return f == f ? f : -INFINITY;
 }
 template <int TYPE> __device__ __forceinline__ typename LOf<TYPE>::t no_entry() {
@@ -49,6 +55,7 @@ struct Scale {
 // exp((l - top) / T) to about 2^-43 of the value: 2^y with y = n + f, |f| <= 1/2, the series of 2^f to the 11th power (the 12th
 // term is below 1e-14).  Half the instructions of the library's exp, which is good to the last bit.
 __device__ __forceinline__ double weight(const Scale& c, float l) {
+#pragma clang fp contract(off)   // the same value wherever it is computed: bins and the entries found in them have to agree
   double y = l == c.top ? 0.0 : ((double)l - (double)c.top) * c.inv_t;
   y = fmax(y, -1000.0);
   const double n = rint(y), f = y - n;
@@ -72,86 +79,82 @@ __device__ __forceinline__ u64 mass_of(double w) {
 }
 
 // ---- the row ---------------------------------------------------------------------------------------------------------------
-// 16-byte chunks on the row's own alignment: chunk c holds the entries c * EPC - pad + 0..EPC-1, of which those outside the row
-// read as no entry.  Either in global memory, where only a chunk that lies in the row is loaded at once, or copied to shared memory.
-template <int TYPE> struct Chunk {
-  typedef typename LOf<TYPE>::t T;
-  static constexpr int EPC = 16 / sizeof(T);
-  T v[EPC];
-};
+// 16-byte chunks on the row's own alignment: chunk c holds the entries c * EPC - pad + 0..EPC-1.
 template <int TYPE> struct Row {
   typedef typename LOf<TYPE>::t T;
-  static constexpr int EPC = Chunk<TYPE>::EPC;
+  static constexpr int EPC = 16 / sizeof(T);
   const T* p;          // entry 0
-  const void* local;   // shared memory, or null
   int n, pad, chunks;
-  __device__ Row(const T* p_, int n_) : p(p_), local(nullptr), n(n_) {
+  __device__ __forceinline__ Row(const T* p_, int n_) : p(p_), n(n_) {
     pad = (int)(((size_t)p & 15) / sizeof(T));
     chunks = (n + pad + EPC - 1) / EPC;
   }
-  __device__ __forceinline__ Chunk<TYPE> global(int c) const {
-    Chunk<TYPE> k;
-    const int i0 = c * EPC - pad;
-    if (i0 >= 0 && i0 + EPC <= n) {
-      *(f32x4*)k.v = *(const f32x4*)(p + i0);
+  __device__ __forceinline__ T entry(f32x4 k, int j) const {
+    if constexpr (TYPE == ST_TYPE_F32) return k[j];
+    else if constexpr (TYPE == ST_TYPE_F16) return __builtin_bit_cast(h8, k)[j];
+    else return (uint16_t)(__float_as_uint(k[j >> 1]) >> (16 * (j & 1)));
+  }
+  // a chunk that sticks out of the row, put together from single entries
+  __device__ __forceinline__ f32x4 edge(int c) const {
+    f32x4 k;
+    if constexpr (TYPE == ST_TYPE_F32) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = c * 4 - pad + j;
+        k[j] = i >= 0 && i < n ? p[i] : -INFINITY;
+      }
     } else {
 #pragma unroll
-      for (int j = 0; j < EPC; ++j) k.v[j] = i0 + j >= 0 && i0 + j < n ? p[i0 + j] : no_entry<TYPE>();
+      for (int j = 0; j < 4; ++j) {
+        uint32_t w = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int i = c * 8 - pad + 2 * j + h;
+          const uint32_t v = i >= 0 && i < n ? (uint32_t)((const uint16_t*)p)[i] : TYPE == ST_TYPE_F16 ? 0xfc00u : 0xff80u;   // -inf
+          w |= v << (16 * h);
+        }
+        k[j] = __uint_as_float(w);
+      }
     }
     return k;
   }
-  template <bool LOCAL> __device__ __forceinline__ Chunk<TYPE> chunk(int c) const {
+  // f(chunk, number) for this thread's chunks, from global memory: two loads under way at a time
+  template <class F> __device__ __forceinline__ void each_global(F f) const {
+    const int first = pad ? 1 : 0, last = (n + pad) / EPC, nt = blockDim.x;   // [first, last): in the row as a whole
+    const f32x4* q = (const f32x4*)(p - pad);
+#pragma unroll 1
+    for (int c = first + (int)threadIdx.x; c < last; c += 2 * nt) {
+      const bool two = c + nt < last;
+      const f32x4 a = q[c], b = q[two ? c + nt : c];
+      f(a, c);
+      if (two) f(b, c + nt);
+    }
+    const int t = nt - 1 - (int)threadIdx.x;   // the last threads have the least to do
+    const int c = t == 0 && first ? 0 : t == 1 && last >= first && last < chunks ? last : -1;
+    if (c >= 0) f(edge(c), c);
+  }
+  // the same from the copy in shared memory (LOCAL), or from global memory again
+  template <bool LOCAL, class F> __device__ __forceinline__ void each(const f32x4* local, F f) const {
     if constexpr (LOCAL) {
-      Chunk<TYPE> k;
-      *(f32x4*)k.v = ((const f32x4*)local)[c];
-      return k;
+#pragma unroll 1
+      for (int c = threadIdx.x; c < chunks; c += blockDim.x) f(local[c], c);
     } else {
-      return global(c);
+      each_global(f);
     }
   }
+  __device__ __forceinline__ int index(int c, int j) const { return c * EPC + j - pad; }
 };
-// f(logit, index) for this thread's share of the entries above -inf
-template <int TYPE, bool LOCAL, class F> __device__ __forceinline__ void each_entry(const Row<TYPE>& r, F f) {
-  constexpr int EPC = Row<TYPE>::EPC;
-#pragma unroll 2
-  for (int c = threadIdx.x; c < r.chunks; c += blockDim.x) {
-    const Chunk<TYPE> k = r.template chunk<LOCAL>(c);
-#pragma unroll
-    for (int j = 0; j < EPC; ++j) {
-      const float l = logit<TYPE>(k.v[j]);
-      if (l > -INFINITY) f(l, c * EPC + j - r.pad);
-    }
-  }
-}
 
 // ---- sums over the workgroup ---------------------------------------------------------------------------------------------
 struct Shared {
   u64 digit_mass[256];
   uint32_t digit_count[256];
-  u64 small[64];
-  u64 wave_u64[16];
+  u64 wave_u64[16], wave_any[16], wave_all[16];
   uint32_t wave_u32[16];
   float wave_f[32];
   u64 found_place, found_mass;
   uint32_t found_count, found_bin, n;
 };
-
-// one wave's choice among n <= 64 elements (lane i: `place`, `m`; elements of shared memory at places[] and masses[])
-template <bool BY_COUNT>
-__device__ __forceinline__ void pick_of_64(Shared& sh, const u64* places, const u64* masses, int n, u64 target, u64 before_mass, uint32_t before_count) {
-  const int lane = threadIdx.x & 63;
-  const u64 mine = lane < n ? places[lane] : ~0ull, m = lane < n ? masses[lane] : 0;
-  uint32_t c = before_count;
-  u64 b = before_mass;
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    const bool earlier = places[i] < mine;
-    c += earlier;
-    b += earlier ? masses[i] : 0;
-  }
-  const bool here = lane < n && (BY_COUNT ? c == target : b <= target && target < b + m);
-  if (here) sh.found_place = mine, sh.found_count = c, sh.found_mass = b;
-}
 
 __device__ __forceinline__ u64 wave_scan(u64 v, int lane) {   // inclusive
 #pragma unroll
@@ -189,151 +192,13 @@ __device__ __forceinline__ void block_max2(float& a, float& b, Shared& sh) {
   for (int i = 0; i < (int)(blockDim.x >> 6); ++i) a = fmaxf(a, sh.wave_f[i]), b = fmaxf(b, sh.wave_f[16 + i]);
 }
 
-// ---- the entry at which a sum passes its target ----------------------------------------------------------------------------
-// Among the elements that `each` gives (f(place, mass)), walked in the order of their places: the first at which the count (or the
-// mass) walked so far, it included, exceeds `target`.  sh.found_*: its place, and count and mass before it.  Eight bits of the
-// place a round, from the highest one in which two elements differ, until 64 elements are left for one wave.
-template <bool BY_COUNT, class E> __device__ void select(Shared& sh, u64 target, E each) {
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  u64 prefix = 0, before_mass = 0;
-  uint32_t before_count = 0;
-  int low = 64;   // the bits from `low` on are settled and equal to prefix's
-  for (;;) {
-    auto inside = [&](u64 place) { return low >= 64 || (place >> low) == (prefix >> low); };
-    // how many are left, and where they differ
-    u64 any = 0, all = ~0ull;
-    uint32_t n = 0;
-    each([&](u64 place, u64) {
-      if (inside(place)) any |= place, all &= place, ++n;
-    });
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) any |= __shfl_xor(any, o, 64), all &= __shfl_xor(all, o, 64), n += __shfl_xor(n, o, 64);
-    __syncthreads();
-    if (tid == 0) sh.n = 0;
-    if (lane == 0) sh.wave_u64[wv] = any, sh.digit_mass[wv] = all, sh.wave_u32[wv] = n;
-    __syncthreads();
-    any = 0, all = ~0ull, n = 0;
-    for (int i = 0; i < (int)(blockDim.x >> 6); ++i) any |= sh.wave_u64[i], all &= sh.digit_mass[i], n += sh.wave_u32[i];
-    __syncthreads();
-    if (n <= 64) {
-      each([&](u64 place, u64 m) {
-        if (inside(place)) {
-          const uint32_t at = atomicAdd(&sh.n, 1u);
-          sh.small[at] = place;
-          sh.digit_mass[at] = m;
-        }
-      });
-      __syncthreads();
-      if (wv == 0) pick_of_64<BY_COUNT>(sh, sh.small, sh.digit_mass, (int)n, target, before_mass, before_count);
-      __syncthreads();
-      return;
-    }
-    const int high = 64 - __clzll(any ^ all);   // above the highest bit that differs; two places are never equal
-    low = high > 8 ? high - 8 : 0;
-    prefix = high >= 64 ? 0 : (any >> high) << high;
-    auto within = [&](u64 place) { return high >= 64 || (place >> high) == (prefix >> high); };
-    for (int i = tid; i < 256; i += blockDim.x) sh.digit_mass[i] = 0, sh.digit_count[i] = 0;
-    __syncthreads();
-    each([&](u64 place, u64 m) {
-      if (within(place)) {
-        const int d = (int)(place >> low) & 255;
-        if constexpr (BY_COUNT) atomicAdd(&sh.digit_count[d], 1u);
-        atomicAdd(&sh.digit_mass[d], m);
-      }
-    });
-    __syncthreads();
-    if (wv == 0) {
-      uint32_t c[4], ct = 0;
-      u64 m[4], mt = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) c[i] = sh.digit_count[4 * lane + i], m[i] = sh.digit_mass[4 * lane + i], ct += c[i], mt += m[i];
-      ct = before_count + wave_scan(ct, lane) - ct;
-      mt = before_mass + wave_scan(mt, lane) - mt;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool here = BY_COUNT ? ct <= target && target < (u64)ct + c[i] : mt <= target && target < mt + m[i];
-        if (here) sh.found_bin = 4 * lane + i, sh.found_count = ct, sh.found_mass = mt;
-        ct += c[i];
-        mt += m[i];
-      }
-    }
-    __syncthreads();
-    prefix |= (u64)sh.found_bin << low;
-    before_count = sh.found_count;
-    before_mass = sh.found_mass;
-  }
-}
-
 // ---- bins ------------------------------------------------------------------------------------------------------------------
 // Bins of equal width in the logit, bin 0 at the top: monotone, so a bin is a stretch of the walk.
-struct Bins {
-  u64* mass;           // [n]
-  uint32_t* count;     // [n], where the list lies later
-  u64* list;           // [n / 2] places
-  int n;
-  float top, per_unit;
+struct BinMap {
+  float top, per_unit, last;   // last: the lowest bin, which takes all the rest
+  __device__ __forceinline__ float place(float l) const { return (top - l) * per_unit; }   // NaN for infinity under infinity
+  __device__ __forceinline__ int bin(float l) const { return l == top ? 0 : (int)fminf(place(l), last); }
 };
-__device__ __forceinline__ int bin_of(const Bins& b, float l) {
-  return l == b.top ? 0 : (int)fminf((b.top - l) * b.per_unit, (float)(b.n - 1));
-}
-
-// the bin at which the count (or mass) exceeds target: sh.found_bin / count / mass.  base_*: what lies before this thread's bins
-template <bool BY_COUNT> __device__ void find_bin(const Bins& b, u64 base_mass, uint32_t base_count, u64 target, Shared& sh) {
-  const int per = b.n / blockDim.x;
-  for (int i = 0; i < per; ++i) {
-    const int bin = threadIdx.x * per + i;
-    const u64 m = b.mass[bin];
-    const uint32_t c = BY_COUNT ? b.count[bin] : 0;
-    const bool here = BY_COUNT ? base_count <= target && target < (u64)base_count + c : base_mass <= target && target < base_mass + m;
-    if (here) sh.found_bin = bin, sh.found_count = base_count, sh.found_mass = base_mass;
-    base_mass += m;
-    base_count += c;
-  }
-  __syncthreads();
-}
-
-// the entry of bin sh.found_bin at which the count (or mass) exceeds target -> sh.found_*
-template <int TYPE, bool LOCAL, bool BY_COUNT>
-__device__ void find_entry(const Row<TYPE>& r, const Bins& b, const Scale& sc, u64 target, Shared& sh) {
-  const int bin = (int)sh.found_bin;
-  const u64 before_mass = sh.found_mass;
-  const uint32_t before_count = sh.found_count;
-  __syncthreads();
-  if (threadIdx.x == 0) sh.n = 0;
-  __syncthreads();
-  const uint32_t room = b.n / 2;
-  each_entry<TYPE, LOCAL>(r, [&](float l, int i) {
-    if (bin_of(b, l) == bin) {
-      const uint32_t at = atomicAdd(&sh.n, 1u);
-      if (at < room) b.list[at] = place_of(l, i);
-    }
-  });
-  __syncthreads();
-  const uint32_t n = sh.n;
-  __syncthreads();
-  const u64 rest = target - (BY_COUNT ? before_count : before_mass);
-  if (n <= 64) {
-    if (threadIdx.x < n) sh.digit_mass[threadIdx.x] = mass_of(weight(sc, of_key((uint32_t)(b.list[threadIdx.x] >> 32))));
-    if (threadIdx.x < 64) pick_of_64<BY_COUNT>(sh, b.list, sh.digit_mass, (int)n, rest, 0, 0);   // one wave's own writes
-    __syncthreads();
-  } else if (n <= room) {
-    select<BY_COUNT>(sh, rest, [&](auto f) {
-      for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
-        const u64 place = b.list[i];
-        f(place, mass_of(weight(sc, of_key((uint32_t)(place >> 32)))));
-      }
-    });
-  } else {
-    // more of the row in one bin than the list holds (equal logits, mostly): straight from the row, round by round
-    select<BY_COUNT>(sh, rest, [&](auto f) {
-      each_entry<TYPE, LOCAL>(r, [&](float l, int i) {
-        if (bin_of(b, l) == bin) f(place_of(l, i), mass_of(weight(sc, l)));
-      });
-    });
-  }
-  if (threadIdx.x == 0) sh.found_mass += before_mass, sh.found_count += before_count;
-  __syncthreads();
-}
 
 struct Settings {
   float temp, top_p, min_p, u;
@@ -360,13 +225,10 @@ __device__ __forceinline__ void answer(const SampleArgs& a, int b, int id, doubl
   a.ids[b] = id;
   if (a.logp) a.logp[b] = (float)log(w * ONE / (double)S);
 }
-__device__ __forceinline__ void answer_none(const SampleArgs& a, int b) {
-  a.ids[b] = -1;
-  if (a.logp) a.logp[b] = -INFINITY;
-}
 
-// list[0 .. n) in ascending order; room: its size, a power of two.  All pairs up to 256 entries, a bitonic network beyond.
-__device__ void sort_places(u64* list, int n, int room, Shared& sh) {
+// ---- sorted lists ----------------------------------------------------------------------------------------------------------
+// list[0 .. n) in ascending order; its size is a power of two.  All pairs up to 256 entries, a bitonic network beyond.
+__device__ __forceinline__ void sort_places(u64* list, int n, Shared& sh) {
   const int tid = threadIdx.x, nt = blockDim.x;
   if (n <= 256) {
     const int e = tid & 255, parts = nt >> 8, part = tid >> 8;
@@ -377,8 +239,7 @@ __device__ void sort_places(u64* list, int n, int room, Shared& sh) {
       uint32_t c = 0;
 #pragma unroll 4
       for (int j = part; j < n; j += parts) c += list[j] < mine;
-      if (parts > 1) atomicAdd(&sh.digit_count[e], c);
-      else sh.digit_count[e] = c;
+      atomicAdd(&sh.digit_count[e], c);
     }
     __syncthreads();
     if (tid < n) list[sh.digit_count[tid]] = mine;
@@ -386,11 +247,14 @@ __device__ void sort_places(u64* list, int n, int room, Shared& sh) {
     return;
   }
   int size = 512;
-  while (size < n) size *= 2;   // n <= room
+  while (size < n) size *= 2;
   for (int i = n + tid; i < size; i += nt) list[i] = ~0ull;
   __syncthreads();
+#pragma unroll 1
   for (int k = 2; k <= size; k *= 2)
+#pragma unroll 1
     for (int j = k / 2; j > 0; j /= 2) {
+#pragma unroll 1
       for (int i = tid; i < size / 2; i += nt) {
         const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
         const u64 x = list[lo], y = list[hi];
@@ -401,19 +265,17 @@ __device__ void sort_places(u64* list, int n, int room, Shared& sh) {
 }
 
 // The answer from a sorted list of the row's first n entries of the walk, where nothing after them can be kept (they are all
-// there is, or the first top_k).  cum: room for n masses; n <= 4 workgroups' threads.
-__device__ void draw_from_sorted(const SampleArgs& a, int b, const u64* list, int n, u64* cum, const Scale& sc, const Settings& o, Shared& sh) {
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, per = (n + blockDim.x - 1) / blockDim.x;
+// there is, or the first top_k).  cum: room for n masses.
+__device__ __forceinline__ void draw_from_sorted(const SampleArgs& a, int b, const u64* list, int n, u64* cum, const Scale& sc, const Settings& o, Shared& sh) {
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, per = (n + blockDim.x - 1) / blockDim.x, e0 = tid * per;
   u64 sum = 0, over = 0;
-  for (int i = 0; i < per; ++i) {
-    const int e = tid * per + i;
-    if (e < n) {
-      const double w = weight(sc, of_key((uint32_t)(list[e] >> 32)));
-      const u64 m = mass_of(w);
-      sum += m;
-      if (w >= (double)o.min_p) over += m;
-      cum[e] = sum;
-    }
+#pragma unroll 1
+  for (int e = e0; e < e0 + per && e < n; ++e) {
+    const double w = weight(sc, of_key((uint32_t)(list[e] >> 32)));
+    const u64 m = mass_of(w);
+    sum += m;
+    if (w >= (double)o.min_p) over += m;
+    cum[e] = sum;
   }
   u64 base = wave_scan(sum, lane);
   if (lane == 63) sh.wave_u64[wv] = base;
@@ -424,19 +286,19 @@ __device__ void draw_from_sorted(const SampleArgs& a, int b, const u64* list, in
     if (i < wv) base += sh.wave_u64[i];
     S += sh.wave_u64[i];
   }
-  auto at_mass = [&](u64 t, auto f) {   // f(entry, mass up to and with it) for the entry at which the mass exceeds t
+  // the entry of this thread, if any, at which the mass exceeds t
+  auto at_mass = [&](u64 t) SM_INLINE {
     u64 before = base;
-    for (int i = 0; i < per; ++i) {
-      const int e = tid * per + i;
-      if (e < n) {
-        const u64 upto = base + cum[e];
-        if (before <= t && t < upto) f(e, upto);
-        before = upto;
-      }
+    for (int e = e0; e < e0 + per && e < n; ++e) {
+      const u64 upto = base + cum[e];
+      if (before <= t && t < upto) return e;
+      before = upto;
     }
+    return -1;
   };
   if (o.top_p < 1.0f) {
-    at_mass(nucleus_target(o.top_p, S), [&](int, u64 upto) { sh.found_mass = upto; });
+    const int e = at_mass(nucleus_target(o.top_p, S));
+    if (e >= 0) sh.found_mass = base + cum[e];
     __syncthreads();
     S = sh.found_mass;
   }
@@ -445,77 +307,151 @@ __device__ void draw_from_sorted(const SampleArgs& a, int b, const u64* list, in
     if (over < S) S = over;
   }
   if (S < ONE_MASS) S = ONE_MASS;   // the largest entry stays whatever is asked
-  at_mass(draw_target(o.u, S), [&](int e, u64) { answer(a, b, (int)(uint32_t)list[e], weight(sc, of_key((uint32_t)(list[e] >> 32))), S); });
+  const int e = at_mass(draw_target(o.u, S));
+  if (e >= 0) answer(a, b, (int)(uint32_t)list[e], weight(sc, of_key((uint32_t)(list[e] >> 32))), S);
 }
 
-// The entries that can be among the k largest: every thread has its largest entry, and the k-th largest of those is no larger
-// than the k-th largest of all.  256 bins over the threads' largest find it; entries of its bin and of those above it go to the
-// list, unsorted.  -> how many (more than `room`: the list is not complete, or fewer than k threads have an entry)
-template <int TYPE, bool LOCAL>
-__device__ uint32_t gather_top(const Row<TYPE>& r, int k, float top, float own_max, u64* list, uint32_t room, int index0, Shared& sh) {
-  const int tid = threadIdx.x, lane = tid & 63;
-  float lowest = own_max > -INFINITY ? -own_max : -INFINITY, unused = 0.0f;
-  block_max2(lowest, unused, sh);
-  const float per_unit = 255.0f / fmaxf(top + lowest, 1e-30f);
-  auto bin = [&](float l) { return l == top ? 0 : (int)fminf((top - l) * per_unit, 255.0f); };
-  for (int i = tid; i < 256; i += blockDim.x) sh.digit_count[i] = 0;
-  if (tid == 0) sh.n = 0, sh.found_bin = 256;
-  __syncthreads();
-  if (own_max > -INFINITY) atomicAdd(&sh.digit_count[bin(own_max)], 1u);
-  __syncthreads();
-  if (tid < 64) {
-    uint32_t c[4], before = 0;
+// One workgroup a row: the row in shared memory (LOCAL), or read again for each pass.
+// Dynamic shared memory: masses of the bins [nbin], a list of places [nbin / 2] (before that, counts of the bins), the row.
+template <int TYPE, bool LOCAL> __global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs a, int nbin) {
+  typedef typename LOf<TYPE>::t T;
+  constexpr int EPC = Row<TYPE>::EPC;
+  extern __shared__ __align__(16) char dyn[];
+  __shared__ Shared sh;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, nt = blockDim.x, nw = nt >> 6;
+  if (a.n_dev && b >= *a.n_dev) return;
+  u64* const mass = (u64*)dyn;
+  u64* const list = mass + nbin;
+  uint32_t* const count = (uint32_t*)list;
+  f32x4* const local = (f32x4*)(list + nbin / 2);
+  const uint32_t room = nbin / 2;
+  const int s = a.idx ? a.idx[b] : b;
+  const Row<TYPE> r((const T*)a.logits + (size_t)b * a.ld, a.V);
+
+  float top = -INFINITY, low = -INFINITY;   // largest logit, largest negated one above -inf
+  r.each_global([&](f32x4 k, int c) SM_INLINE {
+    if constexpr (LOCAL) local[c] = k;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = sh.digit_count[4 * lane + i], before += c[i];
-    before = wave_scan(before, lane) - before;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (before < (uint32_t)k && (uint32_t)k <= before + c[i]) sh.found_bin = 4 * lane + i;
-      before += c[i];
-    }
-  }
-  __syncthreads();
-  const int cut = (int)sh.found_bin;
-  if (cut >= 256) return room + 1;
-  each_entry<TYPE, LOCAL>(r, [&](float l, int i) {
-    if (bin(l) <= cut) {
-      const uint32_t at = atomicAdd(&sh.n, 1u);
-      if (at < room) list[at] = place_of(l, index0 + i);
+    for (int j = 0; j < EPC; ++j) {
+      const float l = raw_logit<TYPE>(r.entry(k, j));
+      top = fmaxf(top, l);
+      low = fmaxf(low, l > -INFINITY ? -l : -INFINITY);
     }
   });
-  __syncthreads();
-  const uint32_t n = sh.n;
-  __syncthreads();
-  return n;
-}
+  const float own_max = top;
+  block_max2(top, low, sh);   // its barriers make the copy visible
+  if (top == -INFINITY) {
+    if (tid == 0) {
+      a.ids[b] = -1;
+      if (a.logp) a.logp[b] = -INFINITY;
+    }
+    return;
+  }
+  const Settings o = settings_of(a, s);
+  const bool greedy = !(o.temp > 0.0f) || o.top_k == 1;
+  const Scale sc = {top, 1.4426950408889634 / (double)fminf(o.temp, 3.4e38f)};
 
-// Any settings: masses (and counts, where a rank is asked for) of the bins in one pass over the row, then each question goes to
-// one bin and to one entry of it.
-template <int TYPE, bool LOCAL>
-__device__ void draw_by_bins(const SampleArgs& a, int b, const Row<TYPE>& r, Bins& bins, const Scale& sc, const Settings& o, Shared& sh) {
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, per = bins.n / blockDim.x;
-  const bool ranked = o.top_k > 0 && o.top_k < r.n;
-  for (int i = tid; i < bins.n; i += blockDim.x) {
-    bins.mass[i] = 0;
-    if (ranked) bins.count[i] = 0;
+  // ---- lists: of the largest alone (greedy), of all entries of a short row, of those that can be among the top_k.  An entry goes
+  // to the list by one comparison, (top - l) * per_unit < to.
+  const bool by_top = !greedy && o.top_k > 0 && o.top_k <= nt / 2 && a.V > 256, all = !greedy && !by_top && a.V <= (int)room;
+  if (greedy || by_top || all) {
+    float per_unit = 0.0f, to = INFINITY;   // all: every product is 0 (or NaN under an infinite top)
+    if (tid == 0) sh.n = greedy ? 0xffffffffu : 0, sh.found_bin = 256;
+    if (by_top) {
+      // every thread has its largest entry, and the k-th largest of those is no larger than the k-th largest of all: 256 bins over
+      // them, the list takes its bin and those above it
+      float lowest = own_max > -INFINITY ? -own_max : -INFINITY, unused = 0.0f;
+      block_max2(lowest, unused, sh);
+      const BinMap map = {top, 255.0f / fmaxf(top + lowest, 1e-30f), 255.0f};
+      for (int i = tid; i < 256; i += nt) sh.digit_count[i] = 0;
+      __syncthreads();
+      if (own_max > -INFINITY) atomicAdd(&sh.digit_count[map.bin(own_max)], 1u);
+      __syncthreads();
+      if (tid < 64) {
+        uint32_t c[4], before = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[i] = sh.digit_count[4 * lane + i], before += c[i];
+        before = wave_scan(before, lane) - before;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (before < (uint32_t)o.top_k && (uint32_t)o.top_k <= before + c[i]) sh.found_bin = 4 * lane + i;
+          before += c[i];
+        }
+      }
+      per_unit = map.per_unit;
+    }
+    __syncthreads();
+    const uint32_t cut = sh.found_bin;
+    if (by_top && cut < 255) to = (float)(cut + 1);
+    if (!by_top || cut < 256) {   // 256: fewer than top_k threads have an entry
+      const bool every = to == INFINITY;
+      r.template each<LOCAL>(local, [&](f32x4 k, int c) SM_INLINE {
+        uint32_t hits = 0;
+#pragma unroll
+        for (int j = 0; j < EPC; ++j) {
+          const float l = raw_logit<TYPE>(r.entry(k, j));
+          const bool in = greedy ? l == top : (every && l > -INFINITY) || (top - l) * per_unit < to || l == top;
+          hits |= (uint32_t)in << j;
+        }
+        if (hits) {
+#pragma unroll
+          for (int j = 0; j < EPC; ++j) {
+            if (!(hits >> j & 1)) continue;
+            const float l = raw_logit<TYPE>(r.entry(k, j));
+            if (greedy) {
+              atomicMin(&sh.n, (uint32_t)r.index(c, j));
+            } else if (l > -INFINITY) {
+              const uint32_t at = atomicAdd(&sh.n, 1u);
+              if (at < room) list[at] = place_of(l, r.index(c, j));
+            }
+          }
+        }
+      });
+      __syncthreads();
+      const uint32_t n = sh.n;
+      if (greedy) {
+        if (tid == 0) answer(a, b, (int)n, 1.0, ONE_MASS);
+        return;
+      }
+      __syncthreads();
+      if (n <= room) {
+        sort_places(list, (int)n, sh);
+        draw_from_sorted(a, b, list, o.top_k > 0 ? min((int)n, o.top_k) : (int)n, mass, sc, o, sh);
+        return;
+      }
+    }
+    __syncthreads();
+  }
+
+  // ---- bins, for any settings: masses (and counts, where a rank is asked for) in one pass over the row; they reach down to 32
+  // temperatures under the top (e^-32 < 2^-45: no mass beyond), or to the lowest logit if that is nearer
+  const BinMap map = {top, (float)nbin / fmaxf(fminf(32.0f * fminf(o.temp, 3.4e38f), top + low), 1e-30f), (float)(nbin - 1)};
+  const bool ranked = o.top_k > 0 && o.top_k < a.V;
+  for (int i = tid; i < nbin; i += nt) {
+    mass[i] = 0;
+    if (ranked) count[i] = 0;
   }
   __syncthreads();
   u64 over = 0;
-  const double q = o.min_p;
-  each_entry<TYPE, LOCAL>(r, [&](float l, int) {
-    const double w = weight(sc, l);
-    const u64 m = mass_of(w);
-    const int bin = bin_of(bins, l);
-    if (m) atomicAdd(&bins.mass[bin], m);
-    if (ranked) atomicAdd(&bins.count[bin], 1u);
-    if (w >= q) over += m;
+  r.template each<LOCAL>(local, [&](f32x4 k, int) SM_INLINE {
+#pragma unroll
+    for (int j = 0; j < EPC; ++j) {
+      const float l = logit<TYPE>(r.entry(k, j));
+      const double w = l > -INFINITY ? weight(sc, l) : 0.0;
+      const u64 m = mass_of(w);
+      const int bin = map.bin(l);
+      if (m) atomicAdd(&mass[bin], m);
+      if (ranked && l > -INFINITY) atomicAdd(&count[bin], 1u);
+      if (w >= (double)o.min_p) over += m;
+    }
   });
   __syncthreads();
+  const int per = nbin / nt;
   u64 base_mass = 0;
   uint32_t base_count = 0;
   for (int i = 0; i < per; ++i) {
-    base_mass += bins.mass[tid * per + i];
-    if (ranked) base_count += bins.count[tid * per + i];
+    base_mass += mass[tid * per + i];
+    if (ranked) base_count += count[tid * per + i];
   }
   const u64 own_mass = base_mass;
   const uint32_t own_count = base_count;
@@ -527,109 +463,160 @@ __device__ void draw_by_bins(const SampleArgs& a, int b, const Row<TYPE>& r, Bin
   base_count -= own_count;
   u64 S = 0;
   uint32_t entries = 0;
-  for (int i = 0; i < (int)(blockDim.x >> 6); ++i) {
+  for (int i = 0; i < nw; ++i) {
     if (i < wv) base_mass += sh.wave_u64[i], base_count += sh.wave_u32[i];
     S += sh.wave_u64[i];
     entries += sh.wave_u32[i];
   }
-  __syncthreads();
-  if (ranked && (uint32_t)o.top_k < entries) {
-    find_bin<true>(bins, base_mass, base_count, o.top_k - 1, sh);
-    find_entry<TYPE, LOCAL, true>(r, bins, sc, o.top_k - 1, sh);
-    S = sh.found_mass + mass_of(weight(sc, of_key((uint32_t)(sh.found_place >> 32))));
-    __syncthreads();
-  }
-  if (o.top_p < 1.0f) {
-    const u64 t = nucleus_target(o.top_p, S);
-    find_bin<false>(bins, base_mass, 0, t, sh);
-    find_entry<TYPE, LOCAL, false>(r, bins, sc, t, sh);
-    S = sh.found_mass + mass_of(weight(sc, of_key((uint32_t)(sh.found_place >> 32))));
-    __syncthreads();
-  }
-  if (o.min_p > 0.0f) {
-    over = block_sum(over, sh);
-    if (over < S) S = over;
-    __syncthreads();
-  }
-  if (S < ONE_MASS) S = ONE_MASS;   // the largest entry stays whatever is asked
-  const u64 t = draw_target(o.u, S);
-  find_bin<false>(bins, base_mass, 0, t, sh);
-  find_entry<TYPE, LOCAL, false>(r, bins, sc, t, sh);
-  if (tid == 0) answer(a, b, (int)(uint32_t)sh.found_place, weight(sc, of_key((uint32_t)(sh.found_place >> 32))), S);
-}
+  if (o.min_p > 0.0f) over = block_sum(over, sh);
 
-// One workgroup a row, the row in shared memory (LOCAL) or read again for each pass.
-template <int TYPE, bool LOCAL> __global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs a, int nbin) {
-  typedef typename LOf<TYPE>::t T;
-  extern __shared__ __align__(16) char dyn[];
-  __shared__ Shared sh;
-  const int b = blockIdx.x, tid = threadIdx.x;
-  if (a.n_dev && b >= *a.n_dev) return;
-  const int s = a.idx ? a.idx[b] : b;
-  Row<TYPE> r((const T*)a.logits + (size_t)b * a.ld, a.V);
-  Bins bins;
-  bins.n = nbin;
-  bins.mass = (u64*)dyn;
-  bins.list = bins.mass + nbin;
-  bins.count = (uint32_t*)bins.list;
-  f32x4* local = (f32x4*)(bins.list + nbin / 2);
-  float top = -INFINITY, low = -INFINITY;   // largest logit, largest negated finite one
-  constexpr int EPC = Row<TYPE>::EPC;
-#pragma unroll 4
-  for (int c = tid; c < r.chunks; c += blockDim.x) {
-    const Chunk<TYPE> k = r.global(c);
-    if constexpr (LOCAL) local[c] = *(const f32x4*)k.v;
-#pragma unroll
-    for (int j = 0; j < EPC; ++j) {
-      const float l = logit<TYPE>(k.v[j]);
-      top = fmaxf(top, l);
-      low = fmaxf(low, l > -INFINITY ? -l : -INFINITY);
+  // ---- three questions, each the entry at which the count or the mass of the walk exceeds a target: the top_k-th entry, the one
+  // that completes top_p, the drawn one.  First its bin, then the entry in the bin.
+#pragma unroll 1
+  for (int question = 0; question < 3; ++question) {
+    const bool by_count = question == 0;
+    u64 target;
+    if (question == 0) {
+      if (!ranked || (uint32_t)o.top_k >= entries) continue;
+      target = (u64)(o.top_k - 1);
+    } else if (question == 1) {
+      if (!(o.top_p < 1.0f)) continue;
+      target = nucleus_target(o.top_p, S);
+    } else {
+      if (o.min_p > 0.0f && over < S) S = over;
+      if (S < ONE_MASS) S = ONE_MASS;   // the largest entry stays whatever is asked
+      target = draw_target(o.u, S);
     }
-  }
-  r.local = local;
-  const float own_max = top;
-  block_max2(top, low, sh);   // its barriers make the copy visible
-  if (top == -INFINITY) {
-    if (tid == 0) answer_none(a, b);
-    return;
-  }
-  const Settings o = settings_of(a, s);
-  if (!(o.temp > 0.0f) || o.top_k == 1) {   // the first of the largest
-    if (tid == 0) sh.n = 0xffffffffu;
     __syncthreads();
-    each_entry<TYPE, LOCAL>(r, [&](float l, int i) {
-      if (l == top) atomicMin(&sh.n, (uint32_t)i);
+    {
+      u64 m0 = base_mass;
+      uint32_t c0 = base_count;
+#pragma unroll 1
+      for (int i = 0; i < per; ++i) {
+        const u64 m1 = m0 + mass[tid * per + i];
+        const uint32_t c1 = by_count ? c0 + count[tid * per + i] : 0;
+        if (by_count ? c0 <= target && target < c1 : m0 <= target && target < m1) sh.found_bin = tid * per + i, sh.found_count = c0, sh.found_mass = m0;
+        m0 = m1;
+        c0 = c1;
+      }
+    }
+    if (tid == 0) sh.n = 0;
+    __syncthreads();
+    const int bin = (int)sh.found_bin;
+    u64 before_mass = sh.found_mass;
+    uint32_t before_count = by_count ? sh.found_count : 0;
+    // the bin's entries: one list (the counts are not needed any more once the first question has its bin)
+    const float from = (float)bin, to = bin == nbin - 1 ? INFINITY : (float)(bin + 1);
+    r.template each<LOCAL>(local, [&](f32x4 k, int c) SM_INLINE {
+      uint32_t hits = 0;
+#pragma unroll
+      for (int j = 0; j < EPC; ++j) {
+        const float l = raw_logit<TYPE>(r.entry(k, j)), at = map.place(l);
+        hits |= (uint32_t)((at >= from && (at < to || to == INFINITY)) || (bin == 0 && l == top)) << j;
+      }
+      if (hits) {
+#pragma unroll
+        for (int j = 0; j < EPC; ++j) {
+          const float l = raw_logit<TYPE>(r.entry(k, j));
+          if ((hits >> j & 1) && l > -INFINITY) {
+            const uint32_t at = atomicAdd(&sh.n, 1u);
+            if (at < room) list[at] = place_of(l, r.index(c, j));
+          }
+        }
+      }
     });
     __syncthreads();
-    if (tid == 0) answer(a, b, (int)sh.n, 1.0, ONE_MASS);
-    return;
-  }
-  const float temp = fminf(o.temp, 3.4e38f);
-  const Scale sc = {top, 1.4426950408889634 / (double)temp};
-  // few entries, or few that can be kept: sort them
-  const int room = nbin / 2;
-  if (a.V <= room || (o.top_k > 0 && o.top_k <= (int)blockDim.x / 2)) {
-    uint32_t n;
-    if (a.V <= room) {
+    const uint32_t n_bin = sh.n;
+    // more of the row in one bin than the list holds (equal logits, mostly): the rounds below go over the row itself
+    const bool from_row = n_bin > room;
+    const int elements = from_row ? a.V : (int)n_bin;
+    auto place_at = [&](int i) SM_INLINE {   // ~0: none
+      if (!from_row) return list[i];
+      float l;
+      if constexpr (LOCAL) l = logit<TYPE>(((const T*)local)[i + r.pad]);
+      else l = logit<TYPE>(r.p[i]);
+      return l > -INFINITY && map.bin(l) == bin ? place_of(l, i) : ~0ull;
+    };
+    // eight bits of the place a round, from the highest one in which two elements differ, until one wave can compare the rest
+    u64 prefix = 0;
+    int high = 64;   // the bits from `high` on are settled: prefix's
+#pragma unroll 1
+    for (;;) {
+      auto inside = [&](u64 place) SM_INLINE { return place != ~0ull && (high >= 64 || (place >> high) == (prefix >> high)); };
+      u64 any = 0, every = ~0ull;
+      uint32_t n = 0;
+#pragma unroll 1
+      for (int i = tid; i < elements; i += nt) {
+        const u64 place = place_at(i);
+        if (inside(place)) any |= place, every &= place, ++n;
+      }
+#pragma unroll
+      for (int d = 32; d > 0; d >>= 1) any |= __shfl_xor(any, d, 64), every &= __shfl_xor(every, d, 64), n += __shfl_xor(n, d, 64);
+      __syncthreads();
       if (tid == 0) sh.n = 0;
+      if (lane == 0) sh.wave_any[wv] = any, sh.wave_all[wv] = every, sh.wave_u32[wv] = n;
+      for (int i = tid; i < 256; i += nt) sh.digit_mass[i] = 0, sh.digit_count[i] = 0;
       __syncthreads();
-      each_entry<TYPE, LOCAL>(r, [&](float l, int i) { bins.list[atomicAdd(&sh.n, 1u)] = place_of(l, i); });
+      any = 0, every = ~0ull, n = 0;
+      for (int i = 0; i < nw; ++i) any |= sh.wave_any[i], every &= sh.wave_all[i], n += sh.wave_u32[i];
+      const bool few = n <= 64;
+      const int top_bit = 64 - __clzll(any ^ every);   // above the highest bit that differs (two places are never equal)
+      const int low_bit = top_bit > 8 ? top_bit - 8 : 0;
+      // few: the digits' array takes the elements themselves, and their masses behind them
+#pragma unroll 1
+      for (int i = tid; i < elements; i += nt) {
+        const u64 place = place_at(i);
+        if (!inside(place)) continue;
+        if (few) {
+          const uint32_t at = atomicAdd(&sh.n, 1u);
+          sh.digit_mass[at] = place;
+          sh.digit_mass[64 + at] = mass_of(weight(sc, of_key((uint32_t)(place >> 32))));
+        } else {
+          const int d = (int)(place >> low_bit) & 255;
+          if (by_count) atomicAdd(&sh.digit_count[d], 1u);
+          atomicAdd(&sh.digit_mass[d], mass_of(weight(sc, of_key((uint32_t)(place >> 32)))));
+        }
+      }
       __syncthreads();
-      n = sh.n;
+      if (few) {
+        if (wv == 0) {
+          const u64 mine = lane < (int)n ? sh.digit_mass[lane] : ~0ull, m = lane < (int)n ? sh.digit_mass[64 + lane] : 0;
+          uint32_t c = before_count;
+          u64 mb = before_mass;
+#pragma unroll 4
+          for (int i = 0; i < (int)n; ++i) {
+            const bool earlier = sh.digit_mass[i] < mine;
+            c += earlier;
+            mb += earlier ? sh.digit_mass[64 + i] : 0;
+          }
+          if (lane < (int)n && (by_count ? c == target : mb <= target && target < mb + m)) sh.found_place = mine, sh.found_mass = mb + m;
+        }
+        __syncthreads();
+        break;
+      }
+      if (wv == 0) {
+        uint32_t c[4], ct = 0;
+        u64 m[4], mt = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[i] = sh.digit_count[4 * lane + i], m[i] = sh.digit_mass[4 * lane + i], ct += c[i], mt += m[i];
+        ct = before_count + wave_scan(ct, lane) - ct;
+        mt = before_mass + wave_scan(mt, lane) - mt;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (by_count ? ct <= target && target < ct + c[i] : mt <= target && target < mt + m[i]) sh.found_bin = 4 * lane + i, sh.found_count = ct, sh.found_mass = mt;
+          ct += c[i];
+          mt += m[i];
+        }
+      }
       __syncthreads();
-    } else {
-      n = gather_top<TYPE, LOCAL>(r, o.top_k, top, own_max, bins.list, room, 0, sh);
+      prefix = (top_bit >= 64 ? 0 : (any >> top_bit) << top_bit) | (u64)(sh.found_bin & 255) << low_bit;
+      high = low_bit;
+      before_count = sh.found_count;
+      before_mass = sh.found_mass;
     }
-    if (n <= (uint32_t)room) {
-      sort_places(bins.list, (int)n, room, sh);
-      draw_from_sorted(a, b, bins.list, o.top_k > 0 ? min((int)n, o.top_k) : (int)n, bins.mass, sc, o, sh);
-      return;
-    }
+    if (question < 2) S = sh.found_mass;
   }
-  // bins down to 32 temperatures under the top (e^-32 < 2^-45: no mass beyond), or to the lowest logit if that is nearer
-  bins.top = top;
-  bins.per_unit = (float)nbin / fmaxf(fminf(32.0f * temp, top + low), 1e-30f);
-  draw_by_bins<TYPE, LOCAL>(a, b, r, bins, sc, o, sh);
+  if (tid == 0) answer(a, b, (int)(uint32_t)sh.found_place, weight(sc, of_key((uint32_t)(sh.found_place >> 32))), S);
 }
 
 template <int TYPE, bool LOCAL> int launch_rows(const SampleArgs& a, int nbin, int threads, size_t lds, hipStream_t st) {
