@@ -122,139 +122,211 @@ template <> struct XOf<ST_TYPE_F32> { typedef float t; };
 template <> struct XOf<ST_TYPE_BF16> { typedef uint16_t t; };
 template <> struct XOf<ST_TYPE_F16> { typedef _Float16 t; };
 
-template <int TYPE> __device__ __forceinline__ float x_value(typename XOf<TYPE>::t v) {
-  if constexpr (TYPE == ST_TYPE_BF16) return __uint_as_float((uint32_t)v << 16);
-  else return (float)v;
-}
-__device__ __forceinline__ uint16_t bf16_of(float v) {   // nearest, ties to even; NaN stays NaN
-  const uint32_t u = __float_as_uint(v);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40);
-  return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1)) >> 16);
-}
-
 struct Q4Args {
   const void* x;
   long ldx;
   int M, N, K, nb, kb;
   const u32x4* codes;
-  const uint16_t* scales;
-  const uint8_t* zeros;
+  const void* scales;
+  const void* zeros;
   const float* bias;
   void* y;
   long ldy;
-  int vec;   // x's rows may be read 8 values at a time
 };
 
-// 8 values of row `row` from column k on as f32; columns from K on and absent rows are 0
-template <int TYPE> __device__ __forceinline__ void load_x8(const Q4Args& a, int row, int k, float (&v)[8]) {
+__device__ __forceinline__ uint16_t bf16_of(float v) {   // nearest, ties to even; NaN stays NaN
+  const uint32_t u = __float_as_uint(v);
+  if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40);
+  return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1)) >> 16);
+}
+template <int TYPE> __device__ __forceinline__ void store_y(const Q4Args& a, int row, int n, float v) {
   typedef typename XOf<TYPE>::t T;
-  const T* p = (const T*)a.x + (size_t)row * a.ldx + k;
-  if (row < a.M && k + 8 <= a.K && a.vec) {
-    T t[8];
-    if constexpr (TYPE == ST_TYPE_F32) {
-      *(f32x4*)&t[0] = *(const f32x4*)p;
-      *(f32x4*)&t[4] = *(const f32x4*)(p + 4);
-    } else {
-      *(f32x4*)&t[0] = *(const f32x4*)p;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = x_value<TYPE>(t[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = row < a.M && k + i < a.K ? x_value<TYPE>(p[i]) : 0.0f;
-  }
+  T* y = (T*)a.y + (size_t)row * a.ldy + n;
+  if constexpr (TYPE == ST_TYPE_BF16) *y = bf16_of(v);
+  else *y = (T)v;
 }
 
-// One workgroup: 16 rows m x 16 NT columns n; its waves take the k blocks in turn and are joined through shared memory.
+// ---- x ---------------------------------------------------------------------------------------------------------------------
+// 8 values of a row from column k on, as they lie in memory (any alignment); absent ones are 0
+template <int TYPE> struct X8 {
+  uint32_t w[TYPE == ST_TYPE_F32 ? 8 : 4];
+  __device__ __forceinline__ void load(const Q4Args& a, int row, int k) {
+    typedef typename XOf<TYPE>::t T;
+    const T* p = (const T*)a.x + (size_t)row * a.ldx + k;
+    if (row < a.M && k + 8 <= a.K) {
+      __builtin_memcpy(w, p, sizeof(w));
+    } else {
+#pragma unroll
+      for (int i = 0; i < (int)(sizeof(w) / 4); ++i) {
+        if constexpr (TYPE == ST_TYPE_F32) {
+          w[i] = row < a.M && k + i < a.K ? __float_as_uint(p[i]) : 0;
+        } else {
+          const uint32_t lo = row < a.M && k + 2 * i < a.K ? ((const uint16_t*)p)[2 * i] : 0;
+          const uint32_t hi = row < a.M && k + 2 * i + 1 < a.K ? ((const uint16_t*)p)[2 * i + 1] : 0;
+          w[i] = lo | hi << 16;
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ float value(int i) const {   // not for f16
+    if constexpr (TYPE == ST_TYPE_F32) return __uint_as_float(w[i]);
+    else return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+  }
+  __device__ __forceinline__ float largest(float m) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(value(i)));
+    return m;
+  }
+  // the values times 2^14 over the row's power of two as f16: rounded towards 0, and for f32 what that leaves, to the nearest
+  __device__ __forceinline__ void split(float shift, h8& hi, h8& lo) const {
+    if constexpr (TYPE == ST_TYPE_F16) {
+      hi = __builtin_bit_cast(h8, *(const u32x4*)w);
+    } else {
+      uint32_t h[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float a = value(2 * i) * shift, b = value(2 * i + 1) * shift;
+        h[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+        if constexpr (TYPE == ST_TYPE_F32) {
+          const h2 q = __builtin_bit_cast(h2, h[i]);
+          lo[2 * i] = (_Float16)fmaxf(a - (float)q[0], -65504.0f);        // an infinity: inf - inf is not wanted
+          lo[2 * i + 1] = (_Float16)fmaxf(b - (float)q[1], -65504.0f);
+        }
+      }
+      hi = __builtin_bit_cast(h8, *(const u32x4*)h);
+    }
+  }
+};
+// The exponent field of a row's largest value so far, 15 at least: 2^(141 - e) brings values of that size to [2^14, 2^15)
+__device__ __forceinline__ int exponent_of(float big) { return (int)((__float_as_uint(big) >> 23) & 255); }
+__device__ __forceinline__ float shift_of(int e) { return __uint_as_float((uint32_t)(268 - e) << 23); }
+__device__ __forceinline__ float unshift_of(int e) { return __uint_as_float((uint32_t)(e - 14) << 23); }
+__device__ __forceinline__ float shrink_of(int from, int to) { return to - from > 126 ? 0.0f : __uint_as_float((uint32_t)(127 - (to - from)) << 23); }
+
+// ---- weights ---------------------------------------------------------------------------------------------------------------
+// what one lane holds of a block: the codes of its row, and the block's scales and zero codes of that row
+template <int GPB> struct W8 {
+  u32x4 codes;
+  uint32_t s[GPB == 4 ? 2 : 1], z;
+  __device__ __forceinline__ void load(const Q4Args& a, int nb, int kb, int lane) {
+    const size_t blk = (size_t)nb * a.kb + kb, at = blk * 16 + (lane & 15);
+    codes = a.codes[blk * 64 + lane];
+    if constexpr (GPB == 4) {
+      const uint2 v = ((const uint2*)a.scales)[at];
+      s[0] = v.x, s[1] = v.y;
+      z = a.zeros ? ((const uint32_t*)a.zeros)[at] : 0x08080808u;
+    } else if constexpr (GPB == 2) {
+      s[0] = ((const uint32_t*)a.scales)[at];
+      z = a.zeros ? ((const uint16_t*)a.zeros)[at] : 0x0808u;
+    } else {
+      s[0] = ((const uint16_t*)a.scales)[at];
+      z = a.zeros ? ((const uint8_t*)a.zeros)[at] : 8u;
+    }
+  }
+  __device__ __forceinline__ float scale(int g) const {
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)(s[g >> 1] >> (16 * (g & 1))));
+  }
+  // the f16 pairs -1024 - z and -64 - z: 0xe400 | z and 0xd400 | z << 4
+  __device__ __forceinline__ h2 zero_low(int g) const { return __builtin_bit_cast(h2, 0xe400e400u | ((z >> (8 * g)) & 15u) * 0x00010001u); }
+  __device__ __forceinline__ h2 zero_high(int g) const { return __builtin_bit_cast(h2, 0xd400d400u | ((z >> (8 * g)) & 15u) * 0x00100010u); }
+};
+
+// One workgroup: 16 rows m x 16 NT columns n; its waves take the k blocks in turn and are joined through shared memory.  For few
+// rows: what bounds it is reading the weights, once, with a block of every wave under way while the last one is multiplied.
 template <int TYPE, int GPB, int NT>
 __global__ __launch_bounds__(512) void q4_rows_kernel(Q4Args a) {
   extern __shared__ float red[];   // [waves][NT][4][64]
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, nw = blockDim.x >> 6;
-  const int m = blockIdx.y * 16 + (lane & 15), kq = 8 * (lane >> 4);
+  const int m = blockIdx.y * 16 + (lane & 15), kq = 8 * (lane >> 4), quad = lane >> 4;
   const int nb0 = blockIdx.x * NT;
-  float shift = 1.0f, unshift = 1.0f;
-  if constexpr (TYPE != ST_TYPE_F16) {
-    float big = 0.0f;
-    for (int b = wv; b < a.kb; b += nw)
-      for (int j = 0; j < 4; ++j) {
-        float v[8];
-        load_x8<TYPE>(a, m, b * KB + 32 * j + kq, v);
+  struct Stage {
+    W8<GPB> w[NT];
+    X8<TYPE> x[4];
+  };
+  auto load = [&](Stage& s, int b) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(v[i]));
-      }
-    big = fmaxf(big, __shfl_xor(big, 16, 64));
-    big = fmaxf(big, __shfl_xor(big, 32, 64));
-    if (big > 0.0f && big < INFINITY) {
-      const int e = min(126, max(-112, 14 - (int)((__float_as_uint(big) >> 23) & 255) + 127));
-      shift = __uint_as_float((uint32_t)(e + 127) << 23);
-      unshift = __uint_as_float((uint32_t)(127 - e) << 23);
-    }
-  }
+    for (int t = 0; t < NT; ++t) s.w[t].load(a, min(nb0 + t, a.nb - 1), b, lane);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s.x[j].load(a, m, b * KB + 32 * j + kq);
+  };
   f32x4 acc[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) acc[t] = f32x4{0, 0, 0, 0};
-  for (int b = wv; b < a.kb; b += nw) {
-    h8 xh[4], xl[4];
+  int e = 15;
+  Stage cur;
+  load(cur, wv);
+#pragma unroll 1
+  for (int b = wv;; b += nw) {
+    const bool more = b + nw < a.kb;
+    Stage next;
+    if (more) load(next, b + nw);
+    float shift = 1.0f;
+    if constexpr (TYPE != ST_TYPE_F16) {
+      float big = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) big = cur.x[j].largest(big);
+      big = fmaxf(big, __shfl_xor(big, 16, 64));
+      big = fmaxf(big, __shfl_xor(big, 32, 64));
+      const int e1 = max(e, min(254, exponent_of(big)));
+      if (b != wv && __any(e1 != e)) {   // rows m of the product are 4 quad + i: their sums so far shrink to the new power of two
+        const float f = shrink_of(e, e1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float fi = __shfl(f, 4 * quad + i, 64);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) acc[t][i] *= fi;
+        }
+      }
+      e = e1;
+      shift = shift_of(e);
+    }
+    f32x4 part[NT];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      float v[8];
-      load_x8<TYPE>(a, m, b * KB + 32 * j + kq, v);
+      h8 xh, xl;
+      cur.x[j].split(shift, xh, xl);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float s = v[i] * shift;
-        xh[j][i] = (_Float16)s;
-        if constexpr (TYPE == ST_TYPE_F32) xl[j][i] = (_Float16)fmaxf(s - (float)xh[j][i], -65504.0f);   // an infinite value: inf - inf
+      for (int t = 0; t < NT; ++t) {
+        const int g = j * GPB / 4;
+        const h8 w = q4_open(cur.w[t].codes[j], cur.w[t].zero_low(g), cur.w[t].zero_high(g));
+        const bool first = j % (4 / GPB) == 0, last = (j + 1) % (4 / GPB) == 0;
+        part[t] = mfma16x32h(xh, w, first ? f32x4{0, 0, 0, 0} : part[t]);
+        if constexpr (TYPE == ST_TYPE_F32) part[t] = mfma16x32h(xl, w, part[t]);
+        if (last) acc[t] += part[t] * cur.w[t].scale(g);
       }
     }
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      if (nb0 + t >= a.nb) continue;
-      const size_t blk = (size_t)(nb0 + t) * a.kb + b;
-      const u32x4 w = a.codes[blk * 64 + lane];
-#pragma unroll
-      for (int g = 0; g < GPB; ++g) {
-        const size_t at = (blk * 16 + (lane & 15)) * GPB + g;
-        const float s = (float)__builtin_bit_cast(_Float16, a.scales[at]);
-        const float z = a.zeros ? (float)a.zeros[at] : 8.0f;
-        const _Float16 zl = (_Float16)(-1024.0f - z), zh = (_Float16)(-64.0f - z);
-        f32x4 part = {0, 0, 0, 0};
-#pragma unroll
-        for (int j = g * (4 / GPB); j < (g + 1) * (4 / GPB); ++j) {
-          const h8 wj = q4_open(w[j], h2{zl, zl}, h2{zh, zh});
-          part = mfma16x32h(xh[j], wj, part);
-          if constexpr (TYPE == ST_TYPE_F32) part = mfma16x32h(xl[j], wj, part);
-        }
-        acc[t] += part * s;
-      }
-    }
+    if (!more) break;
+    cur = next;
   }
-  // the product's rows m are 4 (lane >> 4) + i, its columns n are lane & 15: every row's power of two is taken back here
+  const float unshift = TYPE == ST_TYPE_F16 ? 1.0f : unshift_of(e);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float f = __shfl(unshift, 4 * (lane >> 4) + i, 64);
+    const float f = TYPE == ST_TYPE_F16 ? 1.0f : __shfl(unshift, 4 * quad + i, 64);
 #pragma unroll
     for (int t = 0; t < NT; ++t) red[((wv * NT + t) * 4 + i) * 64 + lane] = acc[t][i] * f;
   }
   __syncthreads();
-  typedef typename XOf<TYPE>::t T;
   for (int o = threadIdx.x; o < NT * 256; o += blockDim.x) {
-    const int row = blockIdx.y * 16 + o / (16 * NT), col = o % (16 * NT), n = nb0 * 16 + col;
-    const int src = ((col >> 4) * 4 + ((o / (16 * NT)) & 3)) * 64 + 16 * ((o / (16 * NT)) >> 2) + (col & 15);
+    const int r = o / (16 * NT), col = o % (16 * NT), row = blockIdx.y * 16 + r, n = nb0 * 16 + col;
     if (row >= a.M || n >= a.N) continue;
-    float s = 0.0f;
+    const int src = ((col >> 4) * 4 + (r & 3)) * 64 + 16 * (r >> 2) + (col & 15);
+    float s = a.bias ? a.bias[n] : 0.0f;
     for (int q = 0; q < nw; ++q) s += red[q * NT * 256 + src];
-    if (a.bias) s += a.bias[n];
-    T* y = (T*)a.y + (size_t)row * a.ldy + n;
-    if constexpr (TYPE == ST_TYPE_BF16) *y = bf16_of(s);
-    else *y = (T)s;
+    store_y<TYPE>(a, row, n, s);
   }
 }
 
-template <int TYPE, int GPB> int q4_launch(const Q4Args& a, hipStream_t st) {
-  const int nw = a.kb < 8 ? a.kb : 8, nt = 4;
-  hipLaunchKernelGGL((q4_rows_kernel<TYPE, GPB, 4>), dim3((a.nb + nt - 1) / nt, (a.M + 15) / 16), dim3(64 * nw), (size_t)nw * nt * 1024, st, a);
+template <int TYPE, int GPB, int NT> int launch_rows(const Q4Args& a, hipStream_t st) {
+  const int nw = a.kb < 8 ? a.kb : 8;
+  hipLaunchKernelGGL((q4_rows_kernel<TYPE, GPB, NT>), dim3((a.nb + NT - 1) / NT, (a.M + 15) / 16), dim3(64 * nw), (size_t)nw * NT * 1024, st, a);
   ST_LAUNCH_CHECK();
   return ST_OK;
+}
+template <int TYPE, int GPB> int q4_launch(const Q4Args& a, hipStream_t st) {
+  const long waves = (long)a.nb * (a.kb < 8 ? a.kb : 8) * ((a.M + 15) / 16);   // with NT = 1
+  if (waves >= 4096) return launch_rows<TYPE, GPB, 4>(a, st);
+  if (waves >= 2048) return launch_rows<TYPE, GPB, 2>(a, st);
+  return launch_rows<TYPE, GPB, 1>(a, st);
 }
 template <int TYPE> int q4_launch_group(const Q4Args& a, int group, hipStream_t st) {
   return group == 32 ? q4_launch<TYPE, 4>(a, st) : group == 64 ? q4_launch<TYPE, 2>(a, st) : q4_launch<TYPE, 1>(a, st);
@@ -309,10 +381,9 @@ extern "C" int st_gemm_q4(const void* x, int type, int64_t ldx, int M, const StQ
   Q4Args a;
   a.x = x; a.ldx = M == 1 ? w->K : ldx; a.M = M; a.N = w->N; a.K = w->K; a.nb = l.nb; a.kb = l.kb;
   a.codes = (const u32x4*)w->image;
-  a.scales = (const uint16_t*)((const char*)w->image + l.scales);
-  a.zeros = w->has_zeros ? (const uint8_t*)w->image + l.zeros : nullptr;
+  a.scales = (const char*)w->image + l.scales;
+  a.zeros = w->has_zeros ? (const char*)w->image + l.zeros : nullptr;
   a.bias = bias; a.y = y; a.ldy = M == 1 ? w->N : ldy;
-  a.vec = ((size_t)x & 15) == 0 && (M == 1 || (size_t)a.ldx * size % 16 == 0);
   hipStream_t st = (hipStream_t)stream;
   return type == ST_TYPE_F32 ? q4_launch_group<ST_TYPE_F32>(a, w->group, st)
          : type == ST_TYPE_BF16 ? q4_launch_group<ST_TYPE_BF16>(a, w->group, st) : q4_launch_group<ST_TYPE_F16>(a, w->group, st);
