@@ -13,7 +13,7 @@ namespace {
 constexpr int KB = 128;   // columns k of a block: 64 lanes x 16 bytes hold 16 rows n x 128 codes
 
 struct Q4Layout {
-  int nb, kb, gpb;         // blocks of 16 n, of 128 k; groups a block
+  int sb, kb, gpb;         // blocks of 64 n, of 128 k; groups a block of k
   size_t scales, zeros, total;   // byte offsets
 };
 
@@ -21,13 +21,13 @@ size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 Q4Layout q4_layout(int N, int K, int group, int has_zeros) {
   Q4Layout y;
-  y.nb = (N + 15) / 16;
+  y.sb = (N + 63) / 64;
   y.kb = (K + KB - 1) / KB;
   y.gpb = KB / group;
-  const size_t blocks = (size_t)y.nb * y.kb;
-  y.scales = blocks * 1024;
-  y.zeros = y.scales + up256(blocks * 16 * y.gpb * 2);
-  y.total = y.zeros + (has_zeros ? up256(blocks * 16 * y.gpb) : 0);
+  const size_t blocks = (size_t)y.sb * y.kb;
+  y.scales = blocks * 4096;
+  y.zeros = y.scales + up256(blocks * 64 * y.gpb * 2);
+  y.total = y.zeros + (has_zeros ? up256(blocks * 64 * y.gpb) : 0);
   return y;
 }
 
@@ -39,39 +39,35 @@ int check_q4_shape(int N, int K, int group) {
 }
 
 // ---- image ---------------------------------------------------------------------------------------------------------------
-// Block (nb, kb) is 1 KB: lane l's 16 bytes are the codes of row n = 16 nb + (l & 15); its word j holds
-// k = 128 kb + 32 j + 8 (l >> 4) + 0..7, the operand of one 16x16x32 product.  In the word, k's pair p (2p, 2p + 1) lies in the
-// nibbles p and p + 4: one and-or makes a pair of f16 out of it.  Scales (f16) and zero codes (bytes) lie block by block,
-// [16 n][groups of the block]: a lane reads those of its row at once.  Rows from N on and groups from K on have scale 0.
+// Block (sb, kb) holds 64 n x 128 k in four tiles of 16 n, 1 KB each: lane l's 16 bytes of tile t are the codes of row
+// n = 64 sb + 16 t + (l & 15); its word j holds k = 128 kb + 32 j + 8 (l >> 4) + 0..7, the operand of one 16x16x32 product.  In the
+// word, k's pair p (2p, 2p + 1) lies in the nibbles p and p + 4: one and-or makes a pair of f16 out of it.  Scales (f16) and zero
+// codes (bytes) lie block by block, [16 l][4 t][groups of the block]: a lane reads those of its four rows at once.  Rows from N on
+// and groups from K on have scale 0.
 __global__ __launch_bounds__(256) void q4_pack_kernel(const uint8_t* __restrict__ codes, const uint16_t* __restrict__ scales,
-                                                      const uint8_t* __restrict__ zeros, int N, int K, int group, int nb_n, int kb_n,
+                                                      const uint8_t* __restrict__ zeros, int N, int K, int group, int kb_n,
                                                       uint32_t* __restrict__ out, uint16_t* __restrict__ out_s, uint8_t* __restrict__ out_z) {
-  const size_t t = (size_t)blockIdx.x * 256 + threadIdx.x;
-  const size_t blocks = (size_t)nb_n * kb_n;
   const int row_bytes = (K + 1) / 2, groups = (K + group - 1) / group, gpb = KB / group;
-  if (t < blocks * 256) {
-    const int j = (int)(t & 3), lane = (int)((t >> 2) & 63);
-    const size_t b = t >> 8;
-    const int kb = (int)(b % kb_n), n = (int)(b / kb_n) * 16 + (lane & 15);
-    const int k0 = kb * KB + 32 * j + 8 * (lane >> 4);
-    uint32_t w = 0;
-    if (n < N)
-      for (int i = 0; i < 8; ++i) {
-        const int k = k0 + i;
-        if (k < K) {
-          const uint32_t c = (codes[(size_t)n * row_bytes + (k >> 1)] >> (4 * (k & 1))) & 15u;
-          w |= c << (4 * ((i >> 1) + 4 * (i & 1)));
-        }
+  const int t = blockIdx.x & 3, j = threadIdx.x & 3, lane = threadIdx.x >> 2;   // one workgroup a tile, a thread a word
+  const size_t b = blockIdx.x >> 2;
+  const int kb = (int)(b % kb_n), n = (int)(b / kb_n) * 64 + 16 * t + (lane & 15);
+  const int k0 = kb * KB + 32 * j + 8 * (lane >> 4);
+  uint32_t w = 0;
+  if (n < N)
+    for (int i = 0; i < 8; ++i) {
+      const int k = k0 + i;
+      if (k < K) {
+        const uint32_t c = (codes[(size_t)n * row_bytes + (k >> 1)] >> (4 * (k & 1))) & 15u;
+        w |= c << (4 * ((i >> 1) + 4 * (i & 1)));
       }
-    out[t] = w;
-  }
-  if (t < blocks * 16 * gpb) {
-    const int i = (int)(t % gpb), r = (int)((t / gpb) & 15);
-    const size_t b = t / (16 * gpb);
-    const int n = (int)(b / kb_n) * 16 + r, g = (int)(b % kb_n) * gpb + i;
-    const bool in = n < N && g < groups;
-    out_s[t] = in ? scales[(size_t)n * groups + g] : (uint16_t)0;
-    if (out_z) out_z[t] = in ? (uint8_t)(zeros[(size_t)n * groups + g] & 15) : (uint8_t)0;
+    }
+  out[(size_t)blockIdx.x * 256 + threadIdx.x] = w;
+  if (threadIdx.x < 16 * gpb) {
+    const int l = threadIdx.x / gpb, i = threadIdx.x % gpb, row = (int)(b / kb_n) * 64 + 16 * t + l, g = kb * gpb + i;
+    const size_t at = ((b * 16 + l) * 4 + t) * gpb + i;
+    const bool in = row < N && g < groups;
+    out_s[at] = in ? scales[(size_t)row * groups + g] : (uint16_t)0;
+    if (out_z) out_z[at] = in ? (uint8_t)(zeros[(size_t)row * groups + g] & 15) : (uint8_t)0;
   }
 }
 
@@ -147,22 +143,21 @@ template <int TYPE> __device__ __forceinline__ void store_y(const Q4Args& a, int
 }
 
 // ---- x ---------------------------------------------------------------------------------------------------------------------
-// 8 values of a row from column k on, as they lie in memory (any alignment); absent ones are 0
+// 8 values of a row from column k on, as they lie in memory (any alignment); columns from K on are 0
 template <int TYPE> struct X8 {
   uint32_t w[TYPE == ST_TYPE_F32 ? 8 : 4];
-  __device__ __forceinline__ void load(const Q4Args& a, int row, int k) {
-    typedef typename XOf<TYPE>::t T;
-    const T* p = (const T*)a.x + (size_t)row * a.ldx + k;
-    if (row < a.M && k + 8 <= a.K) {
-      __builtin_memcpy(w, p, sizeof(w));
+  // FULL: k + 8 <= K
+  template <bool FULL> __device__ __forceinline__ void load(const Q4Args& a, const typename XOf<TYPE>::t* p, int k) {
+    if constexpr (FULL) {
+      __builtin_memcpy(w, p + k, sizeof(w));
     } else {
 #pragma unroll
       for (int i = 0; i < (int)(sizeof(w) / 4); ++i) {
         if constexpr (TYPE == ST_TYPE_F32) {
-          w[i] = row < a.M && k + i < a.K ? __float_as_uint(p[i]) : 0;
+          w[i] = k + i < a.K ? __float_as_uint(p[k + i]) : 0;
         } else {
-          const uint32_t lo = row < a.M && k + 2 * i < a.K ? ((const uint16_t*)p)[2 * i] : 0;
-          const uint32_t hi = row < a.M && k + 2 * i + 1 < a.K ? ((const uint16_t*)p)[2 * i + 1] : 0;
+          const uint32_t lo = k + 2 * i < a.K ? ((const uint16_t*)p)[k + 2 * i] : 0;
+          const uint32_t hi = k + 2 * i + 1 < a.K ? ((const uint16_t*)p)[k + 2 * i + 1] : 0;
           w[i] = lo | hi << 16;
         }
       }
@@ -204,31 +199,41 @@ __device__ __forceinline__ float unshift_of(int e) { return __uint_as_float((uin
 __device__ __forceinline__ float shrink_of(int from, int to) { return to - from > 126 ? 0.0f : __uint_as_float((uint32_t)(127 - (to - from)) << 23); }
 
 // ---- weights ---------------------------------------------------------------------------------------------------------------
-// what one lane holds of a block: the codes of its row, and the block's scales and zero codes of that row
-template <int GPB> struct W8 {
-  u32x4 codes;
-  uint32_t s[GPB == 4 ? 2 : 1], z;
-  __device__ __forceinline__ void load(const Q4Args& a, int nb, int kb, int lane) {
-    const size_t blk = (size_t)nb * a.kb + kb, at = blk * 16 + (lane & 15);
-    codes = a.codes[blk * 64 + lane];
-    if constexpr (GPB == 4) {
-      const uint2 v = ((const uint2*)a.scales)[at];
-      s[0] = v.x, s[1] = v.y;
-      z = a.zeros ? ((const uint32_t*)a.zeros)[at] : 0x08080808u;
-    } else if constexpr (GPB == 2) {
-      s[0] = ((const uint32_t*)a.scales)[at];
-      z = a.zeros ? ((const uint16_t*)a.zeros)[at] : 0x0808u;
-    } else {
-      s[0] = ((const uint16_t*)a.scales)[at];
-      z = a.zeros ? ((const uint8_t*)a.zeros)[at] : 8u;
-    }
+// what one lane holds of NT tiles of a block: codes, and the block's scales and zero codes of its rows
+template <int BYTES> __device__ __forceinline__ void load_bytes(uint32_t* w, const void* p) {
+  if constexpr (BYTES == 1) w[0] = *(const uint8_t*)p;
+  else if constexpr (BYTES == 2) w[0] = *(const uint16_t*)p;
+  else __builtin_memcpy(w, __builtin_assume_aligned(p, BYTES < 16 ? BYTES : 16), BYTES);
+}
+template <int GPB, int NT> struct W8 {
+  u32x4 codes[NT];
+  uint32_t s[(NT * GPB + 1) / 2], z[(NT * GPB + 3) / 4];
+  __device__ __forceinline__ void load(const Q4Args& a, int nb, int kb, int lane) {   // nb: a multiple of NT
+    const size_t blk = (size_t)(nb >> 2) * a.kb + kb, at = (blk * 64 + (lane & 15) * 4 + (nb & 3)) * GPB;
+    const u32x4* c = a.codes + (blk * 4 + (nb & 3)) * 64 + lane;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) codes[t] = c[64 * t];
+    load_bytes<NT * GPB * 2>(s, (const char*)a.scales + at * 2);
+    if (a.zeros) load_bytes<NT * GPB>(z, (const char*)a.zeros + at);
+    else
+#pragma unroll
+      for (int i = 0; i < (NT * GPB + 3) / 4; ++i) z[i] = 0x08080808u;
   }
-  __device__ __forceinline__ float scale(int g) const {
-    return (float)__builtin_bit_cast(_Float16, (uint16_t)(s[g >> 1] >> (16 * (g & 1))));
+  __device__ __forceinline__ float scale(int t, int g) const {
+    const int i = t * GPB + g;
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)(s[i >> 1] >> (16 * (i & 1))));
   }
   // the f16 pairs -1024 - z and -64 - z: 0xe400 | z and 0xd400 | z << 4
-  __device__ __forceinline__ h2 zero_low(int g) const { return __builtin_bit_cast(h2, 0xe400e400u | ((z >> (8 * g)) & 15u) * 0x00010001u); }
-  __device__ __forceinline__ h2 zero_high(int g) const { return __builtin_bit_cast(h2, 0xd400d400u | ((z >> (8 * g)) & 15u) * 0x00100010u); }
+  __device__ __forceinline__ h2 zero_low(int t, int g) const {
+    const int i = t * GPB + g;
+    const uint32_t v = (z[i >> 2] >> (8 * (i & 3))) & 15u;
+    return __builtin_bit_cast(h2, 0xe400e400u | v | v << 16);
+  }
+  __device__ __forceinline__ h2 zero_high(int t, int g) const {
+    const int i = t * GPB + g;
+    const uint32_t v = (z[i >> 2] >> (8 * (i & 3))) & 15u;
+    return __builtin_bit_cast(h2, 0xd400d400u | v << 4 | v << 20);
+  }
 };
 
 // One workgroup: 16 rows m x 16 NT columns n; its waves take the k blocks in turn and are joined through shared memory.  For few
@@ -237,17 +242,23 @@ template <int TYPE, int GPB, int NT>
 __global__ __launch_bounds__(512) void q4_rows_kernel(Q4Args a) {
   extern __shared__ float red[];   // [waves][NT][4][64]
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, nw = blockDim.x >> 6;
-  const int m = blockIdx.y * 16 + (lane & 15), kq = 8 * (lane >> 4), quad = lane >> 4;
+  const int kq = 8 * (lane >> 4), quad = lane >> 4;
   const int nb0 = blockIdx.x * NT;
+  // lanes of absent rows read the last one: nothing comes of it
+  const typename XOf<TYPE>::t* xrow = (const typename XOf<TYPE>::t*)a.x + (size_t)min((int)blockIdx.y * 16 + (lane & 15), a.M - 1) * a.ldx;
   struct Stage {
-    W8<GPB> w[NT];
+    W8<GPB, NT> w;
     X8<TYPE> x[4];
   };
   auto load = [&](Stage& s, int b) __attribute__((always_inline)) {
+    s.w.load(a, nb0, b, lane);
+    if ((b + 1) * KB <= a.K) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) s.w[t].load(a, min(nb0 + t, a.nb - 1), b, lane);
+      for (int j = 0; j < 4; ++j) s.x[j].template load<true>(a, xrow, b * KB + 32 * j + kq);
+    } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s.x[j].load(a, m, b * KB + 32 * j + kq);
+      for (int j = 0; j < 4; ++j) s.x[j].template load<false>(a, xrow, b * KB + 32 * j + kq);
+    }
   };
   f32x4 acc[NT];
 #pragma unroll
@@ -288,11 +299,11 @@ __global__ __launch_bounds__(512) void q4_rows_kernel(Q4Args a) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const int g = j * GPB / 4;
-        const h8 w = q4_open(cur.w[t].codes[j], cur.w[t].zero_low(g), cur.w[t].zero_high(g));
+        const h8 w = q4_open(cur.w.codes[t][j], cur.w.zero_low(t, g), cur.w.zero_high(t, g));
         const bool first = j % (4 / GPB) == 0, last = (j + 1) % (4 / GPB) == 0;
         part[t] = mfma16x32h(xh, w, first ? f32x4{0, 0, 0, 0} : part[t]);
         if constexpr (TYPE == ST_TYPE_F32) part[t] = mfma16x32h(xl, w, part[t]);
-        if (last) acc[t] += part[t] * cur.w[t].scale(g);
+        if (last) acc[t] += part[t] * cur.w.scale(t, g);
       }
     }
     if (!more) break;
@@ -345,11 +356,11 @@ extern "C" int st_pack_weight_q4(const uint8_t* codes, const void* scales, const
   ST_CHECK_ARG(codes && scales && out_packed, "NULL buffer");
   ST_CHECK_ARG(((size_t)out_packed & 15) == 0, "the packed image must lie on 16 bytes");
   const Q4Layout y = q4_layout(N, K, group, zeros != nullptr);
-  const size_t threads = (size_t)y.nb * y.kb * 256;
-  ST_CHECK_ARG(threads / 256 < (1ull << 31), "N=%d K=%d: too large for one launch", N, K);
+  const size_t tiles = (size_t)y.sb * y.kb * 4;
+  ST_CHECK_ARG(tiles < (1ull << 31), "N=%d K=%d: too large for one launch", N, K);
   char* out = (char*)out_packed;
-  hipLaunchKernelGGL(q4_pack_kernel, dim3((unsigned)((size_t)y.nb * y.kb)), dim3(256), 0, (hipStream_t)stream, codes, (const uint16_t*)scales,
-                     zeros, N, K, group, y.nb, y.kb, (uint32_t*)out, (uint16_t*)(out + y.scales), zeros ? (uint8_t*)(out + y.zeros) : nullptr);
+  hipLaunchKernelGGL(q4_pack_kernel, dim3((unsigned)tiles), dim3(256), 0, (hipStream_t)stream, codes, (const uint16_t*)scales,
+                     zeros, N, K, group, y.kb, (uint32_t*)out, (uint16_t*)(out + y.scales), zeros ? (uint8_t*)(out + y.zeros) : nullptr);
   ST_LAUNCH_CHECK();
   return ST_OK;
 }
@@ -379,7 +390,7 @@ extern "C" int st_gemm_q4(const void* x, int type, int64_t ldx, int M, const StQ
   ST_CHECK_ARG(ldx >= 0 && (M == 1 || ldy >= w->N), "ldx=%lld ldy=%lld: negative, or rows of y (%d values) overlap", (long long)ldx, (long long)ldy, w->N);
   const Q4Layout l = q4_layout(w->N, w->K, w->group, w->has_zeros);
   Q4Args a;
-  a.x = x; a.ldx = M == 1 ? w->K : ldx; a.M = M; a.N = w->N; a.K = w->K; a.nb = l.nb; a.kb = l.kb;
+  a.x = x; a.ldx = M == 1 ? w->K : ldx; a.M = M; a.N = w->N; a.K = w->K; a.nb = (w->N + 15) / 16; a.kb = l.kb;
   a.codes = (const u32x4*)w->image;
   a.scales = (const char*)w->image + l.scales;
   a.zeros = w->has_zeros ? (const char*)w->image + l.zeros : nullptr;
