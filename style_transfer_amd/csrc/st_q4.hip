@@ -335,8 +335,8 @@ template <int TYPE, int GPB, int NT> int launch_rows(const Q4Args& a, hipStream_
 }
 template <int TYPE, int GPB> int q4_launch(const Q4Args& a, hipStream_t st) {
   const long waves = (long)a.nb * (a.kb < 8 ? a.kb : 8) * ((a.M + 15) / 16);   // with NT = 1
-  if (waves >= 4096) return launch_rows<TYPE, GPB, 4>(a, st);
-  if (waves >= 2048) return launch_rows<TYPE, GPB, 2>(a, st);
+  if (waves >= 8192) return launch_rows<TYPE, GPB, 4>(a, st);
+  if (waves >= 4096) return launch_rows<TYPE, GPB, 2>(a, st);
   return launch_rows<TYPE, GPB, 1>(a, st);
 }
 template <int TYPE> int q4_launch_group(const Q4Args& a, int group, hipStream_t st) {
