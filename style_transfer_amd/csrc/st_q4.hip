@@ -101,17 +101,21 @@ __global__ __launch_bounds__(256) void q4_quantize_kernel(const float* __restric
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// 8 codes -> 8 f16 values c - z.  0x6400 | c is the f16 1024 + c; with c in the second nibble it is 1024 + 16 c, a sixteenth of
-// which is 64 + c: both corrections are exact.
-__device__ __forceinline__ h8 q4_open(uint32_t w, h2 z_low, h2 z_high) {
-  const h2 sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
-  const h2 a = __builtin_bit_cast(h2, (w & 0x000f000fu) | 0x64006400u) + z_low;
-  const h2 b = __builtin_bit_cast(h2, (w & 0x00f000f0u) | 0x64006400u) * sixteenth + z_high;
-  const uint32_t v = w >> 8;
-  const h2 c = __builtin_bit_cast(h2, (v & 0x000f000fu) | 0x64006400u) + z_low;
-  const h2 d = __builtin_bit_cast(h2, (v & 0x00f000f0u) | 0x64006400u) * sixteenth + z_high;
-  return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
+// 8 codes -> 8 f16 values c - z.  0x6400 | c is the f16 1024 + c, and 0x5400 | c << 4 is 64 + c; both corrections are exact.  The
+// masks lie in registers (the empty asm keeps hipcc from making literals of them): an and-or then is one instruction, and 8 codes
+// take 9 instead of 13, which is what a product with few rows has to do per weight.
+struct Open {
+  uint32_t low, high, b_low, b_high;
+  __device__ __forceinline__ Open() : low(0x000f000fu), high(0x00f000f0u), b_low(0x64006400u), b_high(0x54005400u) {
+    asm("" : "+v"(low), "+v"(high), "+s"(b_low), "+s"(b_high));
+  }
+  __device__ __forceinline__ h8 operator()(uint32_t w, h2 z_low, h2 z_high) const {
+    const uint32_t v = w >> 8;
+    const h2 a = __builtin_bit_cast(h2, (w & low) | b_low) + z_low, b = __builtin_bit_cast(h2, (w & high) | b_high) + z_high;
+    const h2 c = __builtin_bit_cast(h2, (v & low) | b_low) + z_low, d = __builtin_bit_cast(h2, (v & high) | b_high) + z_high;
+    return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+  }
+};
 
 template <int TYPE> struct XOf;
 template <> struct XOf<ST_TYPE_F32> { typedef float t; };
@@ -260,6 +264,7 @@ __global__ __launch_bounds__(512) void q4_rows_kernel(Q4Args a) {
       for (int j = 0; j < 4; ++j) s.x[j].template load<false>(a, xrow, b * KB + 32 * j + kq);
     }
   };
+  const Open open;
   f32x4 acc[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) acc[t] = f32x4{0, 0, 0, 0};
@@ -299,7 +304,7 @@ __global__ __launch_bounds__(512) void q4_rows_kernel(Q4Args a) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const int g = j * GPB / 4;
-        const h8 w = q4_open(cur.w.codes[t][j], cur.w.zero_low(t, g), cur.w.zero_high(t, g));
+        const h8 w = open(cur.w.codes[t][j], cur.w.zero_low(t, g), cur.w.zero_high(t, g));
         const bool first = j % (4 / GPB) == 0, last = (j + 1) % (4 / GPB) == 0;
         part[t] = mfma16x32h(xh, w, first ? f32x4{0, 0, 0, 0} : part[t]);
         if constexpr (TYPE == ST_TYPE_F32) part[t] = mfma16x32h(xl, w, part[t]);
