@@ -122,9 +122,15 @@ template <> struct XOf<ST_TYPE_F32> { typedef float t; };
 template <> struct XOf<ST_TYPE_BF16> { typedef uint16_t t; };
 template <> struct XOf<ST_TYPE_F16> { typedef _Float16 t; };
 
+// a barrier for shared memory alone: loads from global memory stay under way across it (__syncthreads waits for them)
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 struct Q4Args {
   const void* x;
   long ldx;
+  const void* x8;   // where 8 values at a time are read from, at columns up to k8: x and K - 8; with K < 8 any memory (the image)
+  long ldx8;
+  int k8;
   int M, N, K, nb, kb;
   const u32x4* codes;
   const void* scales;
@@ -150,20 +156,18 @@ template <int TYPE> __device__ __forceinline__ void store_y(const Q4Args& a, int
 // 8 values of a row from column k on, as they lie in memory (any alignment); columns from K on are 0
 template <int TYPE> struct X8 {
   uint32_t w[TYPE == ST_TYPE_F32 ? 8 : 4];
-  // FULL: k + 8 <= K
-  template <bool FULL> __device__ __forceinline__ void load(const Q4Args& a, const typename XOf<TYPE>::t* p, int k) {
-    if constexpr (FULL) {
-      __builtin_memcpy(w, p + k, sizeof(w));
-    } else {
+  // no branch stands around a load, so that it can stay under way: where fewer than 8 columns are left the row's last 8 are read,
+  // and whoever uses them comes back for the right ones (tail)
+  __device__ __forceinline__ void load(const Q4Args& a, const typename XOf<TYPE>::t* p8, int k) { __builtin_memcpy(w, p8 + min(k, a.k8), sizeof(w)); }
+  __device__ __forceinline__ void tail(const Q4Args& a, const typename XOf<TYPE>::t* p, int k) {
 #pragma unroll
-      for (int i = 0; i < (int)(sizeof(w) / 4); ++i) {
-        if constexpr (TYPE == ST_TYPE_F32) {
-          w[i] = k + i < a.K ? __float_as_uint(p[k + i]) : 0;
-        } else {
-          const uint32_t lo = k + 2 * i < a.K ? ((const uint16_t*)p)[k + 2 * i] : 0;
-          const uint32_t hi = k + 2 * i + 1 < a.K ? ((const uint16_t*)p)[k + 2 * i + 1] : 0;
-          w[i] = lo | hi << 16;
-        }
+    for (int i = 0; i < (int)(sizeof(w) / 4); ++i) {
+      if constexpr (TYPE == ST_TYPE_F32) {
+        w[i] = k + i < a.K ? __float_as_uint(p[k + i]) : 0;
+      } else {
+        const uint32_t lo = k + 2 * i < a.K ? ((const uint16_t*)p)[k + 2 * i] : 0;
+        const uint32_t hi = k + 2 * i + 1 < a.K ? ((const uint16_t*)p)[k + 2 * i + 1] : 0;
+        w[i] = lo | hi << 16;
       }
     }
   }
@@ -218,10 +222,12 @@ template <int GPB, int NT> struct W8 {
 #pragma unroll
     for (int t = 0; t < NT; ++t) codes[t] = c[64 * t];
     load_bytes<NT * GPB * 2>(s, (const char*)a.scales + at * 2);
-    if (a.zeros) load_bytes<NT * GPB>(z, (const char*)a.zeros + at);
-    else
+    // (no branch here either: without zero codes the scales are read, and dropped)
+    load_bytes<NT * GPB>(z, (const char*)(a.zeros ? a.zeros : a.scales) + at);
+  }
+  __device__ __forceinline__ void settle(const Q4Args& a) {   // before the first use
 #pragma unroll
-      for (int i = 0; i < (NT * GPB + 3) / 4; ++i) z[i] = 0x08080808u;
+    for (int i = 0; i < (NT * GPB + 3) / 4; ++i) z[i] = a.zeros ? z[i] : 0x08080808u;
   }
   __device__ __forceinline__ float scale(int t, int g) const {
     const int i = t * GPB + g;
@@ -242,40 +248,36 @@ template <int GPB, int NT> struct W8 {
 
 // One workgroup: 16 rows m x 16 NT columns n; its waves take the k blocks in turn and are joined through shared memory.  For few
 // rows: what bounds it is reading the weights, once, with a block of every wave under way while the last one is multiplied.
-template <int TYPE, int GPB, int NT>
+template <int TYPE, int GPB, int NT, bool ONE>   // ONE: a block a wave
 __global__ __launch_bounds__(512) void q4_rows_kernel(Q4Args a) {
   extern __shared__ float red[];   // [waves][NT][4][64]
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, nw = blockDim.x >> 6;
   const int kq = 8 * (lane >> 4), quad = lane >> 4;
   const int nb0 = blockIdx.x * NT;
   // lanes of absent rows read the last one: nothing comes of it
-  const typename XOf<TYPE>::t* xrow = (const typename XOf<TYPE>::t*)a.x + (size_t)min((int)blockIdx.y * 16 + (lane & 15), a.M - 1) * a.ldx;
+  typedef typename XOf<TYPE>::t T;
+  const size_t row = min((int)blockIdx.y * 16 + (lane & 15), a.M - 1);
+  const T *xrow = (const T*)a.x + row * a.ldx, *xrow8 = (const T*)a.x8 + row * a.ldx8;
   struct Stage {
     W8<GPB, NT> w;
     X8<TYPE> x[4];
   };
   auto load = [&](Stage& s, int b) __attribute__((always_inline)) {
     s.w.load(a, nb0, b, lane);
-    if ((b + 1) * KB <= a.K) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s.x[j].template load<true>(a, xrow, b * KB + 32 * j + kq);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s.x[j].template load<false>(a, xrow, b * KB + 32 * j + kq);
-    }
+    for (int j = 0; j < 4; ++j) s.x[j].load(a, xrow8, b * KB + 32 * j + kq);
   };
   const Open open;
   f32x4 acc[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) acc[t] = f32x4{0, 0, 0, 0};
   int e = 15;
-  Stage cur;
-  load(cur, wv);
-#pragma unroll 1
-  for (int b = wv;; b += nw) {
-    const bool more = b + nw < a.kb;
-    Stage next;
-    if (more) load(next, b + nw);
+  auto multiply = [&](Stage& cur, int b) __attribute__((always_inline)) {
+    if ((b + 1) * KB > a.K) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) cur.x[j].tail(a, xrow, b * KB + 32 * j + kq);
+    }
+    cur.w.settle(a);
     float shift = 1.0f;
     if constexpr (TYPE != ST_TYPE_F16) {
       float big = 0.0f;
@@ -311,8 +313,21 @@ __global__ __launch_bounds__(512) void q4_rows_kernel(Q4Args a) {
         if (last) acc[t] += part[t] * cur.w.scale(t, g);
       }
     }
-    if (!more) break;
-    cur = next;
+  };
+  Stage cur;
+  load(cur, wv);
+  if constexpr (ONE) {
+    multiply(cur, wv);
+  } else {
+#pragma unroll 1
+    for (int b = wv;; b += nw) {
+      const bool more = b + nw < a.kb;
+      Stage next;
+      if (more) load(next, b + nw);
+      multiply(cur, b);
+      if (!more) break;
+      cur = next;
+    }
   }
   const float unshift = TYPE == ST_TYPE_F16 ? 1.0f : unshift_of(e);
 #pragma unroll
@@ -332,14 +347,198 @@ __global__ __launch_bounds__(512) void q4_rows_kernel(Q4Args a) {
   }
 }
 
-template <int TYPE, int GPB, int NT> int launch_rows(const Q4Args& a, hipStream_t st) {
-  const int nw = a.kb < 8 ? a.kb : 8;
-  hipLaunchKernelGGL((q4_rows_kernel<TYPE, GPB, NT>), dim3((a.nb + NT - 1) / NT, (a.M + 15) / 16), dim3(64 * nw), (size_t)nw * NT * 1024, st, a);
+// One workgroup: 16 MT WM rows m x 16 NT WN columns n, WM x WN waves of MT x NT tiles each, for more than 16 rows.  Every block of
+// 128 k of x is brought to f16 once a workgroup, a thread a row's quarter, into the operand order of the matrix instruction
+// (a wave reads 1 KB in a row: no bank conflicts), in two buffers, so that one barrier a block is enough; the weights go from global
+// memory to registers, a block ahead.
+template <int TYPE, int GPB, int MT, int NT, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void q4_tile_kernel(Q4Args a, int tiles_m, int tiles_n) {
+  constexpr int ROWS = 16 * MT * WM, PARTS = TYPE == ST_TYPE_F32 ? 2 : 1, WAVES = WM * WN, UNITS = ROWS / 16 / WAVES;
+  static_assert(UNITS * WAVES * 16 == ROWS, "every wave stages UNITS times 16 rows");
+  extern __shared__ __align__(16) char dyn[];
+  h8* const xs = (h8*)dyn;                                            // [2][PARTS][ROWS / 16][4][64]
+  float* const shrink = (float*)(xs + 2 * PARTS * ROWS * 16);         // [2][ROWS]
+  int* const shrunk = (int*)(shrink + 2 * ROWS);                      // [2]: the block that the buffer's factors belong to
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, quad = lane >> 4;
+  // tiles of the same columns on the same XCD (workgroups go round the eight of them): its L2 has the weights once
+  const int xcd = blockIdx.x & 7, idx = blockIdx.x >> 3, tile_n = idx / tiles_m * 8 + xcd, tile_m = idx % tiles_m;
+  if (tile_n >= tiles_n) return;
+  const int m0 = tile_m * ROWS, wm = wv / WN, wn = wv % WN, nb0 = (tile_n * WN + wn) * NT;
+  const int nbl = min(nb0, (a.nb - 1) & ~(NT - 1));                  // waves behind the last column read the last ones again
+  // staging: this thread's rows 16 (wv + WAVES u) + (lane & 15) and their columns 8 quad + 32 j
+  typedef typename XOf<TYPE>::t T;
+  const int kq = 8 * quad;
+  int e[UNITS];
+  X8<TYPE> raw[UNITS][4];
+  size_t row[UNITS];
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u) row[u] = min(m0 + 16 * (wv + WAVES * u) + (lane & 15), a.M - 1), e[u] = 15;
+  auto load_x = [&](int b) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) raw[u][j].load(a, (const T*)a.x8 + row[u] * a.ldx8, b * KB + 32 * j + kq);
+  };
+  auto stage = [&](int b) __attribute__((always_inline)) {
+    const int buf = b & 1;
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const int rb = wv + WAVES * u;
+      if ((b + 1) * KB > a.K) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) raw[u][j].tail(a, (const T*)a.x + row[u] * a.ldx, b * KB + 32 * j + kq);
+      }
+      float shift = 1.0f;
+      if constexpr (TYPE != ST_TYPE_F16) {
+        float big = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) big = raw[u][j].largest(big);
+        big = fmaxf(big, __shfl_xor(big, 16, 64));
+        big = fmaxf(big, __shfl_xor(big, 32, 64));
+        const int e1 = max(e[u], min(254, exponent_of(big)));
+        if (quad == 0) shrink[buf * ROWS + 16 * rb + (lane & 15)] = shrink_of(e[u], e1);
+        if (__any(e1 != e[u]) && lane == 0) shrunk[buf] = b;
+        e[u] = e1;
+        shift = shift_of(e1);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        h8 hi, lo;
+        raw[u][j].split(shift, hi, lo);
+        xs[((buf * PARTS + 0) * (ROWS / 16) + rb) * 256 + j * 64 + lane] = hi;
+        if constexpr (PARTS == 2) xs[((buf * PARTS + 1) * (ROWS / 16) + rb) * 256 + j * 64 + lane] = lo;
+      }
+    }
+  };
+  const Open open;
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[i][t] = f32x4{0, 0, 0, 0};
+  if (tid < 2) shrunk[tid] = 0;   // block 0 shrinks sums that are still 0
+  auto multiply = [&](W8<GPB, NT>& cur, int b) __attribute__((always_inline)) {
+    const int buf = b & 1;
+    cur.settle(a);
+    if (TYPE != ST_TYPE_F16 && b > 0 && shrunk[buf] == b) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const f32x4 f = *(const f32x4*)&shrink[buf * ROWS + (wm * MT + i) * 16 + 4 * quad];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[i][t] *= f;
+      }
+    }
+    f32x4 part[MT][NT];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      constexpr int JG = 4 / GPB;
+      const int g = j / JG;
+      const bool first = j % JG == 0, last = (j + 1) % JG == 0;
+      h8 xh[MT], xl[MT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        xh[i] = xs[((buf * PARTS + 0) * (ROWS / 16) + wm * MT + i) * 256 + j * 64 + lane];
+        if constexpr (PARTS == 2) xl[i] = xs[((buf * PARTS + 1) * (ROWS / 16) + wm * MT + i) * 256 + j * 64 + lane];
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const h8 w = open(cur.codes[t][j], cur.zero_low(t, g), cur.zero_high(t, g));
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          part[i][t] = mfma16x32h(xh[i], w, first ? f32x4{0, 0, 0, 0} : part[i][t]);
+          if constexpr (PARTS == 2) part[i][t] = mfma16x32h(xl[i], w, part[i][t]);
+        }
+      }
+      if (last) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const float s = cur.scale(t, g);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) acc[i][t] += part[i][t] * s;
+        }
+      }
+    }
+  };
+  W8<GPB, NT> even, odd;
+  const int last_b = a.kb - 1;
+  load_x(0);
+  even.load(a, nbl, 0, lane);
+  __syncthreads();
+  stage(0);
+#pragma unroll 1
+  for (int b = 0;; b += 2) {
+    lds_barrier();   // block b is staged, and nobody reads the other buffer any more
+    load_x(min(b + 1, last_b));
+    odd.load(a, nbl, min(b + 1, last_b), lane);
+    __builtin_amdgcn_sched_barrier(0);   // they go out before the products
+    multiply(even, b);
+    if (b + 1 > last_b) break;
+    stage(b + 1);
+    lds_barrier();
+    load_x(min(b + 2, last_b));
+    even.load(a, nbl, min(b + 2, last_b), lane);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(odd, b + 1);
+    if (b + 2 > last_b) break;
+    stage(b + 2);
+  }
+  __syncthreads();
+  if (TYPE != ST_TYPE_F16 && quad == 0) {
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) shrink[16 * (wv + WAVES * u) + (lane & 15)] = unshift_of(e[u]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int n = (nb0 + t) * 16 + (lane & 15);
+    if (n >= a.N) continue;
+    const float bias = a.bias ? a.bias[n] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int r = (wm * MT + i) * 16 + 4 * quad;
+      const f32x4 f = TYPE == ST_TYPE_F16 ? f32x4{1, 1, 1, 1} : *(const f32x4*)&shrink[r];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (m0 + r + c < a.M) store_y<TYPE>(a, m0 + r + c, n, acc[i][t][c] * f[c] + bias);
+    }
+  }
+}
+
+template <int TYPE, int GPB, int MT, int NT, int WM, int WN> int launch_tile(const Q4Args& a, hipStream_t st) {
+  constexpr int ROWS = 16 * MT * WM, COLS = NT * WN, PARTS = TYPE == ST_TYPE_F32 ? 2 : 1;
+  constexpr int lds = 2 * PARTS * ROWS * 256 + 2 * ROWS * 4 + 16;
+  const int tiles_m = (a.M + ROWS - 1) / ROWS, tiles_n = (a.nb + COLS - 1) / COLS;
+  const long grid = (long)(tiles_n + 7) / 8 * 8 * tiles_m;
+  ST_CHECK_ARG(grid < (1L << 31), "M=%d N=%d: too large for one launch", a.M, a.N);
+  ST_ENSURE_LDS((q4_tile_kernel<TYPE, GPB, MT, NT, WM, WN>), lds);
+  hipLaunchKernelGGL((q4_tile_kernel<TYPE, GPB, MT, NT, WM, WN>), dim3((unsigned)grid), dim3(64 * WM * WN), lds, st, a, tiles_m, tiles_n);
   ST_LAUNCH_CHECK();
   return ST_OK;
 }
+template <int TYPE, int GPB, int NT> int launch_rows(const Q4Args& a, hipStream_t st) {
+  const int nw = a.kb < 8 ? a.kb : 8;
+  const dim3 grid((a.nb + NT - 1) / NT, (a.M + 15) / 16), block(64 * nw);
+  const size_t lds = (size_t)nw * NT * 1024;
+  if (a.kb <= nw) hipLaunchKernelGGL((q4_rows_kernel<TYPE, GPB, NT, true>), grid, block, lds, st, a);
+  else hipLaunchKernelGGL((q4_rows_kernel<TYPE, GPB, NT, false>), grid, block, lds, st, a);
+  ST_LAUNCH_CHECK();
+  return ST_OK;
+}
+// Which kernel, measured on both sides (f16 / f32, us): the rows kernel reads and opens every weight once for each 16 rows and has
+// a short way for each, the tile kernel once for each 64 or 128, behind a barrier a block of k.  16 x 16 x 128 blocks of the product:
+// 65 536 (128 x 8192 x 2048) 19.8 / 32.8 by rows, 22.7 / 39.4 by tiles; 131 072 (256 x 4096 x 4096) 32 / 57, 37 / 69; 262 144
+// (128 x 16384 x 4096) 63 / 113, 39 / 71.  The large tile, where a launch of it fills the chip: 256 x 32768 x 4096 91 / 214 against
+// 109 / 276; with half as many workgroups (128 x 16384 x 4096) it takes 81 / 104 against 39 / 71.
 template <int TYPE, int GPB> int q4_launch(const Q4Args& a, hipStream_t st) {
-  const long waves = (long)a.nb * (a.kb < 8 ? a.kb : 8) * ((a.M + 15) / 16);   // with NT = 1
+  const long mt = (a.M + 15) / 16;
+  if (mt > 1 && mt * a.nb * a.kb >= 196608) {
+    constexpr int NT = TYPE == ST_TYPE_F32 ? 2 : 4;
+    if ((mt + 7) / 8 * ((a.nb + 4 * NT - 1) / (4 * NT)) >= 192) return launch_tile<TYPE, GPB, 4, NT, 2, 4>(a, st);
+    return launch_tile<TYPE, GPB, 4, 2, 1, 4>(a, st);
+  }
+  // tiles of a wave: one while the launch has fewer than two waves a SIMD and more (4096 x 4096 on one row: 5.2 us, 6.1 with two,
+  // 8.3 with four), four where x is brought to f16 for many (16384 x 4096: 17, 14, 12 us)
+  const long waves = a.nb * (a.kb < 8 ? a.kb : 8) * mt;
   if (waves >= 8192) return launch_rows<TYPE, GPB, 4>(a, st);
   if (waves >= 4096) return launch_rows<TYPE, GPB, 2>(a, st);
   return launch_rows<TYPE, GPB, 1>(a, st);
@@ -399,6 +598,7 @@ extern "C" int st_gemm_q4(const void* x, int type, int64_t ldx, int M, const StQ
   a.codes = (const u32x4*)w->image;
   a.scales = (const char*)w->image + l.scales;
   a.zeros = w->has_zeros ? (const char*)w->image + l.zeros : nullptr;
+  a.x8 = w->K >= 8 ? x : w->image; a.ldx8 = w->K >= 8 ? a.ldx : 0; a.k8 = w->K >= 8 ? w->K - 8 : 0;
   a.bias = bias; a.y = y; a.ldy = M == 1 ? w->N : ldy;
   hipStream_t st = (hipStream_t)stream;
   return type == ST_TYPE_F32 ? q4_launch_group<ST_TYPE_F32>(a, w->group, st)
