@@ -27,12 +27,10 @@ template <int TYPE> struct LOf;
 template <> struct LOf<ST_TYPE_F32> { typedef float t; };
 template <> struct LOf<ST_TYPE_BF16> { typedef uint16_t t; };
 template <> struct LOf<ST_TYPE_F16> { typedef _Float16 t; };
-template <int TYPE> __device__ __forceinline__ float raw_logit(typename LOf<TYPE>::t v) {
-  if constexpr (TYPE == ST_TYPE_BF16) return __uint_as_float((uint32_t)v << 16);
-  else return (float)v;
-}
 template <int TYPE> __device__ __forceinline__ float logit(typename LOf<TYPE>::t v) {   // -inf: no entry (a NaN is none either)
-  const float f = raw_logit<TYPE>(v);
+  float f;
+  if constexpr (TYPE == ST_TYPE_BF16) f = __uint_as_float((uint32_t)v << 16);
+  else f = (float)v;
   return f == f ? f : -INFINITY;
 }
 template <int TYPE> __device__ __forceinline__ typename LOf<TYPE>::t no_entry() {
@@ -89,60 +87,76 @@ template <int TYPE> struct Row {
     pad = (int)(((size_t)p & 15) / sizeof(T));
     chunks = (n + pad + EPC - 1) / EPC;
   }
-  __device__ __forceinline__ T entry(f32x4 k, int j) const {
+  // entry j of a chunk, as f32 (a NaN stays one)
+  static __device__ __forceinline__ float entry(f32x4 k, int j) {
     if constexpr (TYPE == ST_TYPE_F32) return k[j];
-    else if constexpr (TYPE == ST_TYPE_F16) return __builtin_bit_cast(h8, k)[j];
-    else return (uint16_t)(__float_as_uint(k[j >> 1]) >> (16 * (j & 1)));
+    else if constexpr (TYPE == ST_TYPE_F16) return (float)__builtin_bit_cast(h8, k)[j];
+    else return __uint_as_float(j & 1 ? __float_as_uint(k[j >> 1]) & 0xffff0000u : __float_as_uint(k[j >> 1]) << 16);
   }
-  // a chunk that sticks out of the row, put together from single entries
+  // the same where j is not known to hipcc
+  static __device__ __forceinline__ float pick(f32x4 k, int j) {
+    const int w = TYPE == ST_TYPE_F32 ? j : j >> 1;
+    const float v = w & 2 ? (w & 1 ? k[3] : k[2]) : (w & 1 ? k[1] : k[0]);
+    if constexpr (TYPE == ST_TYPE_F32) return v;
+    const uint32_t u = j & 1 ? __float_as_uint(v) >> 16 : __float_as_uint(v) & 0xffffu;
+    if constexpr (TYPE == ST_TYPE_F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)u);
+    else return __uint_as_float(u << 16);
+  }
+  // a chunk that sticks out of the row, put together from single entries; -inf outside
   __device__ __forceinline__ f32x4 edge(int c) const {
     f32x4 k;
-    if constexpr (TYPE == ST_TYPE_F32) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = c * 4 - pad + j;
-        k[j] = i >= 0 && i < n ? p[i] : -INFINITY;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t w = 0;
+    for (int w = 0; w < 4; ++w) {
+      if constexpr (TYPE == ST_TYPE_F32) {
+        const int i = c * 4 - pad + w;
+        k[w] = i >= 0 && i < n ? p[i] : -INFINITY;
+      } else {
+        uint32_t u = 0;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int i = c * 8 - pad + 2 * j + h;
-          const uint32_t v = i >= 0 && i < n ? (uint32_t)((const uint16_t*)p)[i] : TYPE == ST_TYPE_F16 ? 0xfc00u : 0xff80u;   // -inf
-          w |= v << (16 * h);
+          const int i = c * 8 - pad + 2 * w + h;
+          const uint32_t v = i >= 0 && i < n ? (uint32_t)((const uint16_t*)p)[i] : TYPE == ST_TYPE_F16 ? 0xfc00u : 0xff80u;
+          u |= v << (16 * h);
         }
-        k[j] = __uint_as_float(w);
+        k[w] = __uint_as_float(u);
       }
     }
     return k;
   }
-  // f(chunk, number) for this thread's chunks, from global memory: two loads under way at a time
-  template <class F> __device__ __forceinline__ void each_global(F f) const {
+  // f(chunk, number) for this thread's chunks, LOADS of them under way at a time.  A row is read again for each pass: it comes from
+  // the L2 or the last-level cache then, and with the workgroups that shared memory leaves room for that is faster than one copy of
+  // the row in shared memory (1024 x 19724: 69 us against 93) or in registers (98).
+  template <int LOADS, class F> __device__ __forceinline__ void each(F f) const {
     const int first = pad ? 1 : 0, last = (n + pad) / EPC, nt = blockDim.x;   // [first, last): in the row as a whole
     const f32x4* q = (const f32x4*)(p - pad);
 #pragma unroll 1
-    for (int c = first + (int)threadIdx.x; c < last; c += 2 * nt) {
-      const bool two = c + nt < last;
-      const f32x4 a = q[c], b = q[two ? c + nt : c];
-      f(a, c);
-      if (two) f(b, c + nt);
+    for (int c = first + (int)threadIdx.x; c < last; c += LOADS * nt) {
+      f32x4 k[LOADS];
+#pragma unroll
+      for (int u = 0; u < LOADS; ++u) k[u] = q[min(c + u * nt, last - 1)];
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int u = 0; u < LOADS; ++u)
+        if (c + u * nt < last) f(k[u], c + u * nt);
     }
     const int t = nt - 1 - (int)threadIdx.x;   // the last threads have the least to do
     const int c = t == 0 && first ? 0 : t == 1 && last >= first && last < chunks ? last : -1;
     if (c >= 0) f(edge(c), c);
   }
-  // the same from the copy in shared memory (LOCAL), or from global memory again
-  template <bool LOCAL, class F> __device__ __forceinline__ void each(const f32x4* local, F f) const {
-    if constexpr (LOCAL) {
-#pragma unroll 1
-      for (int c = threadIdx.x; c < chunks; c += blockDim.x) f(local[c], c);
-    } else {
-      each_global(f);
-    }
+  // f(logit, index) for the entries above -inf of which yes(logit) holds (it may hold for a NaN or -inf)
+  template <class Y, class F> __device__ __forceinline__ void each_if(Y yes, F f) const {
+    each<2>([&](f32x4 k, int c) SM_INLINE {
+      uint32_t hits = 0;
+#pragma unroll
+      for (int j = 0; j < EPC; ++j) hits |= (uint32_t)yes(entry(k, j)) << j;
+      while (hits) {
+        const int j = __builtin_ctz(hits);
+        hits &= hits - 1;
+        const float l = pick(k, j);
+        if (l > -INFINITY) f(l, c * EPC + j - pad);
+      }
+    });
   }
-  __device__ __forceinline__ int index(int c, int j) const { return c * EPC + j - pad; }
 };
 
 // ---- sums over the workgroup ---------------------------------------------------------------------------------------------
@@ -220,6 +234,10 @@ __device__ __forceinline__ u64 nucleus_target(float top_p, u64 S) {   // a mass 
 __device__ __forceinline__ u64 draw_target(float u, u64 S) {
   const u64 t = (u64)((double)u * (double)S);
   return t < S ? t : S - 1;
+}
+__device__ __forceinline__ void answer_none(const SampleArgs& a, int b) {
+  a.ids[b] = -1;
+  if (a.logp) a.logp[b] = -INFINITY;
 }
 __device__ __forceinline__ void answer(const SampleArgs& a, int b, int id, double w, u64 S) {
   a.ids[b] = id;
@@ -311,142 +329,95 @@ __device__ __forceinline__ void draw_from_sorted(const SampleArgs& a, int b, con
   if (e >= 0) answer(a, b, (int)(uint32_t)list[e], weight(sc, of_key((uint32_t)(list[e] >> 32))), S);
 }
 
-// One workgroup a row: the row in shared memory (LOCAL), or read again for each pass.
-// Dynamic shared memory: masses of the bins [nbin], a list of places [nbin / 2] (before that, counts of the bins), the row.
-template <int TYPE, bool LOCAL> __global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs a, int nbin) {
-  typedef typename LOf<TYPE>::t T;
-  constexpr int EPC = Row<TYPE>::EPC;
-  extern __shared__ __align__(16) char dyn[];
-  __shared__ Shared sh;
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, nt = blockDim.x, nw = nt >> 6;
-  if (a.n_dev && b >= *a.n_dev) return;
-  u64* const mass = (u64*)dyn;
-  u64* const list = mass + nbin;
-  uint32_t* const count = (uint32_t*)list;
-  f32x4* const local = (f32x4*)(list + nbin / 2);
-  const uint32_t room = nbin / 2;
-  const int s = a.idx ? a.idx[b] : b;
-  const Row<TYPE> r((const T*)a.logits + (size_t)b * a.ld, a.V);
-
-  float top = -INFINITY, low = -INFINITY;   // largest logit, largest negated one above -inf
-  r.each_global([&](f32x4 k, int c) SM_INLINE {
-    if constexpr (LOCAL) local[c] = k;
+// ---- passes over a row (or a part of one) ----------------------------------------------------------------------------------
+// the largest logit and the largest negated one above -inf: this thread's
+template <int TYPE> __device__ __forceinline__ void pass_top(const Row<TYPE>& r, float& top, float& low) {
+  top = low = -INFINITY;
+  r.template each<4>([&](f32x4 k, int) SM_INLINE {
 #pragma unroll
-    for (int j = 0; j < EPC; ++j) {
-      const float l = raw_logit<TYPE>(r.entry(k, j));
+    for (int j = 0; j < Row<TYPE>::EPC; ++j) {
+      const float l = r.entry(k, j);
       top = fmaxf(top, l);
       low = fmaxf(low, l > -INFINITY ? -l : -INFINITY);
     }
   });
-  const float own_max = top;
-  block_max2(top, low, sh);   // its barriers make the copy visible
-  if (top == -INFINITY) {
-    if (tid == 0) {
-      a.ids[b] = -1;
-      if (a.logp) a.logp[b] = -INFINITY;
-    }
-    return;
-  }
-  const Settings o = settings_of(a, s);
-  const bool greedy = !(o.temp > 0.0f) || o.top_k == 1;
-  const Scale sc = {top, 1.4426950408889634 / (double)fminf(o.temp, 3.4e38f)};
+}
 
-  // ---- lists: of the largest alone (greedy), of all entries of a short row, of those that can be among the top_k.  An entry goes
-  // to the list by one comparison, (top - l) * per_unit < to.
-  const bool by_top = !greedy && o.top_k > 0 && o.top_k <= nt / 2 && a.V > 256, all = !greedy && !by_top && a.V <= (int)room;
-  if (greedy || by_top || all) {
-    float per_unit = 0.0f, to = INFINITY;   // all: every product is 0 (or NaN under an infinite top)
-    if (tid == 0) sh.n = greedy ? 0xffffffffu : 0, sh.found_bin = 256;
-    if (by_top) {
-      // every thread has its largest entry, and the k-th largest of those is no larger than the k-th largest of all: 256 bins over
-      // them, the list takes its bin and those above it
-      float lowest = own_max > -INFINITY ? -own_max : -INFINITY, unused = 0.0f;
-      block_max2(lowest, unused, sh);
-      const BinMap map = {top, 255.0f / fmaxf(top + lowest, 1e-30f), 255.0f};
-      for (int i = tid; i < 256; i += nt) sh.digit_count[i] = 0;
-      __syncthreads();
-      if (own_max > -INFINITY) atomicAdd(&sh.digit_count[map.bin(own_max)], 1u);
-      __syncthreads();
-      if (tid < 64) {
-        uint32_t c[4], before = 0;
+// The list of the entries that can be among the k largest of the workgroup's: every thread has its largest one, and the k-th largest
+// of those is no larger than the k-th largest of all.  256 bins over them find it; the list takes its bin and those above.
+// -> how many, unsorted; more than room: not complete (too many in the last bin, or fewer than k threads have an entry)
+template <int TYPE, class I>
+__device__ __forceinline__ uint32_t gather_top(const Row<TYPE>& r, int k, float top, float own_max, u64* list, uint32_t room, Shared& sh, I index) {
+  const int tid = threadIdx.x, lane = tid & 63, nt = blockDim.x;
+  float lowest = own_max > -INFINITY ? -own_max : -INFINITY, unused = 0.0f;
+  block_max2(lowest, unused, sh);
+  const BinMap map = {top, 255.0f / fmaxf(top + lowest, 1e-30f), 255.0f};
+  for (int i = tid; i < 256; i += nt) sh.digit_count[i] = 0;
+  if (tid == 0) sh.n = 0, sh.found_bin = 256;
+  __syncthreads();
+  if (own_max > -INFINITY) atomicAdd(&sh.digit_count[map.bin(own_max)], 1u);
+  __syncthreads();
+  if (tid < 64) {
+    uint32_t c[4], before = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c[i] = sh.digit_count[4 * lane + i], before += c[i];
-        before = wave_scan(before, lane) - before;
+    for (int i = 0; i < 4; ++i) c[i] = sh.digit_count[4 * lane + i], before += c[i];
+    before = wave_scan(before, lane) - before;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (before < (uint32_t)o.top_k && (uint32_t)o.top_k <= before + c[i]) sh.found_bin = 4 * lane + i;
-          before += c[i];
-        }
-      }
-      per_unit = map.per_unit;
+    for (int i = 0; i < 4; ++i) {
+      if (before < (uint32_t)k && (uint32_t)k <= before + c[i]) sh.found_bin = 4 * lane + i;
+      before += c[i];
     }
-    __syncthreads();
-    const uint32_t cut = sh.found_bin;
-    if (by_top && cut < 255) to = (float)(cut + 1);
-    if (!by_top || cut < 256) {   // 256: fewer than top_k threads have an entry
-      const bool every = to == INFINITY;
-      r.template each<LOCAL>(local, [&](f32x4 k, int c) SM_INLINE {
-        uint32_t hits = 0;
-#pragma unroll
-        for (int j = 0; j < EPC; ++j) {
-          const float l = raw_logit<TYPE>(r.entry(k, j));
-          const bool in = greedy ? l == top : (every && l > -INFINITY) || (top - l) * per_unit < to || l == top;
-          hits |= (uint32_t)in << j;
-        }
-        if (hits) {
-#pragma unroll
-          for (int j = 0; j < EPC; ++j) {
-            if (!(hits >> j & 1)) continue;
-            const float l = raw_logit<TYPE>(r.entry(k, j));
-            if (greedy) {
-              atomicMin(&sh.n, (uint32_t)r.index(c, j));
-            } else if (l > -INFINITY) {
-              const uint32_t at = atomicAdd(&sh.n, 1u);
-              if (at < room) list[at] = place_of(l, r.index(c, j));
-            }
-          }
-        }
-      });
-      __syncthreads();
-      const uint32_t n = sh.n;
-      if (greedy) {
-        if (tid == 0) answer(a, b, (int)n, 1.0, ONE_MASS);
-        return;
-      }
-      __syncthreads();
-      if (n <= room) {
-        sort_places(list, (int)n, sh);
-        draw_from_sorted(a, b, list, o.top_k > 0 ? min((int)n, o.top_k) : (int)n, mass, sc, o, sh);
-        return;
-      }
-    }
-    __syncthreads();
-  }
-
-  // ---- bins, for any settings: masses (and counts, where a rank is asked for) in one pass over the row; they reach down to 32
-  // temperatures under the top (e^-32 < 2^-45: no mass beyond), or to the lowest logit if that is nearer
-  const BinMap map = {top, (float)nbin / fmaxf(fminf(32.0f * fminf(o.temp, 3.4e38f), top + low), 1e-30f), (float)(nbin - 1)};
-  const bool ranked = o.top_k > 0 && o.top_k < a.V;
-  for (int i = tid; i < nbin; i += nt) {
-    mass[i] = 0;
-    if (ranked) count[i] = 0;
   }
   __syncthreads();
+  const uint32_t cut = sh.found_bin;
+  if (cut > 255) return room + 1;
+  const float to = cut == 255 ? INFINITY : (float)(cut + 1);
+  r.each_if([&](float l) SM_INLINE { return map.place(l) < to || l == top || to == INFINITY; },
+            [&](float l, int i) SM_INLINE {
+              const uint32_t at = atomicAdd(&sh.n, 1u);
+              if (at < room) list[at] = place_of(l, index(i));
+            });
+  __syncthreads();
+  const uint32_t n = sh.n;
+  __syncthreads();
+  return n;
+}
+
+// bins reach down to 32 temperatures under the top (e^-32 < 2^-45: no mass beyond), or to the lowest logit if that is nearer
+__device__ __forceinline__ BinMap bins_of(const Settings& o, float top, float low, int nbin) {
+  return {top, (float)nbin / fmaxf(fminf(32.0f * fminf(o.temp, 3.4e38f), top + low), 1e-30f), (float)(nbin - 1)};
+}
+__device__ __forceinline__ Scale scale_of(const Settings& o, float top) { return {top, 1.4426950408889634 / (double)fminf(o.temp, 3.4e38f)}; }
+
+// masses (and counts, where a rank is asked for) of the bins; -> this thread's mass of the entries with w >= min_p
+template <int TYPE>
+__device__ __forceinline__ u64 pass_bins(const Row<TYPE>& r, const BinMap& map, const Scale& sc, const Settings& o, bool ranked, u64* mass, uint32_t* count) {
   u64 over = 0;
-  r.template each<LOCAL>(local, [&](f32x4 k, int) SM_INLINE {
+  r.template each<2>([&](f32x4 k, int) SM_INLINE {
 #pragma unroll
-    for (int j = 0; j < EPC; ++j) {
-      const float l = logit<TYPE>(r.entry(k, j));
-      const double w = l > -INFINITY ? weight(sc, l) : 0.0;
-      const u64 m = mass_of(w);
-      const int bin = map.bin(l);
-      if (m) atomicAdd(&mass[bin], m);
-      if (ranked && l > -INFINITY) atomicAdd(&count[bin], 1u);
-      if (w >= (double)o.min_p) over += m;
+    for (int j = 0; j < Row<TYPE>::EPC; ++j) {
+      const float l = r.entry(k, j);
+      if (l > -INFINITY) {
+        const double w = weight(sc, l);
+        const u64 m = mass_of(w);
+        const int bin = map.bin(l);
+        if (m) atomicAdd(&mass[bin], m);
+        if (ranked) atomicAdd(&count[bin], 1u);
+        if (w >= (double)o.min_p) over += m;
+      }
+      __builtin_amdgcn_sched_barrier(0);   // one entry's registers at a time
     }
   });
-  __syncthreads();
-  const int per = nbin / nt;
+  return over;
+}
+
+// ---- the answer from the bins ----------------------------------------------------------------------------------------------
+// list: room for nbin / 2 places; count may lie at the same address
+template <int TYPE>
+__device__ __forceinline__ void draw_from_bins(const SampleArgs& a, int b, const Row<TYPE>& r, const BinMap& map, const Scale& sc, const Settings& o, bool ranked,
+                               u64 over, int nbin, const u64* mass, const uint32_t* count, u64* list, Shared& sh) {
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, nt = blockDim.x, nw = nt >> 6, per = nbin / nt;
+  const uint32_t room = nbin / 2;
   u64 base_mass = 0;
   uint32_t base_count = 0;
   for (int i = 0; i < per; ++i) {
@@ -468,10 +439,8 @@ template <int TYPE, bool LOCAL> __global__ __launch_bounds__(1024) void sample_r
     S += sh.wave_u64[i];
     entries += sh.wave_u32[i];
   }
-  if (o.min_p > 0.0f) over = block_sum(over, sh);
-
-  // ---- three questions, each the entry at which the count or the mass of the walk exceeds a target: the top_k-th entry, the one
-  // that completes top_p, the drawn one.  First its bin, then the entry in the bin.
+  // three questions, each the entry at which the count or the mass of the walk exceeds a target: the top_k-th entry, the one that
+  // completes top_p, the drawn one.  First its bin, then the entry in the bin.
 #pragma unroll 1
   for (int question = 0; question < 3; ++question) {
     const bool by_count = question == 0;
@@ -507,34 +476,23 @@ template <int TYPE, bool LOCAL> __global__ __launch_bounds__(1024) void sample_r
     uint32_t before_count = by_count ? sh.found_count : 0;
     // the bin's entries: one list (the counts are not needed any more once the first question has its bin)
     const float from = (float)bin, to = bin == nbin - 1 ? INFINITY : (float)(bin + 1);
-    r.template each<LOCAL>(local, [&](f32x4 k, int c) SM_INLINE {
-      uint32_t hits = 0;
-#pragma unroll
-      for (int j = 0; j < EPC; ++j) {
-        const float l = raw_logit<TYPE>(r.entry(k, j)), at = map.place(l);
-        hits |= (uint32_t)((at >= from && (at < to || to == INFINITY)) || (bin == 0 && l == top)) << j;
-      }
-      if (hits) {
-#pragma unroll
-        for (int j = 0; j < EPC; ++j) {
-          const float l = raw_logit<TYPE>(r.entry(k, j));
-          if ((hits >> j & 1) && l > -INFINITY) {
-            const uint32_t at = atomicAdd(&sh.n, 1u);
-            if (at < room) list[at] = place_of(l, r.index(c, j));
-          }
-        }
-      }
-    });
+    r.each_if([&](float l) SM_INLINE {
+                const float at = map.place(l);
+                return (at >= from && (at < to || to == INFINITY)) || (bin == 0 && l == map.top);
+              },
+              [&](float l, int i) SM_INLINE {
+                const uint32_t at = atomicAdd(&sh.n, 1u);
+                if (at < room) list[at] = place_of(l, i);
+              });
     __syncthreads();
     const uint32_t n_bin = sh.n;
+    __syncthreads();
     // more of the row in one bin than the list holds (equal logits, mostly): the rounds below go over the row itself
     const bool from_row = n_bin > room;
     const int elements = from_row ? a.V : (int)n_bin;
     auto place_at = [&](int i) SM_INLINE {   // ~0: none
       if (!from_row) return list[i];
-      float l;
-      if constexpr (LOCAL) l = logit<TYPE>(((const T*)local)[i + r.pad]);
-      else l = logit<TYPE>(r.p[i]);
+      const float l = logit<TYPE>(r.p[i]);
       return l > -INFINITY && map.bin(l) == bin ? place_of(l, i) : ~0ull;
     };
     // eight bits of the place a round, from the highest one in which two elements differ, until one wave can compare the rest
@@ -543,38 +501,45 @@ template <int TYPE, bool LOCAL> __global__ __launch_bounds__(1024) void sample_r
 #pragma unroll 1
     for (;;) {
       auto inside = [&](u64 place) SM_INLINE { return place != ~0ull && (high >= 64 || (place >> high) == (prefix >> high)); };
-      u64 any = 0, every = ~0ull;
-      uint32_t n = 0;
+      uint32_t n = n_bin;
+      int top_bit = 64;
+      if (n_bin > 64 || from_row) {
+        u64 any = 0, every = ~0ull;
+        n = 0;
 #pragma unroll 1
-      for (int i = tid; i < elements; i += nt) {
-        const u64 place = place_at(i);
-        if (inside(place)) any |= place, every &= place, ++n;
-      }
+        for (int i = tid; i < elements; i += nt) {
+          const u64 place = place_at(i);
+          if (inside(place)) any |= place, every &= place, ++n;
+        }
 #pragma unroll
-      for (int d = 32; d > 0; d >>= 1) any |= __shfl_xor(any, d, 64), every &= __shfl_xor(every, d, 64), n += __shfl_xor(n, d, 64);
-      __syncthreads();
+        for (int d = 32; d > 0; d >>= 1) any |= __shfl_xor(any, d, 64), every &= __shfl_xor(every, d, 64), n += __shfl_xor(n, d, 64);
+        __syncthreads();
+        if (lane == 0) sh.wave_any[wv] = any, sh.wave_all[wv] = every, sh.wave_u32[wv] = n;
+        for (int i = tid; i < 256; i += nt) sh.digit_mass[i] = 0, sh.digit_count[i] = 0;
+        __syncthreads();
+        any = 0, every = ~0ull, n = 0;
+        for (int i = 0; i < nw; ++i) any |= sh.wave_any[i], every &= sh.wave_all[i], n += sh.wave_u32[i];
+        top_bit = 64 - __clzll(any ^ every);   // above the highest bit that differs (two places are never equal)
+        prefix = top_bit >= 64 ? 0 : (any >> top_bit) << top_bit;
+      }
       if (tid == 0) sh.n = 0;
-      if (lane == 0) sh.wave_any[wv] = any, sh.wave_all[wv] = every, sh.wave_u32[wv] = n;
-      for (int i = tid; i < 256; i += nt) sh.digit_mass[i] = 0, sh.digit_count[i] = 0;
       __syncthreads();
-      any = 0, every = ~0ull, n = 0;
-      for (int i = 0; i < nw; ++i) any |= sh.wave_any[i], every &= sh.wave_all[i], n += sh.wave_u32[i];
       const bool few = n <= 64;
-      const int top_bit = 64 - __clzll(any ^ every);   // above the highest bit that differs (two places are never equal)
       const int low_bit = top_bit > 8 ? top_bit - 8 : 0;
       // few: the digits' array takes the elements themselves, and their masses behind them
 #pragma unroll 1
       for (int i = tid; i < elements; i += nt) {
         const u64 place = place_at(i);
         if (!inside(place)) continue;
+        const u64 m = mass_of(weight(sc, of_key((uint32_t)(place >> 32))));
         if (few) {
           const uint32_t at = atomicAdd(&sh.n, 1u);
           sh.digit_mass[at] = place;
-          sh.digit_mass[64 + at] = mass_of(weight(sc, of_key((uint32_t)(place >> 32))));
+          sh.digit_mass[64 + at] = m;
         } else {
           const int d = (int)(place >> low_bit) & 255;
           if (by_count) atomicAdd(&sh.digit_count[d], 1u);
-          atomicAdd(&sh.digit_mass[d], mass_of(weight(sc, of_key((uint32_t)(place >> 32)))));
+          atomicAdd(&sh.digit_mass[d], m);
         }
       }
       __syncthreads();
@@ -609,7 +574,7 @@ template <int TYPE, bool LOCAL> __global__ __launch_bounds__(1024) void sample_r
         }
       }
       __syncthreads();
-      prefix = (top_bit >= 64 ? 0 : (any >> top_bit) << top_bit) | (u64)(sh.found_bin & 255) << low_bit;
+      prefix |= (u64)(sh.found_bin & 255) << low_bit;
       high = low_bit;
       before_count = sh.found_count;
       before_mass = sh.found_mass;
@@ -619,24 +584,282 @@ template <int TYPE, bool LOCAL> __global__ __launch_bounds__(1024) void sample_r
   if (tid == 0) answer(a, b, (int)(uint32_t)sh.found_place, weight(sc, of_key((uint32_t)(sh.found_place >> 32))), S);
 }
 
-template <int TYPE, bool LOCAL> int launch_rows(const SampleArgs& a, int nbin, int threads, size_t lds, hipStream_t st) {
-  ST_ENSURE_LDS((sample_row_kernel<TYPE, LOCAL>), 160 * 1024 - (int)sizeof(Shared));
-  hipLaunchKernelGGL((sample_row_kernel<TYPE, LOCAL>), dim3(a.B), dim3(threads), lds, st, a, nbin);
+// ---- kernels ---------------------------------------------------------------------------------------------------------------
+// What several workgroups of a row leave for each other, in the workspace; a row has
+//   u64 mass[NSPLIT], over; uint32 count[NSPLIT]; Part part[G]; float cand[G][KC]; int cand_index[G][KC]
+constexpr int NSPLIT = 4096, KC = 256, MAX_PARTS = 32;
+struct Part {
+  float top, low;
+  int first;      // index of its first largest entry (greedy rows)
+  int complete;   // cand holds its top_k (or all that it has)
+};
+struct RowSpace {
+  u64 *mass, *over;
+  uint32_t* count;
+  Part* part;
+  float* cand;
+  int* cand_index;
+};
+__host__ __device__ inline size_t row_space_bytes(int parts) {
+  return (size_t)NSPLIT * 12 + 256 + MAX_PARTS * sizeof(Part) + (size_t)parts * KC * 8;
+}
+__device__ __forceinline__ RowSpace row_space(void* ws, int b, int parts) {
+  char* p = (char*)ws + (size_t)b * row_space_bytes(parts);
+  RowSpace s;
+  s.mass = (u64*)p, p += (size_t)NSPLIT * 8;
+  s.count = (uint32_t*)p, p += (size_t)NSPLIT * 4;
+  s.over = (u64*)p, p += 256;
+  s.part = (Part*)p, p += MAX_PARTS * sizeof(Part);
+  s.cand = (float*)p, p += (size_t)parts * KC * 4;
+  s.cand_index = (int*)p;
+  return s;
+}
+__device__ __forceinline__ bool is_greedy(const Settings& o) { return !(o.temp > 0.0f) || o.top_k == 1; }
+// a list of the top_k can be had from the threads' largest entries
+__device__ __forceinline__ bool by_list(const Settings& o) { return o.top_k > 0 && o.top_k <= min((int)blockDim.x / 2, KC); }
+
+// One workgroup a row.  Dynamic shared memory: masses of the bins [nbin], a list of places [nbin / 2] (before that, counts).
+template <int TYPE> __global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs a, int nbin) {
+  typedef typename LOf<TYPE>::t T;
+  extern __shared__ __align__(16) char dyn[];
+  __shared__ Shared sh;
+  const int b = blockIdx.x, tid = threadIdx.x, nt = blockDim.x;
+  if (a.n_dev && b >= *a.n_dev) return;
+  u64* const mass = (u64*)dyn;
+  u64* const list = mass + nbin;
+  uint32_t* const count = (uint32_t*)list;
+  const uint32_t room = nbin / 2;
+  const Settings o = settings_of(a, a.idx ? a.idx[b] : b);
+  const Row<TYPE> r((const T*)a.logits + (size_t)b * a.ld, a.V);
+  float top, low;
+  pass_top(r, top, low);
+  const float own_max = top;
+  block_max2(top, low, sh);
+  if (top == -INFINITY) {
+    if (tid == 0) answer_none(a, b);
+    return;
+  }
+  if (is_greedy(o)) {
+    if (tid == 0) sh.n = 0xffffffffu;
+    __syncthreads();
+    r.each_if([&](float l) SM_INLINE { return l == top; }, [&](float, int i) SM_INLINE { atomicMin(&sh.n, (uint32_t)i); });
+    __syncthreads();
+    if (tid == 0) answer(a, b, (int)sh.n, 1.0, ONE_MASS);
+    return;
+  }
+  const Scale sc = scale_of(o, top);
+  if (by_list(o) || a.V <= (int)room) {
+    uint32_t n;
+    if (by_list(o) && a.V > 256) {
+      n = gather_top(r, o.top_k, top, own_max, list, room, sh, [](int i) SM_INLINE { return i; });
+    } else {
+      if (tid == 0) sh.n = 0;
+      __syncthreads();
+      r.each_if([](float l) SM_INLINE { return l > -INFINITY; }, [&](float l, int i) SM_INLINE {
+        const uint32_t at = atomicAdd(&sh.n, 1u);
+        if (at < room) list[at] = place_of(l, i);
+      });
+      __syncthreads();
+      n = sh.n;
+      __syncthreads();
+    }
+    if (n <= room) {
+      sort_places(list, (int)n, sh);
+      draw_from_sorted(a, b, list, o.top_k > 0 ? min((int)n, o.top_k) : (int)n, mass, sc, o, sh);
+      return;
+    }
+  }
+  const BinMap map = bins_of(o, top, low, nbin);
+  const bool ranked = o.top_k > 0 && o.top_k < a.V;
+  for (int i = tid; i < nbin; i += nt) {
+    mass[i] = 0;
+    if (ranked) count[i] = 0;
+  }
+  __syncthreads();
+  u64 over = pass_bins(r, map, sc, o, ranked, mass, count);
+  __syncthreads();
+  if (o.min_p > 0.0f) over = block_sum(over, sh);
+  draw_from_bins(a, b, r, map, sc, o, ranked, over, nbin, mass, count, list, sh);
+}
+
+// A long row over several workgroups, in three launches: (1) every part's largest entry, and its top_k where a list of them will do;
+// (2) masses of the bins, added up in the workspace (whole numbers: in any order the same); (3) one workgroup a row draws.
+template <int TYPE> __global__ __launch_bounds__(512) void sample_part_kernel(SampleArgs a, int parts, int len) {
+  typedef typename LOf<TYPE>::t T;
+  __shared__ Shared sh;
+  __shared__ u64 list[1024];
+  const int b = blockIdx.y, g = blockIdx.x, tid = threadIdx.x, nt = blockDim.x;
+  if (a.n_dev && b >= *a.n_dev) return;
+  const RowSpace ws = row_space(a.ws, b, parts);
+  for (int i = g * nt + tid; i < NSPLIT; i += parts * nt) ws.mass[i] = 0, ws.count[i] = 0;
+  if (g == 0 && tid == 0) *ws.over = 0;
+  const Settings o = settings_of(a, a.idx ? a.idx[b] : b);
+  const int i0 = g * len;
+  const Row<TYPE> r((const T*)a.logits + (size_t)b * a.ld + i0, min(len, a.V - i0));
+  float top, low;
+  pass_top(r, top, low);
+  const float own_max = top;
+  block_max2(top, low, sh);
+  int complete = 1;
+  if (tid == 0) sh.n = 0xffffffffu;
+  __syncthreads();
+  if (top > -INFINITY && is_greedy(o)) {
+    r.each_if([&](float l) SM_INLINE { return l == top; }, [&](float, int i) SM_INLINE { atomicMin(&sh.n, (uint32_t)(i0 + i)); });
+    __syncthreads();
+  } else if (by_list(o)) {
+    uint32_t n = 0;
+    if (top > -INFINITY) n = gather_top(r, o.top_k, top, own_max, list, 1024, sh, [&](int i) SM_INLINE { return i0 + i; });
+    complete = n <= 1024;
+    if (complete) {
+      if (n > (uint32_t)o.top_k) sort_places(list, (int)n, sh);
+      for (int i = tid; i < KC; i += nt) {
+        const bool in = i < (int)n && i < o.top_k;
+        ws.cand[g * KC + i] = in ? of_key((uint32_t)(list[i] >> 32)) : -INFINITY;
+        ws.cand_index[g * KC + i] = in ? (int)(uint32_t)list[i] : 0;
+      }
+    }
+  }
+  if (tid == 0) ws.part[g] = {top, low, (int)sh.n, complete};
+}
+
+// what all parts of a row have together
+__device__ __forceinline__ void join_parts(const RowSpace& ws, int parts, float& top, float& low, bool& complete, int& first) {
+  top = low = -INFINITY;
+  complete = true;
+  first = -1;
+  for (int g = 0; g < parts; ++g) {
+    const Part p = ws.part[g];
+    if (p.top > top) top = p.top, first = p.first;   // the first part of those with the largest
+    low = fmaxf(low, p.low);
+    complete = complete && p.complete;
+  }
+}
+
+template <int TYPE> __global__ __launch_bounds__(512) void sample_bins_kernel(SampleArgs a, int parts, int len) {
+  typedef typename LOf<TYPE>::t T;
+  extern __shared__ __align__(16) char dyn[];
+  __shared__ Shared sh;
+  const int b = blockIdx.y, g = blockIdx.x, tid = threadIdx.x, nt = blockDim.x;
+  if (a.n_dev && b >= *a.n_dev) return;
+  const RowSpace ws = row_space(a.ws, b, parts);
+  const Settings o = settings_of(a, a.idx ? a.idx[b] : b);
+  float top, low;
+  bool complete;
+  int first;
+  join_parts(ws, parts, top, low, complete, first);
+  if (top == -INFINITY || is_greedy(o) || (by_list(o) && complete)) return;   // no bins are needed
+  const int i0 = g * len;
+  const Row<TYPE> r((const T*)a.logits + (size_t)b * a.ld + i0, min(len, a.V - i0));
+  u64* const mass = (u64*)dyn;
+  uint32_t* const count = (uint32_t*)(mass + NSPLIT);
+  const bool ranked = o.top_k > 0 && o.top_k < a.V;
+  for (int i = tid; i < NSPLIT; i += nt) {
+    mass[i] = 0;
+    if (ranked) count[i] = 0;
+  }
+  __syncthreads();
+  u64 over = pass_bins(r, bins_of(o, top, low, NSPLIT), scale_of(o, top), o, ranked, mass, count);
+  if (o.min_p > 0.0f) {
+    over = block_sum(over, sh);
+    if (tid == 0 && over) atomicAdd(ws.over, over);
+  }
+  __syncthreads();
+  for (int i = tid; i < NSPLIT; i += nt) {
+    if (mass[i]) atomicAdd(&ws.mass[i], mass[i]);
+    if (ranked && count[i]) atomicAdd(&ws.count[i], count[i]);
+  }
+}
+
+template <int TYPE> __global__ __launch_bounds__(1024) void sample_join_kernel(SampleArgs a, int parts) {
+  typedef typename LOf<TYPE>::t T;
+  extern __shared__ __align__(16) char dyn[];
+  __shared__ Shared sh;
+  const int b = blockIdx.x, tid = threadIdx.x, nt = blockDim.x;
+  if (a.n_dev && b >= *a.n_dev) return;
+  const RowSpace ws = row_space(a.ws, b, parts);
+  const Settings o = settings_of(a, a.idx ? a.idx[b] : b);
+  u64* const mass = (u64*)dyn;
+  u64* const list = mass + NSPLIT;
+  uint32_t* const count = (uint32_t*)list;
+  const uint32_t room = NSPLIT / 2;
+  float top, low;
+  bool complete;
+  int first;
+  join_parts(ws, parts, top, low, complete, first);
+  if (top == -INFINITY || is_greedy(o)) {
+    if (tid == 0) {
+      if (top == -INFINITY) answer_none(a, b);
+      else answer(a, b, first, 1.0, ONE_MASS);
+    }
+    return;
+  }
+  const Scale sc = scale_of(o, top);
+  const Row<TYPE> r((const T*)a.logits + (size_t)b * a.ld, a.V);
+  const BinMap map = bins_of(o, top, low, NSPLIT);
+  const bool ranked = o.top_k > 0 && o.top_k < a.V;
+  u64 over = 0;
+  // (half of the part kernel's threads: what it took for a list is one here)
+  if (o.top_k > 0 && o.top_k <= KC && complete) {
+    const Row<ST_TYPE_F32> c(ws.cand, parts * KC);
+    float own, unused;
+    pass_top(c, own, unused);
+    const uint32_t n = gather_top(c, o.top_k, top, own, list, room, sh, [&](int i) SM_INLINE { return ws.cand_index[i]; });
+    if (n <= room) {
+      sort_places(list, (int)n, sh);
+      draw_from_sorted(a, b, list, min((int)n, o.top_k), mass, sc, o, sh);
+      return;
+    }
+    // too many of equal rank, or in too few threads: the bins after all, by this workgroup alone
+    for (int i = tid; i < NSPLIT; i += nt) mass[i] = 0, count[i] = 0;
+    __syncthreads();
+    over = pass_bins(r, map, sc, o, ranked, mass, count);
+    __syncthreads();
+    if (o.min_p > 0.0f) over = block_sum(over, sh);
+  } else {
+    for (int i = tid; i < NSPLIT; i += nt) {
+      mass[i] = ws.mass[i];
+      if (ranked) count[i] = ws.count[i];
+    }
+    over = *ws.over;
+    __syncthreads();
+  }
+  draw_from_bins(a, b, r, map, sc, o, ranked, over, NSPLIT, mass, count, list, sh);
+}
+
+// Parts of a row: few long rows leave most of the chip idle, and one workgroup takes its time over a long row
+int parts_of(int B, int V) {
+  if (V < 16384) return 1;
+  int g = 512 / B;
+  if (g > V / 4096) g = V / 4096;
+  if (g > MAX_PARTS) g = MAX_PARTS;
+  return g < 2 ? 1 : g;
+}
+
+template <int TYPE> int launch_type(const SampleArgs& a, hipStream_t st) {
+  const int parts = parts_of(a.B, a.V);
+  if (parts == 1) {
+    const int nbin = a.V <= 1024 ? 2048 : a.V <= 16384 ? 1024 : a.V <= 65536 ? 2048 : 4096;
+    const int threads = a.V <= 2048 ? 256 : 512;
+    hipLaunchKernelGGL((sample_row_kernel<TYPE>), dim3(a.B), dim3(threads), (size_t)nbin * 12, st, a, nbin);
+    ST_LAUNCH_CHECK();
+    return ST_OK;
+  }
+  const int len = ((a.V + parts - 1) / parts + 63) / 64 * 64, n = (a.V + len - 1) / len;   // n: parts that have entries
+  hipLaunchKernelGGL((sample_part_kernel<TYPE>), dim3(n, a.B), dim3(512), 0, st, a, n, len);
+  ST_LAUNCH_CHECK();
+  hipLaunchKernelGGL((sample_bins_kernel<TYPE>), dim3(n, a.B), dim3(512), (size_t)NSPLIT * 12, st, a, n, len);
+  ST_LAUNCH_CHECK();
+  hipLaunchKernelGGL((sample_join_kernel<TYPE>), dim3(a.B), dim3(1024), (size_t)NSPLIT * 12, st, a, n);
   ST_LAUNCH_CHECK();
   return ST_OK;
-}
-template <int TYPE> int launch_type(const SampleArgs& a, hipStream_t st) {
-  const size_t row = ((size_t)a.V * sizeof(typename LOf<TYPE>::t) + 31) / 16 * 16;
-  const int nbin = a.V <= 1024 ? 2048 : a.V <= 16384 ? 1024 : a.V <= 65536 ? 2048 : 4096;
-  const int threads = a.V <= 2048 ? 256 : a.B >= 1024 && a.V <= 16384 ? 512 : 1024;
-  const size_t lds = (size_t)nbin * 12;
-  if (lds + row <= 128 * 1024) return launch_rows<TYPE, true>(a, nbin, threads, lds + row, st);
-  return launch_rows<TYPE, false>(a, nbin, threads, lds, st);
 }
 
 }  // namespace
 
-size_t sample_workspace(int, int) { return 0; }
+size_t sample_workspace(int B, int V) {
+  const int parts = parts_of(B, V);
+  return parts == 1 ? 0 : (size_t)B * row_space_bytes(parts);
+}
 
 int sample_launch(const SampleArgs& a, hipStream_t st) {
   return a.type == ST_TYPE_F32 ? launch_type<ST_TYPE_F32>(a, st) : a.type == ST_TYPE_BF16 ? launch_type<ST_TYPE_BF16>(a, st) : launch_type<ST_TYPE_F16>(a, st);
@@ -663,6 +886,7 @@ extern "C" int st_sample_logits(const void* logits, int type, int64_t ld, int B,
   ST_CHECK_ARG(logits && u && ids, "NULL buffer");
   ST_CHECK_ARG(((size_t)logits & (type == ST_TYPE_F32 ? 3 : 1)) == 0, "logits must lie on their type's size");
   ST_CHECK_ARG(ld >= 0, "ld=%lld", (long long)ld);
+  ST_CHECK_ARG(((size_t)workspace & 15) == 0, "the workspace must lie on 16 bytes");
   const size_t need = sample_workspace(B, V);
   if (need > workspace_bytes || (need && !workspace)) {
     st_set_error("workspace too small: need %zu bytes, have %zu", need, workspace ? workspace_bytes : (size_t)0);
