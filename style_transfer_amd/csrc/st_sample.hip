@@ -144,8 +144,8 @@ template <int TYPE> struct Row {
     if (c >= 0) f(edge(c), c);
   }
   // f(logit, index) for the entries above -inf of which yes(logit) holds (it may hold for a NaN or -inf)
-  template <class Y, class F> __device__ __forceinline__ void each_if(Y yes, F f) const {
-    each<2>([&](f32x4 k, int c) SM_INLINE {
+  template <int LOADS, class Y, class F> __device__ __forceinline__ void each_if(Y yes, F f) const {
+    each<LOADS>([&](f32x4 k, int c) SM_INLINE {
       uint32_t hits = 0;
 #pragma unroll
       for (int j = 0; j < EPC; ++j) hits |= (uint32_t)yes(entry(k, j)) << j;
@@ -170,38 +170,55 @@ struct Shared {
   uint32_t found_count, found_bin, n;
 };
 
-__device__ __forceinline__ u64 wave_scan(u64 v, int lane) {   // inclusive
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const u64 u = __shfl_up(v, o, 64);
-    if (lane >= o) v += u;
-  }
+// Sums over the lanes up to this one, by row shifts and row broadcasts: no way through shared memory
+#define SM_DPP(v, ctrl, rows) __builtin_amdgcn_update_dpp(0, (int)(v), ctrl, rows, 0xf, false)
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v, int) {
+  v += SM_DPP(v, 0x111, 0xf);   // row_shr:1, 2, 4, 8 (lanes from outside a row of 16 count 0)
+  v += SM_DPP(v, 0x112, 0xf);
+  v += SM_DPP(v, 0x114, 0xf);
+  v += SM_DPP(v, 0x118, 0xf);
+  v += SM_DPP(v, 0x142, 0xa);   // row_bcast:15 into rows 1 and 3
+  v += SM_DPP(v, 0x143, 0xc);   // row_bcast:31 into rows 2 and 3
   return v;
 }
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t u = __shfl_up(v, o, 64);
-    if (lane >= o) v += u;
-  }
+__device__ __forceinline__ u64 wave_scan(u64 v, int) {
+#define SM_ADD(ctrl, rows) v += (u64)(uint32_t)SM_DPP(v >> 32, ctrl, rows) << 32 | (uint32_t)SM_DPP(v, ctrl, rows)
+  SM_ADD(0x111, 0xf);
+  SM_ADD(0x112, 0xf);
+  SM_ADD(0x114, 0xf);
+  SM_ADD(0x118, 0xf);
+  SM_ADD(0x142, 0xa);
+  SM_ADD(0x143, 0xc);
+#undef SM_ADD
   return v;
 }
 __device__ __forceinline__ u64 block_sum(u64 v, Shared& sh) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  v = wave_scan(v, 0);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh.wave_u64[threadIdx.x >> 6] = v;
+  if ((threadIdx.x & 63) == 63) sh.wave_u64[threadIdx.x >> 6] = v;
   __syncthreads();
   u64 s = 0;
   for (int i = 0; i < (int)(blockDim.x >> 6); ++i) s += sh.wave_u64[i];
   return s;
 }
+__device__ __forceinline__ float wave_largest(float v) {   // in lane 63
+#define SM_MAX(ctrl, rows) \
+  v = fmaxf(v, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp((int)0xff800000, (int)__float_as_uint(v), ctrl, rows, 0xf, false)))
+  SM_MAX(0x111, 0xf);
+  SM_MAX(0x112, 0xf);
+  SM_MAX(0x114, 0xf);
+  SM_MAX(0x118, 0xf);
+  SM_MAX(0x142, 0xa);
+  SM_MAX(0x143, 0xc);
+#undef SM_MAX
+  return v;
+}
 // (largest a, largest b) over the workgroup
 __device__ __forceinline__ void block_max2(float& a, float& b, Shared& sh) {
-  a = wave_max(a);
-  b = wave_max(b);
+  a = wave_largest(a);
+  b = wave_largest(b);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh.wave_f[threadIdx.x >> 6] = a, sh.wave_f[16 + (threadIdx.x >> 6)] = b;
+  if ((threadIdx.x & 63) == 63) sh.wave_f[threadIdx.x >> 6] = a, sh.wave_f[16 + (threadIdx.x >> 6)] = b;
   __syncthreads();
   for (int i = 0; i < (int)(blockDim.x >> 6); ++i) a = fmaxf(a, sh.wave_f[i]), b = fmaxf(b, sh.wave_f[16 + i]);
 }
@@ -346,7 +363,7 @@ template <int TYPE> __device__ __forceinline__ void pass_top(const Row<TYPE>& r,
 // The list of the entries that can be among the k largest of the workgroup's: every thread has its largest one, and the k-th largest
 // of those is no larger than the k-th largest of all.  256 bins over them find it; the list takes its bin and those above.
 // -> how many, unsorted; more than room: not complete (too many in the last bin, or fewer than k threads have an entry)
-template <int TYPE, class I>
+template <int LOADS, int TYPE, class I>
 __device__ __forceinline__ uint32_t gather_top(const Row<TYPE>& r, int k, float top, float own_max, u64* list, uint32_t room, Shared& sh, I index) {
   const int tid = threadIdx.x, lane = tid & 63, nt = blockDim.x;
   float lowest = own_max > -INFINITY ? -own_max : -INFINITY, unused = 0.0f;
@@ -372,7 +389,7 @@ __device__ __forceinline__ uint32_t gather_top(const Row<TYPE>& r, int k, float 
   const uint32_t cut = sh.found_bin;
   if (cut > 255) return room + 1;
   const float to = cut == 255 ? INFINITY : (float)(cut + 1);
-  r.each_if([&](float l) SM_INLINE { return map.place(l) < to || l == top || to == INFINITY; },
+  r.template each_if<LOADS>([&](float l) SM_INLINE { return map.place(l) < to || l == top || to == INFINITY; },
             [&](float l, int i) SM_INLINE {
               const uint32_t at = atomicAdd(&sh.n, 1u);
               if (at < room) list[at] = place_of(l, index(i));
@@ -413,7 +430,7 @@ __device__ __forceinline__ u64 pass_bins(const Row<TYPE>& r, const BinMap& map, 
 
 // ---- the answer from the bins ----------------------------------------------------------------------------------------------
 // list: room for nbin / 2 places; count may lie at the same address
-template <int TYPE>
+template <int LOADS, int TYPE>
 __device__ __forceinline__ void draw_from_bins(const SampleArgs& a, int b, const Row<TYPE>& r, const BinMap& map, const Scale& sc, const Settings& o, bool ranked,
                                u64 over, int nbin, const u64* mass, const uint32_t* count, u64* list, Shared& sh) {
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, nt = blockDim.x, nw = nt >> 6, per = nbin / nt;
@@ -476,41 +493,41 @@ __device__ __forceinline__ void draw_from_bins(const SampleArgs& a, int b, const
     uint32_t before_count = by_count ? sh.found_count : 0;
     // the bin's entries: one list (the counts are not needed any more once the first question has its bin)
     const float from = (float)bin, to = bin == nbin - 1 ? INFINITY : (float)(bin + 1);
-    r.each_if([&](float l) SM_INLINE {
-                const float at = map.place(l);
-                return (at >= from && (at < to || to == INFINITY)) || (bin == 0 && l == map.top);
-              },
-              [&](float l, int i) SM_INLINE {
-                const uint32_t at = atomicAdd(&sh.n, 1u);
-                if (at < room) list[at] = place_of(l, i);
-              });
+    auto in_bin = [&](float l) SM_INLINE {
+      const float at = map.place(l);
+      return (at >= from && (at < to || to == INFINITY)) || (bin == 0 && l == map.top);
+    };
+    r.template each_if<LOADS>(in_bin, [&](float l, int i) SM_INLINE {
+      const uint32_t at = atomicAdd(&sh.n, 1u);
+      if (at < room) list[at] = place_of(l, i);
+    });
     __syncthreads();
     const uint32_t n_bin = sh.n;
     __syncthreads();
     // more of the row in one bin than the list holds (equal logits, mostly): the rounds below go over the row itself
     const bool from_row = n_bin > room;
-    const int elements = from_row ? a.V : (int)n_bin;
-    auto place_at = [&](int i) SM_INLINE {   // ~0: none
-      if (!from_row) return list[i];
-      const float l = logit<TYPE>(r.p[i]);
-      return l > -INFINITY && map.bin(l) == bin ? place_of(l, i) : ~0ull;
+    auto walk = [&](auto f) SM_INLINE {   // f(place) for this thread's share of the bin
+      if (from_row) {
+        r.template each_if<LOADS>(in_bin, [&](float l, int i) SM_INLINE { f(place_of(l, i)); });
+      } else {
+#pragma unroll 1
+        for (uint32_t i = tid; i < n_bin; i += nt) f(list[i]);
+      }
     };
     // eight bits of the place a round, from the highest one in which two elements differ, until one wave can compare the rest
     u64 prefix = 0;
     int high = 64;   // the bits from `high` on are settled: prefix's
 #pragma unroll 1
     for (;;) {
-      auto inside = [&](u64 place) SM_INLINE { return place != ~0ull && (high >= 64 || (place >> high) == (prefix >> high)); };
+      auto inside = [&](u64 place) SM_INLINE { return high >= 64 || (place >> high) == (prefix >> high); };
       uint32_t n = n_bin;
       int top_bit = 64;
       if (n_bin > 64 || from_row) {
         u64 any = 0, every = ~0ull;
         n = 0;
-#pragma unroll 1
-        for (int i = tid; i < elements; i += nt) {
-          const u64 place = place_at(i);
+        walk([&](u64 place) SM_INLINE {
           if (inside(place)) any |= place, every &= place, ++n;
-        }
+        });
 #pragma unroll
         for (int d = 32; d > 0; d >>= 1) any |= __shfl_xor(any, d, 64), every &= __shfl_xor(every, d, 64), n += __shfl_xor(n, d, 64);
         __syncthreads();
@@ -527,10 +544,8 @@ __device__ __forceinline__ void draw_from_bins(const SampleArgs& a, int b, const
       const bool few = n <= 64;
       const int low_bit = top_bit > 8 ? top_bit - 8 : 0;
       // few: the digits' array takes the elements themselves, and their masses behind them
-#pragma unroll 1
-      for (int i = tid; i < elements; i += nt) {
-        const u64 place = place_at(i);
-        if (!inside(place)) continue;
+      walk([&](u64 place) SM_INLINE {
+        if (!inside(place)) return;
         const u64 m = mass_of(weight(sc, of_key((uint32_t)(place >> 32))));
         if (few) {
           const uint32_t at = atomicAdd(&sh.n, 1u);
@@ -541,7 +556,7 @@ __device__ __forceinline__ void draw_from_bins(const SampleArgs& a, int b, const
           if (by_count) atomicAdd(&sh.digit_count[d], 1u);
           atomicAdd(&sh.digit_mass[d], m);
         }
-      }
+      });
       __syncthreads();
       if (few) {
         if (wv == 0) {
@@ -615,8 +630,8 @@ __device__ __forceinline__ RowSpace row_space(void* ws, int b, int parts) {
   return s;
 }
 __device__ __forceinline__ bool is_greedy(const Settings& o) { return !(o.temp > 0.0f) || o.top_k == 1; }
-// a list of the top_k can be had from the threads' largest entries
-__device__ __forceinline__ bool by_list(const Settings& o) { return o.top_k > 0 && o.top_k <= min((int)blockDim.x / 2, KC); }
+// a list of the top_k can be had from the threads' largest entries, twice as many as are asked for
+__device__ __forceinline__ bool by_list(const Settings& o, int chunks) { return o.top_k > 0 && o.top_k <= min(min((int)blockDim.x, chunks) / 2, KC); }
 
 // One workgroup a row.  Dynamic shared memory: masses of the bins [nbin], a list of places [nbin / 2] (before that, counts).
 template <int TYPE> __global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs a, int nbin) {
@@ -642,20 +657,21 @@ template <int TYPE> __global__ __launch_bounds__(1024) void sample_row_kernel(Sa
   if (is_greedy(o)) {
     if (tid == 0) sh.n = 0xffffffffu;
     __syncthreads();
-    r.each_if([&](float l) SM_INLINE { return l == top; }, [&](float, int i) SM_INLINE { atomicMin(&sh.n, (uint32_t)i); });
+    r.template each_if<4>([&](float l) SM_INLINE { return l == top; }, [&](float, int i) SM_INLINE { atomicMin(&sh.n, (uint32_t)i); });
     __syncthreads();
     if (tid == 0) answer(a, b, (int)sh.n, 1.0, ONE_MASS);
     return;
   }
   const Scale sc = scale_of(o, top);
-  if (by_list(o) || a.V <= (int)room) {
+  const bool listed = by_list(o, r.chunks);
+  if (listed || a.V <= (int)room) {
     uint32_t n;
-    if (by_list(o) && a.V > 256) {
-      n = gather_top(r, o.top_k, top, own_max, list, room, sh, [](int i) SM_INLINE { return i; });
+    if (listed && a.V > 256) {
+      n = gather_top<4>(r, o.top_k, top, own_max, list, room, sh, [](int i) SM_INLINE { return i; });
     } else {
       if (tid == 0) sh.n = 0;
       __syncthreads();
-      r.each_if([](float l) SM_INLINE { return l > -INFINITY; }, [&](float l, int i) SM_INLINE {
+      r.template each_if<2>([](float l) SM_INLINE { return l > -INFINITY; }, [&](float l, int i) SM_INLINE {
         const uint32_t at = atomicAdd(&sh.n, 1u);
         if (at < room) list[at] = place_of(l, i);
       });
@@ -679,7 +695,7 @@ template <int TYPE> __global__ __launch_bounds__(1024) void sample_row_kernel(Sa
   u64 over = pass_bins(r, map, sc, o, ranked, mass, count);
   __syncthreads();
   if (o.min_p > 0.0f) over = block_sum(over, sh);
-  draw_from_bins(a, b, r, map, sc, o, ranked, over, nbin, mass, count, list, sh);
+  draw_from_bins<4>(a, b, r, map, sc, o, ranked, over, nbin, mass, count, list, sh);
 }
 
 // A long row over several workgroups, in three launches: (1) every part's largest entry, and its top_k where a list of them will do;
@@ -704,11 +720,11 @@ template <int TYPE> __global__ __launch_bounds__(512) void sample_part_kernel(Sa
   if (tid == 0) sh.n = 0xffffffffu;
   __syncthreads();
   if (top > -INFINITY && is_greedy(o)) {
-    r.each_if([&](float l) SM_INLINE { return l == top; }, [&](float, int i) SM_INLINE { atomicMin(&sh.n, (uint32_t)(i0 + i)); });
+    r.template each_if<4>([&](float l) SM_INLINE { return l == top; }, [&](float, int i) SM_INLINE { atomicMin(&sh.n, (uint32_t)(i0 + i)); });
     __syncthreads();
-  } else if (by_list(o)) {
+  } else if (by_list(o, 1024)) {
     uint32_t n = 0;
-    if (top > -INFINITY) n = gather_top(r, o.top_k, top, own_max, list, 1024, sh, [&](int i) SM_INLINE { return i0 + i; });
+    if (top > -INFINITY) n = gather_top<4>(r, o.top_k, top, own_max, list, 1024, sh, [&](int i) SM_INLINE { return i0 + i; });
     complete = n <= 1024;
     if (complete) {
       if (n > (uint32_t)o.top_k) sort_places(list, (int)n, sh);
@@ -722,17 +738,15 @@ template <int TYPE> __global__ __launch_bounds__(512) void sample_part_kernel(Sa
   if (tid == 0) ws.part[g] = {top, low, (int)sh.n, complete};
 }
 
-// what all parts of a row have together
+// what all parts of a row have together, a lane a part (every wave for itself)
 __device__ __forceinline__ void join_parts(const RowSpace& ws, int parts, float& top, float& low, bool& complete, int& first) {
-  top = low = -INFINITY;
-  complete = true;
-  first = -1;
-  for (int g = 0; g < parts; ++g) {
-    const Part p = ws.part[g];
-    if (p.top > top) top = p.top, first = p.first;   // the first part of those with the largest
-    low = fmaxf(low, p.low);
-    complete = complete && p.complete;
-  }
+  const int lane = threadIdx.x & 63;
+  Part p = {-INFINITY, -INFINITY, -1, 1};
+  if (lane < parts) p = ws.part[lane];
+  top = __shfl(wave_largest(p.top), 63, 64);
+  low = __shfl(wave_largest(p.low), 63, 64);
+  complete = __ballot(!p.complete) == 0;
+  first = __shfl(p.first, __ffsll(__ballot(p.top == top)) - 1, 64);   // of the first part with the largest
 }
 
 template <int TYPE> __global__ __launch_bounds__(512) void sample_bins_kernel(SampleArgs a, int parts, int len) {
@@ -747,7 +761,7 @@ template <int TYPE> __global__ __launch_bounds__(512) void sample_bins_kernel(Sa
   bool complete;
   int first;
   join_parts(ws, parts, top, low, complete, first);
-  if (top == -INFINITY || is_greedy(o) || (by_list(o) && complete)) return;   // no bins are needed
+  if (top == -INFINITY || is_greedy(o) || (by_list(o, 1024) && complete)) return;   // no bins are needed
   const int i0 = g * len;
   const Row<TYPE> r((const T*)a.logits + (size_t)b * a.ld + i0, min(len, a.V - i0));
   u64* const mass = (u64*)dyn;
@@ -803,7 +817,7 @@ template <int TYPE> __global__ __launch_bounds__(1024) void sample_join_kernel(S
     const Row<ST_TYPE_F32> c(ws.cand, parts * KC);
     float own, unused;
     pass_top(c, own, unused);
-    const uint32_t n = gather_top(c, o.top_k, top, own, list, room, sh, [&](int i) SM_INLINE { return ws.cand_index[i]; });
+    const uint32_t n = gather_top<4>(c, o.top_k, top, own, list, room, sh, [&](int i) SM_INLINE { return ws.cand_index[i]; });
     if (n <= room) {
       sort_places(list, (int)n, sh);
       draw_from_sorted(a, b, list, min((int)n, o.top_k), mass, sc, o, sh);
@@ -823,7 +837,7 @@ template <int TYPE> __global__ __launch_bounds__(1024) void sample_join_kernel(S
     over = *ws.over;
     __syncthreads();
   }
-  draw_from_bins(a, b, r, map, sc, o, ranked, over, NSPLIT, mass, count, list, sh);
+  draw_from_bins<8>(a, b, r, map, sc, o, ranked, over, NSPLIT, mass, count, list, sh);
 }
 
 // Parts of a row: few long rows leave most of the chip idle, and one workgroup takes its time over a long row
