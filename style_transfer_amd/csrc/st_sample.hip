@@ -168,6 +168,7 @@ struct Shared {
   float wave_f[32];
   u64 found_place, found_mass;
   uint32_t found_count, found_bin, n;
+  uint32_t part_end[32], part_at[32];
 };
 
 // Sums over the lanes up to this one, by row shifts and row broadcasts: no way through shared memory
@@ -408,7 +409,7 @@ __device__ __forceinline__ Scale scale_of(const Settings& o, float top) { return
 
 // masses (and counts, where a rank is asked for) of the bins; -> this thread's mass of the entries with w >= min_p
 template <int TYPE>
-__device__ __forceinline__ u64 pass_bins(const Row<TYPE>& r, const BinMap& map, const Scale& sc, const Settings& o, bool ranked, u64* mass, uint32_t* count) {
+__device__ __forceinline__ u64 pass_bins(const Row<TYPE>& r, const BinMap& map, const Scale& sc, const Settings& o, bool counted, u64* mass, uint32_t* count) {
   u64 over = 0;
   r.template each<2>([&](f32x4 k, int) SM_INLINE {
 #pragma unroll
@@ -419,7 +420,7 @@ __device__ __forceinline__ u64 pass_bins(const Row<TYPE>& r, const BinMap& map, 
         const u64 m = mass_of(w);
         const int bin = map.bin(l);
         if (m) atomicAdd(&mass[bin], m);
-        if (ranked) atomicAdd(&count[bin], 1u);
+        if (counted) atomicAdd(&count[bin], 1u);
         if (w >= (double)o.min_p) over += m;
       }
       __builtin_amdgcn_sched_barrier(0);   // one entry's registers at a time
@@ -428,13 +429,49 @@ __device__ __forceinline__ u64 pass_bins(const Row<TYPE>& r, const BinMap& map, 
   return over;
 }
 
+// What several workgroups of a row leave for each other, in the workspace; a row has
+//   u64 mass[NSPLIT], over; uint32 count[NSPLIT]; Part part[32]; float cand[parts][KC]; int cand_index[parts][KC];
+//   uint32 offset[parts][NSPLIT + 64]; uint16 order[parts][len]: the part's entries by bins, and where a bin of it begins
+constexpr int NSPLIT = 4096, KC = 256, MAX_PARTS = 32, OFFSETS = NSPLIT + 64;
+struct Part {
+  float top, low;
+  int first;      // index of its first largest entry (greedy rows)
+  int complete;   // cand holds its top_k (or all that it has)
+};
+struct RowSpace {
+  u64 *mass, *over;
+  uint32_t* count;
+  Part* part;
+  float* cand;
+  int* cand_index;
+  uint32_t* offset;
+  uint16_t* order;
+};
+__host__ __device__ inline size_t row_space_bytes(int parts, int len) {   // len: a multiple of 64
+  return (size_t)NSPLIT * 12 + 256 + MAX_PARTS * sizeof(Part) + (size_t)parts * (KC * 8 + OFFSETS * 4 + (size_t)len * 2);
+}
+__device__ __forceinline__ RowSpace row_space(void* ws, int b, int parts, int len) {
+  char* p = (char*)ws + (size_t)b * row_space_bytes(parts, len);
+  RowSpace s;
+  s.mass = (u64*)p, p += (size_t)NSPLIT * 8;
+  s.count = (uint32_t*)p, p += (size_t)NSPLIT * 4;
+  s.over = (u64*)p, p += 256;
+  s.part = (Part*)p, p += MAX_PARTS * sizeof(Part);
+  s.cand = (float*)p, p += (size_t)parts * KC * 4;
+  s.cand_index = (int*)p, p += (size_t)parts * KC * 4;
+  s.offset = (uint32_t*)p, p += (size_t)parts * OFFSETS * 4;
+  s.order = (uint16_t*)p;
+  return s;
+}
+
 // ---- the answer from the bins ----------------------------------------------------------------------------------------------
-// list: room for nbin / 2 places; count may lie at the same address
-template <int LOADS, int TYPE>
+// list: room for so many places; count may lie at the same address.  SPLIT: the bins' entries are found in the parts' order, not in
+// the row.
+template <bool SPLIT, int TYPE>
 __device__ __forceinline__ void draw_from_bins(const SampleArgs& a, int b, const Row<TYPE>& r, const BinMap& map, const Scale& sc, const Settings& o, bool ranked,
-                               u64 over, int nbin, const u64* mass, const uint32_t* count, u64* list, Shared& sh) {
+                               u64 over, int nbin, const u64* mass, const uint32_t* count, u64* list, uint32_t room, Shared& sh,
+                               const RowSpace& ws, int parts, int len) {
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, nt = blockDim.x, nw = nt >> 6, per = nbin / nt;
-  const uint32_t room = nbin / 2;
   u64 base_mass = 0;
   uint32_t base_count = 0;
   for (int i = 0; i < per; ++i) {
@@ -497,21 +534,44 @@ __device__ __forceinline__ void draw_from_bins(const SampleArgs& a, int b, const
       const float at = map.place(l);
       return (at >= from && (at < to || to == INFINITY)) || (bin == 0 && l == map.top);
     };
-    r.template each_if<LOADS>(in_bin, [&](float l, int i) SM_INLINE {
-      const uint32_t at = atomicAdd(&sh.n, 1u);
-      if (at < room) list[at] = place_of(l, i);
-    });
+    auto element = [&](uint32_t t) SM_INLINE {   // SPLIT: the place of the bin's t-th entry
+      int g = 0;
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) g += sh.part_end[g + d - 1] <= t ? d : 0;
+      const int i = g * len + ws.order[(size_t)g * len + (uint32_t)(sh.part_at[g] + t)];   // (the sum, modulo 2^32, is the place in the part)
+      return place_of(logit<TYPE>(r.p[i]), i);
+    };
+    if constexpr (SPLIT) {
+      if (wv == 0) {
+        uint32_t from_at = 0, n = 0;
+        if (lane < parts) {
+          from_at = ws.offset[(size_t)lane * OFFSETS + bin];
+          n = ws.offset[(size_t)lane * OFFSETS + bin + 1] - from_at;
+        }
+        const uint32_t end = wave_scan(n, lane);
+        if (lane < MAX_PARTS) sh.part_end[lane] = end, sh.part_at[lane] = from_at - (end - n);
+        if (lane == 63) sh.n = end;
+      }
+      __syncthreads();
+      if (sh.n <= room)
+        for (uint32_t t = tid; t < sh.n; t += nt) list[t] = element(t);
+    } else {
+      r.template each_if<4>(in_bin, [&](float l, int i) SM_INLINE {
+        const uint32_t at = atomicAdd(&sh.n, 1u);
+        if (at < room) list[at] = place_of(l, i);
+      });
+    }
     __syncthreads();
     const uint32_t n_bin = sh.n;
     __syncthreads();
     // more of the row in one bin than the list holds (equal logits, mostly): the rounds below go over the row itself
     const bool from_row = n_bin > room;
     auto walk = [&](auto f) SM_INLINE {   // f(place) for this thread's share of the bin
-      if (from_row) {
-        r.template each_if<LOADS>(in_bin, [&](float l, int i) SM_INLINE { f(place_of(l, i)); });
-      } else {
+      if (SPLIT || !from_row) {
 #pragma unroll 1
-        for (uint32_t i = tid; i < n_bin; i += nt) f(list[i]);
+        for (uint32_t i = tid; i < n_bin; i += nt) f(SPLIT && from_row ? element(i) : list[i]);
+      } else if constexpr (!SPLIT) {
+        r.template each_if<4>(in_bin, [&](float l, int i) SM_INLINE { f(place_of(l, i)); });
       }
     };
     // eight bits of the place a round, from the highest one in which two elements differ, until one wave can compare the rest
@@ -600,35 +660,6 @@ __device__ __forceinline__ void draw_from_bins(const SampleArgs& a, int b, const
 }
 
 // ---- kernels ---------------------------------------------------------------------------------------------------------------
-// What several workgroups of a row leave for each other, in the workspace; a row has
-//   u64 mass[NSPLIT], over; uint32 count[NSPLIT]; Part part[G]; float cand[G][KC]; int cand_index[G][KC]
-constexpr int NSPLIT = 4096, KC = 256, MAX_PARTS = 32;
-struct Part {
-  float top, low;
-  int first;      // index of its first largest entry (greedy rows)
-  int complete;   // cand holds its top_k (or all that it has)
-};
-struct RowSpace {
-  u64 *mass, *over;
-  uint32_t* count;
-  Part* part;
-  float* cand;
-  int* cand_index;
-};
-__host__ __device__ inline size_t row_space_bytes(int parts) {
-  return (size_t)NSPLIT * 12 + 256 + MAX_PARTS * sizeof(Part) + (size_t)parts * KC * 8;
-}
-__device__ __forceinline__ RowSpace row_space(void* ws, int b, int parts) {
-  char* p = (char*)ws + (size_t)b * row_space_bytes(parts);
-  RowSpace s;
-  s.mass = (u64*)p, p += (size_t)NSPLIT * 8;
-  s.count = (uint32_t*)p, p += (size_t)NSPLIT * 4;
-  s.over = (u64*)p, p += 256;
-  s.part = (Part*)p, p += MAX_PARTS * sizeof(Part);
-  s.cand = (float*)p, p += (size_t)parts * KC * 4;
-  s.cand_index = (int*)p;
-  return s;
-}
 __device__ __forceinline__ bool is_greedy(const Settings& o) { return !(o.temp > 0.0f) || o.top_k == 1; }
 // a list of the top_k can be had from the threads' largest entries, twice as many as are asked for
 __device__ __forceinline__ bool by_list(const Settings& o, int chunks) { return o.top_k > 0 && o.top_k <= min(min((int)blockDim.x, chunks) / 2, KC); }
@@ -695,7 +726,7 @@ template <int TYPE> __global__ __launch_bounds__(1024) void sample_row_kernel(Sa
   u64 over = pass_bins(r, map, sc, o, ranked, mass, count);
   __syncthreads();
   if (o.min_p > 0.0f) over = block_sum(over, sh);
-  draw_from_bins<4>(a, b, r, map, sc, o, ranked, over, nbin, mass, count, list, sh);
+  draw_from_bins<false>(a, b, r, map, sc, o, ranked, over, nbin, mass, count, list, room, sh, RowSpace{}, 0, 0);
 }
 
 // A long row over several workgroups, in three launches: (1) every part's largest entry, and its top_k where a list of them will do;
@@ -706,7 +737,7 @@ template <int TYPE> __global__ __launch_bounds__(512) void sample_part_kernel(Sa
   __shared__ u64 list[1024];
   const int b = blockIdx.y, g = blockIdx.x, tid = threadIdx.x, nt = blockDim.x;
   if (a.n_dev && b >= *a.n_dev) return;
-  const RowSpace ws = row_space(a.ws, b, parts);
+  const RowSpace ws = row_space(a.ws, b, parts, len);
   for (int i = g * nt + tid; i < NSPLIT; i += parts * nt) ws.mass[i] = 0, ws.count[i] = 0;
   if (g == 0 && tid == 0) *ws.over = 0;
   const Settings o = settings_of(a, a.idx ? a.idx[b] : b);
@@ -755,7 +786,7 @@ template <int TYPE> __global__ __launch_bounds__(512) void sample_bins_kernel(Sa
   __shared__ Shared sh;
   const int b = blockIdx.y, g = blockIdx.x, tid = threadIdx.x, nt = blockDim.x;
   if (a.n_dev && b >= *a.n_dev) return;
-  const RowSpace ws = row_space(a.ws, b, parts);
+  const RowSpace ws = row_space(a.ws, b, parts, len);
   const Settings o = settings_of(a, a.idx ? a.idx[b] : b);
   float top, low;
   bool complete;
@@ -767,12 +798,10 @@ template <int TYPE> __global__ __launch_bounds__(512) void sample_bins_kernel(Sa
   u64* const mass = (u64*)dyn;
   uint32_t* const count = (uint32_t*)(mass + NSPLIT);
   const bool ranked = o.top_k > 0 && o.top_k < a.V;
-  for (int i = tid; i < NSPLIT; i += nt) {
-    mass[i] = 0;
-    if (ranked) count[i] = 0;
-  }
+  for (int i = tid; i < NSPLIT; i += nt) mass[i] = 0, count[i] = 0;
   __syncthreads();
-  u64 over = pass_bins(r, bins_of(o, top, low, NSPLIT), scale_of(o, top), o, ranked, mass, count);
+  const BinMap map = bins_of(o, top, low, NSPLIT);
+  u64 over = pass_bins(r, map, scale_of(o, top), o, true, mass, count);
   if (o.min_p > 0.0f) {
     over = block_sum(over, sh);
     if (tid == 0 && over) atomicAdd(ws.over, over);
@@ -782,20 +811,47 @@ template <int TYPE> __global__ __launch_bounds__(512) void sample_bins_kernel(Sa
     if (mass[i]) atomicAdd(&ws.mass[i], mass[i]);
     if (ranked && count[i]) atomicAdd(&ws.count[i], count[i]);
   }
+  // the entries by bins, so that the last kernel need not look for them: where each bin begins, and then every entry in its place
+  constexpr int PER = NSPLIT / 512;
+  uint32_t c[PER], before = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) c[i] = count[tid * PER + i], before += c[i];
+  const uint32_t own = before;
+  before = wave_scan(before, tid & 63);
+  if ((tid & 63) == 63) sh.wave_u32[tid >> 6] = before;
+  __syncthreads();   // and nobody reads the counts any more
+  before -= own;
+  for (int i = 0; i < (tid >> 6); ++i) before += sh.wave_u32[i];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    count[tid * PER + i] = before;
+    ws.offset[(size_t)g * OFFSETS + tid * PER + i] = before;
+    before += c[i];
+  }
+  if (tid == nt - 1) ws.offset[(size_t)g * OFFSETS + NSPLIT] = before;
+  __syncthreads();
+  r.template each<4>([&](f32x4 k, int ch) SM_INLINE {
+#pragma unroll
+    for (int j = 0; j < Row<TYPE>::EPC; ++j) {
+      const float l = r.entry(k, j);
+      if (l > -INFINITY) ws.order[(size_t)g * len + atomicAdd(&count[map.bin(l)], 1u)] = (uint16_t)(ch * Row<TYPE>::EPC + j - r.pad);
+    }
+  });
 }
 
-template <int TYPE> __global__ __launch_bounds__(1024) void sample_join_kernel(SampleArgs a, int parts) {
+constexpr int JOIN_ROOM = MAX_PARTS * KC;   // places in the list: all parts' candidates
+template <int TYPE> __global__ __launch_bounds__(1024) void sample_join_kernel(SampleArgs a, int parts, int len) {
   typedef typename LOf<TYPE>::t T;
   extern __shared__ __align__(16) char dyn[];
   __shared__ Shared sh;
   const int b = blockIdx.x, tid = threadIdx.x, nt = blockDim.x;
   if (a.n_dev && b >= *a.n_dev) return;
-  const RowSpace ws = row_space(a.ws, b, parts);
+  const RowSpace ws = row_space(a.ws, b, parts, len);
   const Settings o = settings_of(a, a.idx ? a.idx[b] : b);
   u64* const mass = (u64*)dyn;
   u64* const list = mass + NSPLIT;
   uint32_t* const count = (uint32_t*)list;
-  const uint32_t room = NSPLIT / 2;
+  const uint32_t room = JOIN_ROOM;
   float top, low;
   bool complete;
   int first;
@@ -811,46 +867,47 @@ template <int TYPE> __global__ __launch_bounds__(1024) void sample_join_kernel(S
   const Row<TYPE> r((const T*)a.logits + (size_t)b * a.ld, a.V);
   const BinMap map = bins_of(o, top, low, NSPLIT);
   const bool ranked = o.top_k > 0 && o.top_k < a.V;
-  u64 over = 0;
   // (half of the part kernel's threads: what it took for a list is one here)
   if (o.top_k > 0 && o.top_k <= KC && complete) {
     const Row<ST_TYPE_F32> c(ws.cand, parts * KC);
     float own, unused;
     pass_top(c, own, unused);
-    const uint32_t n = gather_top<4>(c, o.top_k, top, own, list, room, sh, [&](int i) SM_INLINE { return ws.cand_index[i]; });
-    if (n <= room) {
-      sort_places(list, (int)n, sh);
-      draw_from_sorted(a, b, list, min((int)n, o.top_k), mass, sc, o, sh);
-      return;
+    uint32_t n = gather_top<4>(c, o.top_k, top, own, list, room, sh, [&](int i) SM_INLINE { return ws.cand_index[i]; });
+    if (n > room) {   // too few threads have one: all of them, JOIN_ROOM at most
+      if (tid == 0) sh.n = 0;
+      __syncthreads();
+      for (int i = tid; i < parts * KC; i += nt)
+        if (ws.cand[i] > -INFINITY) list[atomicAdd(&sh.n, 1u)] = place_of(ws.cand[i], ws.cand_index[i]);
+      __syncthreads();
+      n = sh.n;
+      __syncthreads();
     }
-    // too many of equal rank, or in too few threads: the bins after all, by this workgroup alone
-    for (int i = tid; i < NSPLIT; i += nt) mass[i] = 0, count[i] = 0;
-    __syncthreads();
-    over = pass_bins(r, map, sc, o, ranked, mass, count);
-    __syncthreads();
-    if (o.min_p > 0.0f) over = block_sum(over, sh);
-  } else {
-    for (int i = tid; i < NSPLIT; i += nt) {
-      mass[i] = ws.mass[i];
-      if (ranked) count[i] = ws.count[i];
-    }
-    over = *ws.over;
-    __syncthreads();
+    sort_places(list, (int)n, sh);
+    draw_from_sorted(a, b, list, min((int)n, o.top_k), mass, sc, o, sh);
+    return;
   }
-  draw_from_bins<8>(a, b, r, map, sc, o, ranked, over, NSPLIT, mass, count, list, sh);
+  for (int i = tid; i < NSPLIT; i += nt) {
+    mass[i] = ws.mass[i];
+    if (ranked) count[i] = ws.count[i];
+  }
+  const u64 over = *ws.over;
+  __syncthreads();
+  draw_from_bins<true>(a, b, r, map, sc, o, ranked, over, NSPLIT, mass, count, list, room, sh, ws, parts, len);
 }
 
 // Parts of a row: few long rows leave most of the chip idle, and one workgroup takes its time over a long row
-int parts_of(int B, int V) {
-  if (V < 16384) return 1;
-  int g = 512 / B;
+int parts_of(int B, int V, int* len) {
+  int g = V < 16384 ? 1 : 512 / B;
   if (g > V / 4096) g = V / 4096;
   if (g > MAX_PARTS) g = MAX_PARTS;
-  return g < 2 ? 1 : g;
+  if (g < 4) return 1;
+  *len = ((V + g - 1) / g + 63) / 64 * 64;
+  return (V + *len - 1) / *len;   // those that have entries
 }
 
 template <int TYPE> int launch_type(const SampleArgs& a, hipStream_t st) {
-  const int parts = parts_of(a.B, a.V);
+  int len = 0;
+  const int parts = parts_of(a.B, a.V, &len);
   if (parts == 1) {
     const int nbin = a.V <= 1024 ? 2048 : a.V <= 16384 ? 1024 : a.V <= 65536 ? 2048 : 4096;
     const int threads = a.V <= 2048 ? 256 : 512;
@@ -858,12 +915,13 @@ template <int TYPE> int launch_type(const SampleArgs& a, hipStream_t st) {
     ST_LAUNCH_CHECK();
     return ST_OK;
   }
-  const int len = ((a.V + parts - 1) / parts + 63) / 64 * 64, n = (a.V + len - 1) / len;   // n: parts that have entries
-  hipLaunchKernelGGL((sample_part_kernel<TYPE>), dim3(n, a.B), dim3(512), 0, st, a, n, len);
+  constexpr int join_lds = NSPLIT * 8 + JOIN_ROOM * 8;
+  ST_ENSURE_LDS(sample_join_kernel<TYPE>, join_lds);
+  hipLaunchKernelGGL((sample_part_kernel<TYPE>), dim3(parts, a.B), dim3(512), 0, st, a, parts, len);
   ST_LAUNCH_CHECK();
-  hipLaunchKernelGGL((sample_bins_kernel<TYPE>), dim3(n, a.B), dim3(512), (size_t)NSPLIT * 12, st, a, n, len);
+  hipLaunchKernelGGL((sample_bins_kernel<TYPE>), dim3(parts, a.B), dim3(512), (size_t)NSPLIT * 12, st, a, parts, len);
   ST_LAUNCH_CHECK();
-  hipLaunchKernelGGL((sample_join_kernel<TYPE>), dim3(a.B), dim3(1024), (size_t)NSPLIT * 12, st, a, n);
+  hipLaunchKernelGGL((sample_join_kernel<TYPE>), dim3(a.B), dim3(1024), join_lds, st, a, parts, len);
   ST_LAUNCH_CHECK();
   return ST_OK;
 }
@@ -871,8 +929,9 @@ template <int TYPE> int launch_type(const SampleArgs& a, hipStream_t st) {
 }  // namespace
 
 size_t sample_workspace(int B, int V) {
-  const int parts = parts_of(B, V);
-  return parts == 1 ? 0 : (size_t)B * row_space_bytes(parts);
+  int len = 0;
+  const int parts = parts_of(B, V, &len);
+  return parts == 1 ? 0 : (size_t)B * row_space_bytes(parts, len);
 }
 
 int sample_launch(const SampleArgs& a, hipStream_t st) {
