@@ -267,7 +267,7 @@ __device__ __forceinline__ void answer(const SampleArgs& a, int b, int id, doubl
 __device__ __forceinline__ void sort_places(u64* list, int n, Shared& sh) {
   const int tid = threadIdx.x, nt = blockDim.x;
   if (n <= 256) {
-    const int e = tid & 255, parts = nt >> 8, part = tid >> 8;
+    const int width = n <= 64 ? 64 : n <= 128 ? 128 : 256, e = tid & (width - 1), parts = nt / width, part = tid / width;
     const u64 mine = e < n ? list[e] : 0;
     if (tid < 256) sh.digit_count[tid] = 0;
     __syncthreads();
@@ -278,7 +278,7 @@ __device__ __forceinline__ void sort_places(u64* list, int n, Shared& sh) {
       atomicAdd(&sh.digit_count[e], c);
     }
     __syncthreads();
-    if (tid < n) list[sh.digit_count[tid]] = mine;
+    if (tid < width && e < n) list[sh.digit_count[e]] = mine;
     __syncthreads();
     return;
   }
@@ -423,7 +423,7 @@ __device__ __forceinline__ u64 pass_bins(const Row<TYPE>& r, const BinMap& map, 
         if (counted) atomicAdd(&count[bin], 1u);
         if (w >= (double)o.min_p) over += m;
       }
-      __builtin_amdgcn_sched_barrier(0);   // one entry's registers at a time
+      if (j & 1) __builtin_amdgcn_sched_barrier(0);   // two entries' registers at a time
     }
   });
   return over;
@@ -599,9 +599,10 @@ __device__ __forceinline__ void draw_from_bins(const SampleArgs& a, int b, const
         top_bit = 64 - __clzll(any ^ every);   // above the highest bit that differs (two places are never equal)
         prefix = top_bit >= 64 ? 0 : (any >> top_bit) << top_bit;
       }
-      if (tid == 0) sh.n = 0;
-      __syncthreads();
       const bool few = n <= 64;
+      if (tid == 0) sh.n = 0;
+      if (few && tid < 64) sh.digit_count[tid] = 0, sh.digit_mass[128 + tid] = 0;
+      __syncthreads();
       const int low_bit = top_bit > 8 ? top_bit - 8 : 0;
       // few: the digits' array takes the elements themselves, and their masses behind them
       walk([&](u64 place) SM_INLINE {
@@ -619,17 +620,22 @@ __device__ __forceinline__ void draw_from_bins(const SampleArgs& a, int b, const
       });
       __syncthreads();
       if (few) {
-        if (wv == 0) {
-          const u64 mine = lane < (int)n ? sh.digit_mass[lane] : ~0ull, m = lane < (int)n ? sh.digit_mass[64 + lane] : 0;
-          uint32_t c = before_count;
-          u64 mb = before_mass;
-#pragma unroll 4
-          for (int i = 0; i < (int)n; ++i) {
-            const bool earlier = sh.digit_mass[i] < mine;
-            c += earlier;
-            mb += earlier ? sh.digit_mass[64 + i] : 0;
-          }
-          if (lane < (int)n && (by_count ? c == target : mb <= target && target < mb + m)) sh.found_place = mine, sh.found_mass = mb + m;
+        // every element against every other: each wave takes its share of the others
+        const u64 mine = lane < (int)n ? sh.digit_mass[lane] : 0;
+        uint32_t c = 0;
+        u64 mb = 0;
+        for (int i = wv; i < (int)n; i += nw)
+          if (sh.digit_mass[i] < mine) ++c, mb += sh.digit_mass[64 + i];
+        if (c) {
+          atomicAdd(&sh.digit_count[lane], c);
+          atomicAdd(&sh.digit_mass[128 + lane], mb);
+        }
+        __syncthreads();
+        if (wv == 0 && lane < (int)n) {
+          const u64 m = sh.digit_mass[64 + lane];
+          c = before_count + sh.digit_count[lane];
+          mb = before_mass + sh.digit_mass[128 + lane];
+          if (by_count ? c == target : mb <= target && target < mb + m) sh.found_place = mine, sh.found_mass = mb + m;
         }
         __syncthreads();
         break;
