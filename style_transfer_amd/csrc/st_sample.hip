@@ -510,6 +510,7 @@ __device__ __forceinline__ void draw_from_bins(const SampleArgs& a, int b, const
       if (S < ONE_MASS) S = ONE_MASS;   // the largest entry stays whatever is asked
       target = draw_target(o.u, S);
     }
+    if (tid == 0) sh.n = 0, sh.found_bin = 0, sh.found_count = 0, sh.found_mass = 0, sh.found_place = 0;
     __syncthreads();
     {
       u64 m0 = base_mass;
@@ -523,7 +524,6 @@ __device__ __forceinline__ void draw_from_bins(const SampleArgs& a, int b, const
         c0 = c1;
       }
     }
-    if (tid == 0) sh.n = 0;
     __syncthreads();
     const int bin = (int)sh.found_bin;
     u64 before_mass = sh.found_mass;
@@ -539,7 +539,7 @@ __device__ __forceinline__ void draw_from_bins(const SampleArgs& a, int b, const
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) g += sh.part_end[g + d - 1] <= t ? d : 0;
       const int i = g * len + ws.order[(size_t)g * len + (uint32_t)(sh.part_at[g] + t)];   // (the sum, modulo 2^32, is the place in the part)
-      return place_of(logit<TYPE>(r.p[i]), i);
+      return place_of(logit<TYPE>(r.p[min(i, r.n - 1)]), i);
     };
     if constexpr (SPLIT) {
       if (wv == 0) {
@@ -661,6 +661,7 @@ __device__ __forceinline__ void draw_from_bins(const SampleArgs& a, int b, const
       before_mass = sh.found_mass;
     }
     if (question < 2) S = sh.found_mass;
+    __syncthreads();
   }
   if (tid == 0) answer(a, b, (int)(uint32_t)sh.found_place, weight(sc, of_key((uint32_t)(sh.found_place >> 32))), S);
 }
@@ -840,7 +841,10 @@ template <int TYPE> __global__ __launch_bounds__(512) void sample_bins_kernel(Sa
 #pragma unroll
     for (int j = 0; j < Row<TYPE>::EPC; ++j) {
       const float l = r.entry(k, j);
-      if (l > -INFINITY) ws.order[(size_t)g * len + atomicAdd(&count[map.bin(l)], 1u)] = (uint16_t)(ch * Row<TYPE>::EPC + j - r.pad);
+      if (l > -INFINITY) {
+        const uint32_t at = atomicAdd(&count[map.bin(l)], 1u);
+        if (at < (uint32_t)len) ws.order[(size_t)g * len + at] = (uint16_t)(ch * Row<TYPE>::EPC + j - r.pad);
+      }
     }
   });
 }
