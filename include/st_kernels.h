@@ -488,6 +488,16 @@ size_t st_sample_workspace_bytes(int B, int V);
 int st_sample_logits(const void* logits, int type, int64_t ld, int B, int V, const float* u, const StSampleSettings* settings,
                      int32_t* ids, float* logp, void* workspace, size_t workspace_bytes, void* stream);
 
+/* st_decode_greedy with a draw in the argmax's place: the decoder's own steps, then the logits of the live rows (generator of the
+ * weights struct, or `head`, a packed 4-bit [vocab, 256] weight, with the struct's bias) and st_sample_logits on each with
+ * u [B, max_len - 1]; settings arrays go by sentence.  out_logp [B, max_len - 1] (may be NULL): log-probability of each drawn token
+ * (0 after an early exit).  A row whose logits are all NaN or -inf writes PAD and stops.  Other arguments, synchronisation and
+ * errors as st_decode_greedy.                                                                                              */
+size_t st_decode_sample_workspace_bytes(const StDecoderWeights* w, int B, int max_len, int options);
+int st_decode_sample(const StDecoderWeights* w, const StQ4Weight* head, const float* latent, int B, int max_len, int bos, int eos,
+                     int pad, int options, int sync_every, const float* u, const StSampleSettings* settings, int32_t* out_ids,
+                     float* out_logp, void* workspace, size_t workspace_bytes, int* n_steps_host, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

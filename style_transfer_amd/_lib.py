@@ -136,6 +136,9 @@ EXPORTS = {
     "st_gemm_q4": (C.c_int, [fp, C.c_int, C.c_int64, C.c_int, C.POINTER(StQ4Weight), fp, fp, C.c_int64, fp]),
     "st_sample_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
     "st_sample_logits": (C.c_int, [fp, C.c_int, C.c_int64, C.c_int, C.c_int, fp, C.POINTER(StSampleSettings), fp, fp, fp, C.c_size_t, fp]),
+    "st_decode_sample_workspace_bytes": (C.c_size_t, [C.POINTER(StDecoderWeights), C.c_int, C.c_int, C.c_int]),
+    "st_decode_sample": (C.c_int, [C.POINTER(StDecoderWeights), C.POINTER(StQ4Weight), fp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
+                                   C.c_int, C.c_int, fp, C.POINTER(StSampleSettings), fp, fp, fp, C.c_size_t, C.POINTER(C.c_int), fp]),
     "st_encode_latent": (C.c_int, [C.POINTER(StEncoderWeights), fp, fp, fp, C.c_int, C.c_int, C.c_int, fp, fp, C.c_size_t, fp]),
 }
 

@@ -20,7 +20,7 @@ int sl_small_views(const float* ori, const float* like0, int n_views, int B, flo
 
 // internal: a draw from rows of logits (csrc/st_sample.hip; used by csrc/st_decode.hip).  Row r of the logits belongs to sentence
 // s = idx ? idx[r] : r, whose uniform number is u[s * u_stride] and whose settings are the s-th of the *_rows; ids and logp are
-// written at r; rows from *n_dev on (n_dev given) are left alone.
+// written at r; rows with row0 + r >= *n_dev (n_dev given) are left alone.
 struct SampleArgs {
   const void* logits;
   int type;
@@ -31,12 +31,14 @@ struct SampleArgs {
   StSampleSettings set;
   const int* idx;
   const int* n_dev;
+  int row0;
   int32_t* ids;
   float* logp;
   void* ws;
 };
 int sample_check(const StSampleSettings* s);
 size_t sample_workspace(int B, int V);
+size_t sample_workspace_most(int B, int V);
 int sample_launch(const SampleArgs& a, hipStream_t st);
 
 #define ST_CHECK_ARG(cond, ...)   \

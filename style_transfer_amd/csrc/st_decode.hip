@@ -662,6 +662,35 @@ __global__ __launch_bounds__(FIN_THREADS) void finish_kernel(const float4* __res
   if (live) idx_next[slot] = s;
 }
 
+// ---- sampled decode: the final LayerNorm of the live rows (the 4-bit head multiplies plain rows), and the step's end ---------
+__global__ __launch_bounds__(256) void ln_rows_kernel(const float* __restrict__ x, const float* __restrict__ ln_a, const float* __restrict__ ln_b,
+                                                      int n, float* __restrict__ y) {
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (r >= n) return;
+  const f32x4 v = *(const f32x4*)(x + (size_t)r * 256 + lane * 4);
+  *(f32x4*)(y + (size_t)r * 256 + lane * 4) = layernorm256(v, *(const f32x4*)(ln_a + lane * 4), *(const f32x4*)(ln_b + lane * 4));
+}
+// writes the drawn tokens of the live rows; a row goes on unless it drew EOS / PAD (early exit), had nothing to draw from (id -1: PAD is
+// written) or this was the last step
+__global__ __launch_bounds__(FIN_THREADS) void sample_finish_kernel(const int32_t* __restrict__ tok, const float* __restrict__ lp,
+                                                            const int* __restrict__ idx, const int* __restrict__ n_dev, int32_t* __restrict__ ys,
+                                                            float* __restrict__ logp, int T, int pos, int eos, int pad, int early, int last,
+                                                            int* __restrict__ idx_next, int* __restrict__ n_next) {
+  __shared__ int app[FIN_THREADS / 64 + 1];
+  const int r = blockIdx.x * FIN_THREADS + threadIdx.x;
+  bool live = false;
+  int s = 0;
+  if (r < *n_dev) {
+    const int id = tok[r];
+    s = idx[r];
+    ys[(size_t)s * T + pos] = id < 0 ? pad : id;
+    if (logp) logp[(size_t)s * T + pos] = lp[r];
+    live = id >= 0 && !(last || (early && (id == eos || id == pad)));
+  }
+  const int slot = block_append(n_next, live, app);
+  if (live) idx_next[slot] = s;
+}
+
 __global__ void iota_kernel(int* idx, int* n_dev, int n) {
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
   if (i < n) idx[i] = i;
@@ -704,7 +733,23 @@ struct DecodeWs {
   int* cnt;        // [0],[1]: live counts (ping-pong), [2]: ambiguous rows of the current step
   float* slab;     // [d_ff/256][64][256] split-K partials of feed_forward.w_2 when one panel of rows is left
   float* colpad;   // [2][32 ceil(vocab / 32)] padded generator bias and column norms (screening pass)
+  float* logits;   // sampled decode: [sample_rows(B)][vocab]
+  int32_t* tok;    // [B] drawn tokens
+  float* lp;       // [B] their log-probabilities
+  void* smp;       // the draw's own workspace
   size_t total;
+};
+// rows of logits that are held at a time: 256 MB of them, 64 rows at least
+static int sample_rows(const StDecoderWeights* w, int B) {
+  const long r = ((256L << 20) / ((long)w->vocab * 4) + 63) / 64 * 64;
+  return r < B ? (int)(r < 64 ? 64 : r) : B;
+}
+// what a sampled decode has beside a greedy one's arguments
+struct DecodeSampling {
+  const StQ4Weight* head;         // NULL: the generator of the weights struct
+  const float* u;                 // [B][T]
+  const StSampleSettings* set;
+  float* logp;                    // [B][T] or NULL
 };
 #define ST_GEN_SPLITS 16        /* max column splits of the generator (partials per row) */
 #define ST_SCREEN_MIN_ROWS 2048 /* below this the two extra launches of the screened argmax cost more than they save */
@@ -712,7 +757,7 @@ struct DecodeWs {
 #define ST_GEN_SPLITS_SMALL 96  /* ... when few rows are live: the late steps are latency-bound on streaming W */
 
 // kv_layers: decoder layers that keep a K / V cache (all of them, or all but the first when it reads the (token, position) table)
-static DecodeWs carve(const StDecoderWeights* w, int B, int max_len, char* base, int kv_layers) {
+static DecodeWs carve(const StDecoderWeights* w, int B, int max_len, char* base, int kv_layers, bool sampled = false) {
   DecodeWs ws;
   const int T = max_len - 1, L = w->n_layers;
   size_t off = 0;
@@ -734,6 +779,13 @@ static DecodeWs carve(const StDecoderWeights* w, int B, int max_len, char* base,
   ws.cnt = (int*)take(256);
   ws.slab = (float*)take((size_t)(w->d_ff / 256) * 64 * 256 * 4);
   ws.colpad = (float*)take(rp_screen_colpad_floats(w->vocab) * 4);
+  if (sampled) {
+    const int rows = sample_rows(w, B);
+    ws.logits = (float*)take((size_t)rows * w->vocab * 4);
+    ws.tok = (int32_t*)take((size_t)B * 4);
+    ws.lp = (float*)take((size_t)B * 4);
+    ws.smp = take(sample_workspace_most(rows, w->vocab));
+  }
   ws.total = off;
   return ws;
 }
@@ -769,9 +821,37 @@ extern "C" size_t st_decode_workspace_bytes(const StDecoderWeights* w, int B, in
   return st_decode_workspace_bytes_opt(w, B, max_len, ST_DEC_NO_L0_TABLE);   // enough for every option
 }
 
-extern "C" int st_decode_greedy(const StDecoderWeights* w, const float* latent, int B, int max_len, int bos, int eos,
-                                int pad, int options, int sync_every, int32_t* out_ids, float* top2gap,
-                                void* workspace, size_t workspace_bytes, int* n_steps_host, void* stream) {
+// the drawn tokens of one step: logits of the live rows, sample_rows at a time, and a draw from each (dead rows behind the live
+// count are multiplied too, where the host's count is stale; nothing is drawn from them)
+static int sample_step(const StDecoderWeights* w, const DecodeSampling& sm, const DecodeWs& ws, const int* idx, const int* n_dev, int n_bound,
+                       int chunk, int T, int pos, hipStream_t st) {
+  if (sm.head) {
+    hipLaunchKernelGGL(ln_rows_kernel, dim3((n_bound + 3) / 4), dim3(256), 0, st, ws.x, w->lnf_a, w->lnf_b, n_bound, ws.att);
+    ST_LAUNCH_CHECK();
+  }
+  for (int r0 = 0; r0 < n_bound; r0 += chunk) {
+    const int n = n_bound - r0 < chunk ? n_bound - r0 : chunk;
+    if (sm.head) {
+      ST_TRY(st_gemm_q4(ws.att + (size_t)r0 * 256, ST_TYPE_F32, 256, n, sm.head, w->gen_b, ws.logits, w->vocab, st));
+    } else {
+      GemmArgs g = {};
+      g.fmt = w->gemm_format; g.range_flag = ws.cnt + 3;
+      g.X = ws.x + (size_t)r0 * 256; g.n_host = n; g.ln_a = w->lnf_a; g.ln_b = w->lnf_b;
+      g.W = w->gen_w; g.bias = w->gen_b; g.N = w->vocab; g.out = ws.logits; g.ldo = w->vocab;
+      ST_TRY(launch_rp<EPI_BIAS>(g, n, rp_splits(n, w->vocab, ST_GEN_SPLITS_SMALL), st));
+    }
+    SampleArgs a = {};
+    a.logits = ws.logits; a.type = ST_TYPE_F32; a.ld = w->vocab; a.B = n; a.V = w->vocab;
+    a.u = sm.u + pos; a.u_stride = T; a.set = *sm.set; a.idx = idx + r0; a.n_dev = n_dev; a.row0 = r0;
+    a.ids = ws.tok + r0; a.logp = sm.logp ? ws.lp + r0 : nullptr; a.ws = ws.smp;
+    ST_TRY(sample_launch(a, st));
+  }
+  return ST_OK;
+}
+
+static int decode_loop(const StDecoderWeights* w, const float* latent, int B, int max_len, int bos, int eos, int pad, int options,
+                       int sync_every, int32_t* out_ids, float* top2gap, const DecodeSampling* sm, void* workspace,
+                       size_t workspace_bytes, int* n_steps_host, void* stream) {
   ST_TRY(check_weights(w, max_len));
   ST_CHECK_ARG(B >= 0, "B=%d", B);
   rp_ab_env();
@@ -783,7 +863,7 @@ extern "C" int st_decode_greedy(const StDecoderWeights* w, const float* latent, 
   const int T = max_len - 1, L = w->n_layers;
   const bool use_tab = dec_uses_l0_table(w, max_len, options);
   const int kv_first = use_tab ? 1 : 0, kv_layers = L - kv_first;   // the first layer keeps no K / V cache when it reads the table
-  DecodeWs ws = carve(w, B, max_len, (char*)workspace, kv_layers);
+  DecodeWs ws = carve(w, B, max_len, (char*)workspace, kv_layers, sm != nullptr);
   if (ws.total > workspace_bytes) {
     st_set_error("workspace too small: need %zu bytes, have %zu", ws.total, workspace_bytes);
     return ST_ENOMEM;
@@ -802,6 +882,7 @@ extern "C" int st_decode_greedy(const StDecoderWeights* w, const float* latent, 
 
   ST_HIP(hipMemsetAsync(out_ids, 0, (size_t)B * T * 4, st));  // PAD after an early exit
   if (top2gap) ST_HIP(hipMemsetAsync(top2gap, 0, (size_t)B * T * 4, st));
+  if (sm && sm->logp) ST_HIP(hipMemsetAsync(sm->logp, 0, (size_t)B * T * 4, st));
   ST_HIP(hipMemsetAsync(ws.cnt, 0, 256, st));  // counters and the f16-range flag (cnt[3])
   hipLaunchKernelGGL(iota_kernel, dim3((B + 255) / 256), dim3(256), 0, st, ws.idx[0], ws.cnt + 0, B);
   ST_LAUNCH_CHECK();
@@ -933,6 +1014,13 @@ extern "C" int st_decode_greedy(const StDecoderWeights* w, const float* latent, 
         ST_TRY(launch_rp_kchunk<EPI_RESID>(f2, n_bound, st));
       }
     }
+    const int last = pos == T - 1 ? 1 : 0;
+    if (sm) {
+      ST_TRY(sample_step(w, *sm, ws, idx, n_dev, n_bound, sample_rows(w, B), T, pos, st));
+      hipLaunchKernelGGL(sample_finish_kernel, dim3((n_bound + FIN_THREADS - 1) / FIN_THREADS), dim3(FIN_THREADS), 0, st, ws.tok, ws.lp, idx,
+                         n_dev, out_ids, sm->logp, T, pos, eos, pad, early, last, ws.idx[cur ^ 1], ws.cnt + (cur ^ 1));
+      ST_LAUNCH_CHECK();
+    } else {
     GemmArgs gg = {};
     gg.fmt = w->gemm_format; gg.range_flag = ws.cnt + 3;
     gg.X = ws.x; gg.n_dev = n_dev; gg.n_host = n_bound; gg.ln_a = w->lnf_a; gg.ln_b = w->lnf_b;
@@ -941,7 +1029,6 @@ extern "C" int st_decode_greedy(const StDecoderWeights* w, const float* latent, 
     // partial buffer: B * ST_GEN_SPLITS + 64 * ST_GEN_SPLITS_SMALL entries
     const long room = ((long)B * ST_GEN_SPLITS + 64L * ST_GEN_SPLITS_SMALL) / n_bound;
     const int gsplits = rp_splits(n_bound, w->vocab, (int)(room < ST_GEN_SPLITS_SMALL ? (room < ST_GEN_SPLITS ? ST_GEN_SPLITS : room) : ST_GEN_SPLITS_SMALL));
-    const int last = pos == T - 1 ? 1 : 0;
     // (a vocabulary beyond 32768 would not fit the block number into the screening kernel's 8 key bits: no screening)
     const bool screen = screen_ok && n_bound >= ST_SCREEN_MIN_ROWS && (w->vocab + 127) / 128 <= RS_MAX_BLOCKS;
     ProfPair pp;
@@ -975,6 +1062,7 @@ extern "C" int st_decode_greedy(const StDecoderWeights* w, const float* latent, 
       ST_LAUNCH_CHECK();
     }
     if (g_prof_on == ST_PROF_GENERATOR) ST_TRY(prof_end(&pp, st));
+    }
     cur ^= 1;
     ++steps;
     // The host reads the live count to size the next grids.  With few rows left (the straggler tail: a handful of
@@ -1005,6 +1093,32 @@ extern "C" int st_decode_greedy(const StDecoderWeights* w, const float* latent, 
     }
   }
   return ST_OK;
+}
+
+extern "C" int st_decode_greedy(const StDecoderWeights* w, const float* latent, int B, int max_len, int bos, int eos,
+                                int pad, int options, int sync_every, int32_t* out_ids, float* top2gap,
+                                void* workspace, size_t workspace_bytes, int* n_steps_host, void* stream) {
+  return decode_loop(w, latent, B, max_len, bos, eos, pad, options, sync_every, out_ids, top2gap, nullptr, workspace, workspace_bytes,
+                     n_steps_host, stream);
+}
+
+extern "C" size_t st_decode_sample_workspace_bytes(const StDecoderWeights* w, int B, int max_len, int options) {
+  if (!w || B <= 0 || max_len < 2 || w->vocab < 1 || w->vocab > ST_SAMPLE_MAX_VOCAB) return 0;
+  return carve(w, B, max_len, nullptr, w->n_layers - (dec_uses_l0_table(w, max_len, options) ? 1 : 0), true).total;
+}
+
+extern "C" int st_decode_sample(const StDecoderWeights* w, const StQ4Weight* head, const float* latent, int B, int max_len, int bos, int eos,
+                                int pad, int options, int sync_every, const float* u, const StSampleSettings* settings, int32_t* out_ids,
+                                float* out_logp, void* workspace, size_t workspace_bytes, int* n_steps_host, void* stream) {
+  ST_TRY(check_weights(w, max_len));
+  ST_TRY(sample_check(settings));
+  ST_CHECK_ARG(w->vocab <= ST_SAMPLE_MAX_VOCAB, "vocab=%d: at most %d are drawn from", w->vocab, ST_SAMPLE_MAX_VOCAB);
+  ST_CHECK_ARG(!head || (head->image && head->N == w->vocab && head->K == ST_D), "head: N=%d K=%d, expected a packed [%d, %d]",
+               head->N, head->K, w->vocab, ST_D);
+  ST_CHECK_ARG(B <= 0 || u, "NULL buffer");
+  const DecodeSampling sm = {head, u, settings, out_logp};
+  return decode_loop(w, latent, B, max_len, bos, eos, pad, options, sync_every, out_ids, nullptr, &sm, workspace, workspace_bytes,
+                     n_steps_host, stream);
 }
 
 extern "C" int st_gemm_argmax(const float* h, const float* ln_a, const float* ln_b, const float* W, const float* b,

@@ -677,7 +677,7 @@ template <int TYPE> __global__ __launch_bounds__(1024) void sample_row_kernel(Sa
   extern __shared__ __align__(16) char dyn[];
   __shared__ Shared sh;
   const int b = blockIdx.x, tid = threadIdx.x, nt = blockDim.x;
-  if (a.n_dev && b >= *a.n_dev) return;
+  if (a.n_dev && a.row0 + b >= *a.n_dev) return;
   u64* const mass = (u64*)dyn;
   u64* const list = mass + nbin;
   uint32_t* const count = (uint32_t*)list;
@@ -743,7 +743,7 @@ template <int TYPE> __global__ __launch_bounds__(512) void sample_part_kernel(Sa
   __shared__ Shared sh;
   __shared__ u64 list[1024];
   const int b = blockIdx.y, g = blockIdx.x, tid = threadIdx.x, nt = blockDim.x;
-  if (a.n_dev && b >= *a.n_dev) return;
+  if (a.n_dev && a.row0 + b >= *a.n_dev) return;
   const RowSpace ws = row_space(a.ws, b, parts, len);
   for (int i = g * nt + tid; i < NSPLIT; i += parts * nt) ws.mass[i] = 0, ws.count[i] = 0;
   if (g == 0 && tid == 0) *ws.over = 0;
@@ -792,7 +792,7 @@ template <int TYPE> __global__ __launch_bounds__(512) void sample_bins_kernel(Sa
   extern __shared__ __align__(16) char dyn[];
   __shared__ Shared sh;
   const int b = blockIdx.y, g = blockIdx.x, tid = threadIdx.x, nt = blockDim.x;
-  if (a.n_dev && b >= *a.n_dev) return;
+  if (a.n_dev && a.row0 + b >= *a.n_dev) return;
   const RowSpace ws = row_space(a.ws, b, parts, len);
   const Settings o = settings_of(a, a.idx ? a.idx[b] : b);
   float top, low;
@@ -855,7 +855,7 @@ template <int TYPE> __global__ __launch_bounds__(1024) void sample_join_kernel(S
   extern __shared__ __align__(16) char dyn[];
   __shared__ Shared sh;
   const int b = blockIdx.x, tid = threadIdx.x, nt = blockDim.x;
-  if (a.n_dev && b >= *a.n_dev) return;
+  if (a.n_dev && a.row0 + b >= *a.n_dev) return;
   const RowSpace ws = row_space(a.ws, b, parts, len);
   const Settings o = settings_of(a, a.idx ? a.idx[b] : b);
   u64* const mass = (u64*)dyn;
@@ -938,6 +938,12 @@ template <int TYPE> int launch_type(const SampleArgs& a, hipStream_t st) {
 
 }  // namespace
 
+// the most that a call with up to B rows needs (fewer rows are cut into more parts)
+size_t sample_workspace_most(int B, int V) {
+  size_t most = 0;
+  for (int n = B < 128 ? B : 128; n > 0; --n) most = sample_workspace(n, V) > most ? sample_workspace(n, V) : most;   // 128: parts_of's 4 parts
+  return most;
+}
 size_t sample_workspace(int B, int V) {
   int len = 0;
   const int parts = parts_of(B, V, &len);

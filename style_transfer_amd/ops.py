@@ -7,6 +7,8 @@ Names mirror the reference functions they replace:
   scorer_edit_step      <- get_contrastive_loss + backward + Adam.step (:796-810)
   gemm_argmax           <- Generator + torch.max                 (model.py:200-207, :290-292)
   accept_changes        <- id2text_sentence compare + Change bookkeeping (:816-839)
+Without a counterpart there: sample_logits / sample_decode (a draw in the argmax's place), quantize_weight_q4 / pack_weight_q4 /
+gemm_q4 (products with 4-bit weights).
 """
 import ctypes as C
 import math
@@ -369,6 +371,16 @@ def _sample_settings(B, dev, temperature, top_k, top_p, min_p):
     return s
 
 
+def _workspace(ws, nbytes, device):
+    """a DecodeWorkspace's buffer, or one for this call alone"""
+    if ws is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    buf = ws.get(nbytes)
+    if buf.device != device:
+        raise ValueError("ws is on %s, not on %s" % (buf.device, device))
+    return buf
+
+
 def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, want_logp=True, ws: DecodeWorkspace = None):
     """One token per row of logits [B, V] (f32, bf16 or f16; rows may be strided) from the uniform numbers u [B] (f32, in
     [0, 1)) -> (ids int32 [B], logp f32 [B] or None).  Filters in the order temperature, top_k (0: off), top_p (1: off),
@@ -383,6 +395,33 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, wan
     ids = torch.empty(B, dtype=torch.int32, device=dev)
     logp = torch.empty(B, dtype=torch.float32, device=dev) if want_logp else None
     nbytes = lib().st_sample_workspace_bytes(B, V)
-    buf = None if nbytes == 0 else ws.get(nbytes) if ws is not None else torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    buf = None if nbytes == 0 else _workspace(ws, nbytes, dev)
     _call(dev, "st_sample_logits", logits.data_ptr(), kind, ld, B, V, u.data_ptr(), C.byref(s), ids.data_ptr(), _p(logp), _p(buf), nbytes)
     return ids, logp
+
+
+def sample_decode(ae, latent, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, head=None, max_len=60, start_id=2, eos=3, pad=0,
+                  early_exit=True, sync_every=1, want_logp=True, ws: DecodeWorkspace = None, l0_table=True):
+    """greedy_decode with a draw in the argmax's place (st_decode_sample): latent [B, 256], uniform numbers u [B, max_len - 1]
+    (f32, in [0, 1)) -> (ids int32 [B, max_len - 1], logp f32 of the same shape or None, steps run).  Settings as sample_logits,
+    numbers or tensors [B].  head: the generator as a Q4Weight (ae.quantized_generator()), None: as the weights were packed.
+    temperature 0 gives greedy_decode's tokens."""
+    if not (torch.is_tensor(latent) and latent.dim() == 2 and latent.shape[1] == 256):
+        raise ValueError("latent: expected [B, 256]")
+    B, T, dev = latent.shape[0], max_len - 1, latent.device
+    _on(latent, "latent", torch.float32, (B, 256))
+    _on(u, "u", torch.float32, (B, T), dev)
+    if head is not None and (not isinstance(head, Q4Weight) or (head.N, head.K) != (ae.vocab, 256) or head.image.device != dev):
+        raise ValueError("head: expected a Q4Weight [%d, 256] on %s" % (ae.vocab, dev))
+    s = _sample_settings(B, dev, temperature, top_k, top_p, min_p)
+    ids = torch.empty(B, T, dtype=torch.int32, device=dev)
+    logp = torch.empty(B, T, dtype=torch.float32, device=dev) if want_logp else None
+    if B == 0:
+        return ids, logp, 0
+    options = (_lib.ST_DEC_EARLY_EXIT if early_exit else 0) | (0 if l0_table else _lib.ST_DEC_NO_L0_TABLE)
+    need = lib().st_decode_sample_workspace_bytes(C.byref(ae.dec), B, max_len, options)
+    buf = _workspace(ws, need, dev)
+    steps = C.c_int(0)
+    _call(dev, "st_decode_sample", C.byref(ae.dec), None if head is None else head.ref, latent.data_ptr(), B, max_len, start_id, eos, pad,
+          options, sync_every, u.data_ptr(), C.byref(s), ids.data_ptr(), _p(logp), buf.data_ptr(), buf.numel(), C.byref(steps))
+    return ids, logp, steps.value

@@ -98,6 +98,7 @@ class AEWeights(_Packed):
         self.dec.emb, self.dec.pe = self.emb_ptr, self.pe_ptr
         self.dec.lnf_a, self.dec.lnf_b = self.dev(sd["decoder.norm.a_2"]), self.dev(sd["decoder.norm.b_2"])
         self.dec.gen_w, self.dec.gen_b = self.packed(sd["generator.proj.weight"]), self.dev(sd["generator.proj.bias"])
+        self._generator = sd["generator.proj.weight"]
         for l in range(self.n_layers):
             p = "decoder.layers.%d." % l
             y = self.dec.layer[l]
@@ -160,6 +161,13 @@ class AEWeights(_Packed):
                 del scratch
                 self._keep.append(tab)
                 s.l0_table, s.l0_table_len = tab.data_ptr(), T
+
+
+    def quantized_generator(self, group=64, zero_points=False):
+        """the generator matrix [vocab, 256] in 4 bits with a scale per `group` columns (ops.Q4Weight): ops.sample_decode's head"""
+        from . import ops
+        W = self._generator.detach().to(device=self.device, dtype=torch.float32).contiguous()
+        return ops.pack_weight_q4(*ops.quantize_weight_q4(W, group, zero_points), group=group)
 
 
 def fold_bn(w, b, bn_w, bn_b, mean, var, eps=1e-5):

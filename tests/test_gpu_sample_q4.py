@@ -434,3 +434,130 @@ def test_head_and_draw(dev, rows):
     check_sample(logits, u, ids, logp, **s)
     ids0, _ = ops.sample_logits(logits, u, temperature=0.0)
     assert torch.equal(ids0.long(), logits.argmax(1))
+
+
+# ---- the decoder's loop with draws --------------------------------------------------------------------------------------
+
+@pytest.fixture(scope="module", params=["f16x3", "f32"])
+def ae(request, ae_sd_torch, dev):
+    from style_transfer_amd.weights import AEWeights
+    return AEWeights(ae_sd_torch, dev, gemm_format=request.param)
+
+
+@pytest.fixture(scope="module")
+def latents(dev):
+    from conftest import gold
+    z = gold("attack_notnll.npz")["latent"].reshape(-1, 256).astype(np.float32)
+    return torch.from_numpy(np.ascontiguousarray(z[:: max(1, len(z) // 60)][:60])).to(dev)
+
+
+def lengths_of(ids):
+    """tokens of each row up to its first EOS / PAD, that one included"""
+    return [next((i + 1 for i, x in enumerate(r) if x in (0, 3)), len(r)) for r in ids]
+
+
+def test_sample_decode_greedy(dev, ae, latents):
+    """temperature 0 (for all, and for every other sentence between sampled ones): greedy_decode's tokens, log-probability 0.
+    (Where the two best logits are closer than the products' rounding, 1e-3, the two may part.)"""
+    from style_transfer_amd import ops
+    B = latents.shape[0]
+    g = torch.Generator(device=dev).manual_seed(1)
+    u = torch.rand(B, 59, generator=g, device=dev)
+    ids, gap, _ = ops.greedy_decode(ae, latents, want_gap=True)
+    ids, gap = ids.cpu().numpy(), gap.cpu().numpy()
+    alone, logp, steps = ops.sample_decode(ae, latents, u, temperature=0.0)
+    assert bool((logp == 0).all()) and steps > 0
+    t = torch.where(torch.arange(B, device=dev) % 2 == 0, 0.0, 1.0)
+    mixed, _, _ = ops.sample_decode(ae, latents, u, temperature=t)
+    same = 0
+    for s, n in enumerate(lengths_of(ids)):
+        if gap[s, :n].min() <= 1e-3:
+            continue
+        same += 1
+        assert np.array_equal(alone[s, :n].cpu().numpy(), ids[s, :n]), s
+        assert bool((alone[s, n:] == 0).all())
+        if s % 2 == 0:
+            assert np.array_equal(mixed[s, :n].cpu().numpy(), ids[s, :n]), s
+    assert same > B // 2
+
+
+@pytest.mark.parametrize("head_bits", [0, 4])
+def test_sample_decode_draws(dev, ae, ae_sd, latents, head_bits):
+    """every drawn token against the CPU oracle's logits for the tokens before it (with the 4-bit head: of the weights that the codes
+    stand for): its log-probability within 1e-2, and u between the masses before and behind it within 1e-2 (logits are good to 2e-4
+    of the largest, about 30, which moves a share by 2 x 6e-3 of itself at most)"""
+    import st_oracle as O
+    from style_transfer_amd import ops
+    sd, head = dict(ae_sd), None
+    if head_bits:
+        W = torch.from_numpy(np.ascontiguousarray(ae_sd["generator.proj.weight"])).to(dev)
+        codes, scales, z = ops.quantize_weight_q4(W, 64, True)
+        sd["generator.proj.weight"] = weight_of(codes, scales, z, 256, 64).astype(np.float32)
+        head = ae.quantized_generator(64, True)
+    z = latents[:20]
+    g = torch.Generator(device=dev).manual_seed(7 + head_bits)
+    u = torch.rand(20, 59, generator=g, device=dev)
+    pe = O.positional_encoding(60)
+    for s in (dict(temperature=1.0), dict(temperature=1.3, top_k=8), dict(temperature=0.9, top_p=0.8, min_p=0.01)):
+        ids, logp, _ = ops.sample_decode(ae, z, u, head=head, **s)
+        again, logp2, _ = ops.sample_decode(ae, z, u, head=head, **s)
+        assert torch.equal(ids, again) and torch.equal(logp, logp2)
+        few, _, _ = ops.sample_decode(ae, z[3:5].contiguous(), u[3:5].contiguous(), head=head, **s)
+        assert torch.equal(few, ids[3:5])                       # a sentence's draws are its own, whoever is decoded with it
+        ids, logp, un = ids.cpu().numpy(), logp.cpu().numpy(), u.cpu().numpy()
+        ys = np.concatenate([np.full((20, 1), 2), ids[:, :-1]], 1).astype(np.int64)
+        logits = O.linear(O.decode_full(sd, z.cpu().numpy(), ys, pe), sd, "generator.proj").astype(np.float64)
+        for b, n in enumerate(lengths_of(ids)):
+            assert (ids[b, n:] == 0).all() and (logp[b, n:] == 0).all()
+            for t in range(n):
+                row, k = logits[b, t], ids[b, t]
+                order = np.argsort(-row, kind="stable")
+                if s.get("top_k"):
+                    order = order[:s["top_k"]]
+                w = np.exp((row[order] - row[order[0]]) / s["temperature"])
+                c = np.cumsum(w)
+                keep = int(np.searchsorted(np.concatenate(([0.0], c))[:-1], s.get("top_p", 1.0) * c[-1] * (1 + 1e-12))) if "top_p" in s else len(w)
+                keep = max(1, min(keep, int((w >= s.get("min_p", 0.0)).sum())))
+                at = int(np.nonzero(order == k)[0][0]) if k in order[:min(len(order), keep + 2)] else -1
+                assert at >= 0, "sentence %d token %d: %d is not among the kept ones" % (b, t, k)
+                # an entry at the border may be kept by one side alone: shares go by the set that has the token
+                S = c[max(keep - 1, at)]
+                assert abs(logp[b, t] - math.log(w[at] / S)) < 1e-2 + 2 * w[keep - 1] / S, (b, t)
+                slack = 1e-2 + 2 * w[keep - 1] / S * (keep < len(w))
+                assert (c[at] - w[at]) / S - slack <= un[b, t] <= c[at] / S + slack, (b, t, un[b, t], c[at] / S)
+
+
+def test_sample_decode_large_vocabulary_and_batches(dev, ae_sd_torch):
+    """more live rows than logits are held at a time, steps that end rows, and the parts of long rows: a sentence draws the same tokens
+    in any batch"""
+    from conftest import GOLD
+    import os
+    from style_transfer_amd import ops, weights as W
+    sd = W.expand_ae_state_dict(W.load_state_dict_file(os.path.join(GOLD, "surrogate_ae_amazon.safetensors")))
+    ae = W.AEWeights(sd, dev, l0_table=False)
+    g = torch.Generator(device=dev).manual_seed(3)
+    from conftest import gold
+    z = torch.from_numpy(gold("attack_amazon.npz")["latent"].reshape(-1, 256).astype(np.float32)).to(dev)
+    z = z[torch.randint(0, z.shape[0], (3700,), generator=g, device=dev)].contiguous()
+    u = torch.rand(3700, 59, generator=g, device=dev)
+    s = dict(temperature=0.8, top_p=0.9)
+    head = ae.quantized_generator()
+    ids, logp, _ = ops.sample_decode(ae, z, u, head=head, **s)
+    assert bool(torch.isfinite(logp).all()) and bool((logp <= 0).all()) and int(ids.min()) >= 0 and int(ids.max()) < ae.vocab
+    pick = torch.tensor([0, 1, 1700, 3390, 3699], device=dev)
+    few, lf, _ = ops.sample_decode(ae, z[pick].contiguous(), u[pick].contiguous(), head=head, **s)
+    assert torch.equal(few, ids[pick]) and bool(((lf - logp[pick]).abs() < 1e-3).all())
+
+
+def test_sample_decode_refusals(dev, ae, latents):
+    from style_transfer_amd import ops
+    z, u = latents[:4].contiguous(), torch.rand(4, 59, device=dev)
+    head = ae.quantized_generator()
+    wrong = ops.pack_weight_q4(*ops.quantize_weight_q4(torch.randn(100, 256, device=dev)))
+    for a, b, kw in ((z.half(), u, {}), (z[:, :100], u, {}), (z, u[:, :58], {}), (z, u[:3], {}), (z, u.double(), {}), (z.cpu(), u, {}),
+                     (z, u, dict(head=wrong)), (z, u, dict(head=head.image)), (z, u, dict(top_p=0.0)), (z, u, dict(temperature=-1.0)),
+                     (z, u, dict(top_k=torch.ones(3, dtype=torch.int32, device=dev)))):
+        with pytest.raises(ValueError):
+            ops.sample_decode(ae, a, b, **kw)
+    ids, logp, steps = ops.sample_decode(ae, z[:0], u[:0])
+    assert ids.shape == (0, 59) and steps == 0

@@ -1,0 +1,103 @@
+"""CPU: what st_sample_logits, st_gemm_q4 and st_decode_sample refuse before any GPU call, the sizes they ask for, and the checks of
+their Python callables."""
+import ctypes as C
+
+import pytest
+import torch
+
+from style_transfer_amd import _lib, ops
+
+
+@pytest.fixture(scope="module")
+def L():
+    return _lib.lib()
+
+
+def refused(L, rc, word, code=-1):
+    text = L.st_last_error().decode()
+    assert rc == code and word in text, (rc, text)
+
+
+def settings(**kw):
+    s = _lib.StSampleSettings(1.0, 0, 1.0, 0.0)
+    for k, v in kw.items():
+        setattr(s, k, v)
+    return s
+
+
+def test_sample_arguments(L):
+    buf = C.create_string_buffer(4096)
+    p = C.addressof(buf)
+    call = lambda s=settings(), x=p, kind=0, ld=8, B=2, V=8, u=p, ids=p, ws=None, n=0: L.st_sample_logits(  # noqa: E731
+        x, kind, ld, B, V, u, C.byref(s) if s is not None else None, ids, None, ws, n, None)
+    refused(L, call(None), "settings")
+    for kw, word in ((dict(temperature=-1.0), "temperature"), (dict(temperature=float("nan")), "temperature"),
+                     (dict(temperature=float("inf")), "temperature"), (dict(top_k=-1), "top_k"), (dict(top_p=0.0), "top_p"),
+                     (dict(top_p=1.5), "top_p"), (dict(top_p=float("nan")), "top_p"), (dict(min_p=-0.5), "min_p"), (dict(min_p=2.0), "min_p")):
+        refused(L, call(settings(**kw)), word)
+    refused(L, call(kind=3), "type")
+    refused(L, call(B=-1), "B=")
+    refused(L, call(V=0), "V=")
+    refused(L, call(V=_lib.ST_SAMPLE_MAX_VOCAB + 1), "V=")
+    refused(L, call(ld=-1), "ld=")
+    refused(L, call(x=None), "NULL")
+    refused(L, call(u=None), "NULL")
+    refused(L, call(ids=None), "NULL")
+    refused(L, call(x=p + 2), "size")
+    refused(L, call(x=p + 1, kind=1), "size")
+    refused(L, call(V=131072), "workspace too small", -3)
+    refused(L, call(V=131072, ws=p, n=4096), "workspace too small", -3)
+    refused(L, call(ws=p + 4, n=4096), "16 bytes")
+    assert call(B=0, x=None, u=None, ids=None) == 0
+
+
+def test_sample_workspace(L):
+    assert L.st_sample_workspace_bytes(1, 9339) == 0 and L.st_sample_workspace_bytes(4096, 131072) == 0
+    assert L.st_sample_workspace_bytes(1, 131072) > 0
+    assert L.st_sample_workspace_bytes(0, 100) == 0 and L.st_sample_workspace_bytes(1, 1 << 20) == 0
+
+
+def test_q4_arguments(L):
+    buf = C.create_string_buffer(4096 + 16)
+    p = (C.addressof(buf) + 15) // 16 * 16
+    assert L.st_q4_packed_bytes(64, 128, 128, 0) == 4096 + 256 and L.st_q4_packed_bytes(64, 128, 128, 1) == 4096 + 512
+    assert L.st_q4_packed_bytes(0, 128, 128, 0) == 0 and L.st_q4_packed_bytes(64, 128, 48, 0) == 0
+    refused(L, L.st_pack_weight_q4(p, p, None, 4, 8, 16, p, None), "group")
+    refused(L, L.st_pack_weight_q4(p, p, None, 0, 8, 32, p, None), "positive")
+    refused(L, L.st_pack_weight_q4(p, None, None, 4, 8, 32, p, None), "NULL")
+    refused(L, L.st_pack_weight_q4(p, p, None, 4, 8, 32, p + 4, None), "16 bytes")
+    refused(L, L.st_quantize_weight_q4(p, 4, -8, 32, p, p, None, None), "positive")
+    refused(L, L.st_quantize_weight_q4(None, 4, 8, 32, p, p, None, None), "NULL")
+    w = _lib.StQ4Weight(p, 16, 8, 32, 0)
+    call = lambda w=w, x=p, kind=0, ldx=8, M=2, y=p, ldy=16: L.st_gemm_q4(x, kind, ldx, M, C.byref(w) if w else None, None, y, ldy, None)  # noqa: E731
+    refused(L, call(w=None), "weights")
+    refused(L, call(w=_lib.StQ4Weight(p, 16, 8, 33, 0)), "group")
+    refused(L, call(w=_lib.StQ4Weight(p, 16, 0, 32, 0)), "positive")
+    refused(L, call(w=_lib.StQ4Weight(p + 8, 16, 8, 32, 0)), "16 bytes")
+    refused(L, call(w=_lib.StQ4Weight(None, 16, 8, 32, 0)), "NULL")
+    refused(L, call(kind=7), "type")
+    refused(L, call(M=-1), "M=")
+    refused(L, call(ldx=-8), "ldx")
+    refused(L, call(ldy=15), "overlap")
+    refused(L, call(x=None), "NULL")
+    refused(L, call(y=p + 2), "size")
+    assert call(M=0, x=None, y=None) == 0
+
+
+def test_decode_sample_arguments(L):
+    w = _lib.StDecoderWeights()
+    w.d_model = 512
+    s = settings()
+    rc = L.st_decode_sample(C.byref(w), None, 0, 4, 60, 2, 3, 0, 0, 1, 0, C.byref(s), 0, None, 0, 0, None, None)
+    refused(L, rc, "d_model")
+    assert L.st_decode_sample_workspace_bytes(None, 4, 60, 0) == 0
+
+
+def test_callables_refuse_cpu_tensors():
+    x, u = torch.zeros(2, 8), torch.zeros(2)
+    with pytest.raises(ValueError):
+        ops.sample_logits(x, u)
+    with pytest.raises(ValueError):
+        ops.quantize_weight_q4(x)
+    with pytest.raises(ValueError):
+        ops.pack_weight_q4(torch.zeros(2, 4, dtype=torch.uint8), torch.zeros(2, 1, dtype=torch.float16))
