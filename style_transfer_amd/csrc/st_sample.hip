@@ -672,12 +672,18 @@ __device__ __forceinline__ bool is_greedy(const Settings& o) { return !(o.temp >
 __device__ __forceinline__ bool by_list(const Settings& o, int chunks) { return o.top_k > 0 && o.top_k <= min(min((int)blockDim.x, chunks) / 2, KC); }
 
 // One workgroup a row.  Dynamic shared memory: masses of the bins [nbin], a list of places [nbin / 2] (before that, counts).
-template <int TYPE> __global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs a, int nbin) {
+// LISTS: rows that a sorted list answers (greedy ones, short ones, a top_k that the threads' largest entries bound); BINS: any row.
+// With LISTS alone a row that needs the bins is marked TODO in ids, and BINS alone takes the marked ones (todo) or all.  Apart, the
+// lists' kernel needs 64 registers and the chip holds twice as many rows of it: 4096 x 9339 with top-k 79 us together, 57 apart.
+constexpr int TODO = -2;
+template <int TYPE, bool LISTS, bool BINS, int WAVES>
+__global__ __launch_bounds__(512, WAVES) void sample_row_kernel(SampleArgs a, int nbin, int todo) {
   typedef typename LOf<TYPE>::t T;
   extern __shared__ __align__(16) char dyn[];
   __shared__ Shared sh;
   const int b = blockIdx.x, tid = threadIdx.x, nt = blockDim.x;
   if (a.n_dev && a.row0 + b >= *a.n_dev) return;
+  if (todo && a.ids[b] != TODO) return;
   u64* const mass = (u64*)dyn;
   u64* const list = mass + nbin;
   uint32_t* const count = (uint32_t*)list;
@@ -692,48 +698,56 @@ template <int TYPE> __global__ __launch_bounds__(1024) void sample_row_kernel(Sa
     if (tid == 0) answer_none(a, b);
     return;
   }
-  if (is_greedy(o)) {
-    if (tid == 0) sh.n = 0xffffffffu;
-    __syncthreads();
-    r.template each_if<4>([&](float l) SM_INLINE { return l == top; }, [&](float, int i) SM_INLINE { atomicMin(&sh.n, (uint32_t)i); });
-    __syncthreads();
-    if (tid == 0) answer(a, b, (int)sh.n, 1.0, ONE_MASS);
-    return;
-  }
   const Scale sc = scale_of(o, top);
-  const bool listed = by_list(o, r.chunks);
-  if (listed || a.V <= (int)room) {
-    uint32_t n;
-    if (listed && a.V > 256) {
-      n = gather_top<4>(r, o.top_k, top, own_max, list, room, sh, [](int i) SM_INLINE { return i; });
-    } else {
-      if (tid == 0) sh.n = 0;
+  if constexpr (LISTS) {
+    if (is_greedy(o)) {
+      if (tid == 0) sh.n = 0xffffffffu;
       __syncthreads();
-      r.template each_if<2>([](float l) SM_INLINE { return l > -INFINITY; }, [&](float l, int i) SM_INLINE {
-        const uint32_t at = atomicAdd(&sh.n, 1u);
-        if (at < room) list[at] = place_of(l, i);
-      });
+      r.template each_if<4>([&](float l) SM_INLINE { return l == top; }, [&](float, int i) SM_INLINE { atomicMin(&sh.n, (uint32_t)i); });
       __syncthreads();
-      n = sh.n;
-      __syncthreads();
+      if (tid == 0) answer(a, b, (int)sh.n, 1.0, ONE_MASS);
+      return;
     }
-    if (n <= room) {
-      sort_places(list, (int)n, sh);
-      draw_from_sorted(a, b, list, o.top_k > 0 ? min((int)n, o.top_k) : (int)n, mass, sc, o, sh);
+    const bool listed = by_list(o, r.chunks);
+    if (listed || a.V <= (int)room) {
+      uint32_t n;
+      if (listed && a.V > 256) {
+        n = gather_top<4>(r, o.top_k, top, own_max, list, room, sh, [](int i) SM_INLINE { return i; });
+      } else {
+        if (tid == 0) sh.n = 0;
+        __syncthreads();
+        r.template each_if<2>([](float l) SM_INLINE { return l > -INFINITY; }, [&](float l, int i) SM_INLINE {
+          const uint32_t at = atomicAdd(&sh.n, 1u);
+          if (at < room) list[at] = place_of(l, i);
+        });
+        __syncthreads();
+        n = sh.n;
+        __syncthreads();
+      }
+      if (n <= room) {
+        sort_places(list, (int)n, sh);
+        draw_from_sorted(a, b, list, o.top_k > 0 ? min((int)n, o.top_k) : (int)n, mass, sc, o, sh);
+        return;
+      }
+    }
+    if constexpr (!BINS) {
+      if (tid == 0) a.ids[b] = TODO;
       return;
     }
   }
-  const BinMap map = bins_of(o, top, low, nbin);
-  const bool ranked = o.top_k > 0 && o.top_k < a.V;
-  for (int i = tid; i < nbin; i += nt) {
-    mass[i] = 0;
-    if (ranked) count[i] = 0;
+  if constexpr (BINS) {
+    const BinMap map = bins_of(o, top, low, nbin);
+    const bool ranked = o.top_k > 0 && o.top_k < a.V;
+    for (int i = tid; i < nbin; i += nt) {
+      mass[i] = 0;
+      if (ranked) count[i] = 0;
+    }
+    __syncthreads();
+    u64 over = pass_bins(r, map, sc, o, ranked, mass, count);
+    __syncthreads();
+    if (o.min_p > 0.0f) over = block_sum(over, sh);
+    draw_from_bins<false>(a, b, r, map, sc, o, ranked, over, nbin, mass, count, list, room, sh, RowSpace{}, 0, 0);
   }
-  __syncthreads();
-  u64 over = pass_bins(r, map, sc, o, ranked, mass, count);
-  __syncthreads();
-  if (o.min_p > 0.0f) over = block_sum(over, sh);
-  draw_from_bins<false>(a, b, r, map, sc, o, ranked, over, nbin, mass, count, list, room, sh, RowSpace{}, 0, 0);
 }
 
 // A long row over several workgroups, in three launches: (1) every part's largest entry, and its top_k where a list of them will do;
@@ -920,8 +934,20 @@ template <int TYPE> int launch_type(const SampleArgs& a, hipStream_t st) {
   const int parts = parts_of(a.B, a.V, &len);
   if (parts == 1) {
     const int nbin = a.V <= 1024 ? 2048 : a.V <= 16384 ? 1024 : a.V <= 65536 ? 2048 : 4096;
+    const size_t lds = (size_t)nbin * 12;
     const int threads = a.V <= 2048 ? 256 : 512;
-    hipLaunchKernelGGL((sample_row_kernel<TYPE>), dim3(a.B), dim3(threads), (size_t)nbin * 12, st, a, nbin);
+    const bool alike = !a.set.temperature_rows && !a.set.top_k_rows;
+    const bool lists = a.V <= nbin / 2 || (alike && (!(a.set.temperature > 0.0f) || (a.set.top_k > 0 && a.set.top_k <= 128)));
+    if (lists && a.B >= 512) {
+      hipLaunchKernelGGL((sample_row_kernel<TYPE, true, false, 8>), dim3(a.B), dim3(256), lds, st, a, nbin, 0);
+      ST_LAUNCH_CHECK();
+      if (a.V > nbin / 2 && a.set.top_k != 1 && a.set.temperature > 0.0f)   // equal logits may not have fitted into a list
+        hipLaunchKernelGGL((sample_row_kernel<TYPE, false, true, 4>), dim3(a.B), dim3(threads), lds, st, a, nbin, 1);
+    } else if (alike && !lists) {
+      hipLaunchKernelGGL((sample_row_kernel<TYPE, false, true, 4>), dim3(a.B), dim3(threads), lds, st, a, nbin, 0);
+    } else {
+      hipLaunchKernelGGL((sample_row_kernel<TYPE, true, true, 4>), dim3(a.B), dim3(threads), lds, st, a, nbin, 0);
+    }
     ST_LAUNCH_CHECK();
     return ST_OK;
   }

@@ -95,6 +95,18 @@ def test_sample_many_rows(dev):
         check_sample(logits, u, ids, logp, **s)
 
 
+def test_sample_many_rows_of_ties(dev):
+    """many rows with a top_k: those whose equal logits do not fit into a list, beside rows that do"""
+    from style_transfer_amd import ops
+    logits, u, g = some_logits(dev, 700, 3001, "f32", 6)
+    logits[::3] = torch.randint(0, 3, (3001,), generator=g, device=dev).float()
+    logits[5] = -math.inf
+    logits[6, 7:] = -math.inf
+    for s in (dict(top_k=20, top_p=0.9), dict(top_k=128), dict(top_k=200, min_p=0.01), dict(temperature=0.0), dict(top_k=1)):
+        ids, logp = ops.sample_logits(logits, u, **s)
+        check_sample(logits, u, ids, logp, **s)
+
+
 @pytest.mark.parametrize("v", [524288, 262147])
 def test_sample_largest_vocabulary(dev, v):
     from style_transfer_amd import ops
