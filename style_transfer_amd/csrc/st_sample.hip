@@ -433,6 +433,8 @@ __device__ __forceinline__ u64 pass_bins(const Row<TYPE>& r, const BinMap& map, 
 //   u64 mass[NSPLIT], over; uint32 count[NSPLIT]; Part part[32]; float cand[parts][KC]; int cand_index[parts][KC];
 //   uint32 offset[parts][NSPLIT + 64]; uint16 order[parts][len]: the part's entries by bins, and where a bin of it begins
 constexpr int NSPLIT = 4096, KC = 256, MAX_PARTS = 32, OFFSETS = NSPLIT + 64;
+constexpr int MAX_LEN = 4 * NSPLIT;   // entries of a part: their order lies where the masses of its bins were, two bytes each
+static_assert(MAX_LEN <= 65536 && MAX_LEN * MAX_PARTS >= ST_SAMPLE_MAX_VOCAB, "16-bit order, parts enough");
 struct Part {
   float top, low;
   int first;      // index of its first largest entry (greedy rows)
@@ -578,7 +580,7 @@ __device__ __forceinline__ void draw_from_bins(const SampleArgs& a, int b, const
     u64 prefix = 0;
     int high = 64;   // the bits from `high` on are settled: prefix's
 #pragma unroll 1
-    for (;;) {
+    for (int round = 0; round < 9; ++round) {   // the ninth has 64 bits settled
       auto inside = [&](u64 place) SM_INLINE { return high >= 64 || (place >> high) == (prefix >> high); };
       uint32_t n = n_bin;
       int top_bit = 64;
@@ -677,7 +679,7 @@ __device__ __forceinline__ bool by_list(const Settings& o, int chunks) { return 
 // lists' kernel needs 64 registers and the chip holds twice as many rows of it: 4096 x 9339 with top-k 79 us together, 57 apart.
 constexpr int TODO = -2;
 template <int TYPE, bool LISTS, bool BINS, int WAVES>
-__global__ __launch_bounds__(512, WAVES) void sample_row_kernel(SampleArgs a, int nbin, int todo) {
+__global__ __launch_bounds__(BINS ? 1024 : 512, WAVES) void sample_row_kernel(SampleArgs a, int nbin, int todo) {
   typedef typename LOf<TYPE>::t T;
   extern __shared__ __align__(16) char dyn[];
   __shared__ Shared sh;
@@ -851,16 +853,20 @@ template <int TYPE> __global__ __launch_bounds__(512) void sample_bins_kernel(Sa
   }
   if (tid == nt - 1) ws.offset[(size_t)g * OFFSETS + NSPLIT] = before;
   __syncthreads();
+  uint16_t* const order = (uint16_t*)mass;
   r.template each<4>([&](f32x4 k, int ch) SM_INLINE {
 #pragma unroll
     for (int j = 0; j < Row<TYPE>::EPC; ++j) {
       const float l = r.entry(k, j);
       if (l > -INFINITY) {
         const uint32_t at = atomicAdd(&count[map.bin(l)], 1u);
-        if (at < (uint32_t)len) ws.order[(size_t)g * len + at] = (uint16_t)(ch * Row<TYPE>::EPC + j - r.pad);
+        if (at < (uint32_t)len) order[at] = (uint16_t)(ch * Row<TYPE>::EPC + j - r.pad);
       }
     }
   });
+  __syncthreads();
+  // (places that no entry has are copied too, and never read)
+  for (int i = tid; i < len / 4; i += nt) ((u64*)(ws.order + (size_t)g * len))[i] = mass[i];
 }
 
 constexpr int JOIN_ROOM = MAX_PARTS * KC;   // places in the list: all parts' candidates
@@ -919,12 +925,14 @@ template <int TYPE> __global__ __launch_bounds__(1024) void sample_join_kernel(S
   draw_from_bins<true>(a, b, r, map, sc, o, ranked, over, NSPLIT, mass, count, list, room, sh, ws, parts, len);
 }
 
-// Parts of a row: few long rows leave most of the chip idle, and one workgroup takes its time over a long row
+// Parts of a row: few long rows leave most of the chip idle, and one workgroup takes its time over a long row.  About two workgroups
+// a CU, parts of 4096 entries and more (and MAX_LEN at most); for fewer than four the three launches do not pay.
 int parts_of(int B, int V, int* len) {
   int g = V < 16384 ? 1 : 512 / B;
-  if (g > V / 4096) g = V / 4096;
-  if (g > MAX_PARTS) g = MAX_PARTS;
   if (g < 4) return 1;
+  if (g > V / 4096) g = V / 4096;
+  if (g < (V + MAX_LEN - 1) / MAX_LEN) g = (V + MAX_LEN - 1) / MAX_LEN;
+  if (g > MAX_PARTS) g = MAX_PARTS;
   *len = ((V + g - 1) / g + 63) / 64 * 64;
   return (V + *len - 1) / *len;   // those that have entries
 }
@@ -935,7 +943,8 @@ template <int TYPE> int launch_type(const SampleArgs& a, hipStream_t st) {
   if (parts == 1) {
     const int nbin = a.V <= 1024 ? 2048 : a.V <= 16384 ? 1024 : a.V <= 65536 ? 2048 : 4096;
     const size_t lds = (size_t)nbin * 12;
-    const int threads = a.V <= 2048 ? 256 : 512;
+    // 256 x 131072 bf16: 151 us with 1024, 189 with 512; 128 x 9339: 16.0 and 14.5
+    const int threads = a.V <= 2048 ? 256 : a.V <= 32768 ? 512 : 1024;
     const bool alike = !a.set.temperature_rows && !a.set.top_k_rows;
     const bool lists = a.V <= nbin / 2 || (alike && (!(a.set.temperature > 0.0f) || (a.set.top_k > 0 && a.set.top_k <= 128)));
     if (lists && a.B >= 512) {
@@ -951,6 +960,7 @@ template <int TYPE> int launch_type(const SampleArgs& a, hipStream_t st) {
     ST_LAUNCH_CHECK();
     return ST_OK;
   }
+  ST_CHECK_ARG(parts <= MAX_PARTS && len <= MAX_LEN, "V=%d in %d parts of %d", a.V, parts, len);
   constexpr int join_lds = NSPLIT * 8 + JOIN_ROOM * 8;
   ST_ENSURE_LDS(sample_join_kernel<TYPE>, join_lds);
   hipLaunchKernelGGL((sample_part_kernel<TYPE>), dim3(parts, a.B), dim3(512), 0, st, a, parts, len);

@@ -95,6 +95,18 @@ def test_sample_many_rows(dev):
         check_sample(logits, u, ids, logp, **s)
 
 
+@pytest.mark.parametrize("b,v", [(100, 131072), (70, 262144), (128, 524288), (127, 16384), (129, 70000)])
+def test_sample_parts(dev, b, v):
+    """rows in parts of every size, and just too many rows for it (a few of them against the definition)"""
+    from style_transfer_amd import ops
+    logits, u, _ = some_logits(dev, b, v, "bf16", b)
+    for s in (dict(top_p=0.9), dict(top_k=30, temperature=0.7), dict()):
+        ids, logp = ops.sample_logits(logits, u, **s)
+        pick = [0, 1, b // 2, b - 1]
+        check_sample(logits[pick], u[pick], ids[pick], logp[pick], **s)
+        assert int(ids.min()) >= 0 and int(ids.max()) < v
+
+
 def test_sample_many_rows_of_ties(dev):
     """many rows with a top_k: those whose equal logits do not fit into a list, beside rows that do"""
     from style_transfer_amd import ops
