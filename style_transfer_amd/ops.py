@@ -241,8 +241,8 @@ _TYPES = {torch.float32: _lib.ST_TYPE_F32, torch.bfloat16: _lib.ST_TYPE_BF16, to
 
 
 def _on(t, name, dtype, shape, device=None):
-    """a contiguous GPU tensor of this type and shape (a tuple), or a ValueError that names it"""
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is dtype and t.shape == shape and t.is_contiguous()):
+    """a contiguous GPU tensor of this type and shape, or a ValueError that names it"""
+    if not (torch.is_tensor(t) and t.is_cuda and t.dtype == dtype and tuple(t.shape) == tuple(shape) and t.is_contiguous()):
         raise ValueError("%s: expected a contiguous %s GPU tensor of shape %s, got %s" % (
             name, dtype, tuple(shape), "%s %s on %s" % (t.dtype, tuple(t.shape), t.device) if torch.is_tensor(t) else type(t).__name__))
     if device is not None and t.device != device:
@@ -251,21 +251,20 @@ def _on(t, name, dtype, shape, device=None):
 
 
 def _rows_of(t, name):
-    """-> (type, rows, columns, values between rows) of a 2-d GPU tensor whose rows are contiguous"""
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _TYPES and t.dim() == 2):
+    """-> (type, values between rows) of a 2-d GPU tensor whose rows are contiguous"""
+    if not (torch.is_tensor(t) and t.is_cuda and t.dim() == 2 and t.dtype in _TYPES):
         raise ValueError("%s: expected a 2-d float32, bfloat16 or float16 GPU tensor" % name)
-    rows, cols = t.shape
     ld, one = t.stride()
-    if one != 1 and cols > 1:
+    if one != 1 and t.shape[1] > 1:
         raise ValueError("%s: the values of a row must be contiguous (stride %s)" % (name, t.stride()))
-    return _TYPES[t.dtype], rows, cols, ld
+    return _TYPES[t.dtype], ld
 
 
 def _call(device, name, *args):
-    """one call of the library on `device`'s current stream, whichever device is current.  (The bare handles of the device and the
-    stream: torch's objects around them cost 3 us of a 7 us call.)"""
-    fn, i = getattr(_lib._lib or lib(), name), device.index
-    if i == torch._C._cuda_getDevice():
+    """one call of the library on `device`'s current stream, whichever device is current.  (The stream's bare handle: a Stream
+    object around it costs 2.7 us of a 7 us call.)"""
+    fn, i = getattr(lib(), name), device.index
+    if i == torch.cuda.current_device():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
         with torch.cuda.device(device):
@@ -280,7 +279,6 @@ class Q4Weight:
 
     def __init__(self, image, N, K, group, has_zeros):
         self.image, self.N, self.K, self.group = image, N, K, group
-        self.device = image.device
         self.c = _lib.StQ4Weight(image.data_ptr(), N, K, group, 1 if has_zeros else 0)
         self.ref = C.byref(self.c)
 
@@ -325,21 +323,21 @@ def pack_weight_q4(codes, scales, zeros=None, k=None, group=128):
 def gemm_q4(x, weight, bias=None, out=None):
     """x [M, K] (f32, bf16 or f16; rows may be strided) times a Q4Weight's transpose, plus bias f32 [N] -> [M, N] of x's type
     (written into `out` when given: same type, rows may be strided)."""
-    kind, M, K, ldx = _rows_of(x, "x")
-    dev, N = x.device, weight.N
-    if K != weight.K:
-        raise ValueError("x has %d columns, the weight %d" % (K, weight.K))
-    if weight.device != dev:
-        raise ValueError("the weight is on %s, x on %s" % (weight.device, dev))
+    kind, ldx = _rows_of(x, "x")
+    M, dev = x.shape[0], x.device
+    if x.shape[1] != weight.K:
+        raise ValueError("x has %d columns, the weight %d" % (x.shape[1], weight.K))
+    if weight.image.device != dev:
+        raise ValueError("the weight is on %s, x on %s" % (weight.image.device, dev))
     if bias is not None:
-        _on(bias, "bias", torch.float32, (N,), dev)
+        _on(bias, "bias", torch.float32, (weight.N,), dev)
     if out is None:
-        out, ldy = torch.empty((M, N), dtype=x.dtype, device=dev), N
+        out, ldy = torch.empty(M, weight.N, dtype=x.dtype, device=dev), weight.N
     else:
-        ldy = _rows_of(out, "out")[3]
-        if out.dtype != x.dtype or out.shape != (M, N) or out.device != dev:
-            raise ValueError("out: expected %s of shape %s on %s" % (x.dtype, (M, N), dev))
-    _call(dev, "st_gemm_q4", x.data_ptr(), kind, ldx, M, weight.ref, None if bias is None else bias.data_ptr(), out.data_ptr(), ldy)
+        ldy = _rows_of(out, "out")[1]
+        if out.dtype != x.dtype or tuple(out.shape) != (M, weight.N) or out.device != dev:
+            raise ValueError("out: expected %s of shape %s on %s" % (x.dtype, (M, weight.N), dev))
+    _call(dev, "st_gemm_q4", x.data_ptr(), kind, ldx, M, weight.ref, _p(bias), out.data_ptr(), ldy)
     return out
 
 
@@ -387,14 +385,15 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, wan
     """One token per row of logits [B, V] (f32, bf16 or f16; rows may be strided) from the uniform numbers u [B] (f32, in
     [0, 1)) -> (ids int32 [B], logp f32 [B] or None).  Filters in the order temperature, top_k (0: off), top_p (1: off),
     min_p (0: off); each is a number or a tensor [B].  temperature 0: argmax.  A row of -inf / NaN alone: id -1, logp -inf."""
-    kind, B, V, ld = _rows_of(logits, "logits")
+    kind, ld = _rows_of(logits, "logits")
+    B, V = logits.shape
     dev = logits.device
     if V < 1 or V > _lib.ST_SAMPLE_MAX_VOCAB:
         raise ValueError("logits: rows of %d values (1 .. %d)" % (V, _lib.ST_SAMPLE_MAX_VOCAB))
     _on(u, "u", torch.float32, (B,), dev)
     s = _sample_settings(B, dev, temperature, top_k, top_p, min_p)
-    ids = torch.empty((B,), dtype=torch.int32, device=dev)
-    logp = torch.empty_like(u) if want_logp else None
+    ids = torch.empty(B, dtype=torch.int32, device=dev)
+    logp = torch.empty(B, dtype=torch.float32, device=dev) if want_logp else None
     nbytes = lib().st_sample_workspace_bytes(B, V)
     buf = None if nbytes == 0 else _workspace(ws, nbytes, dev)
     _call(dev, "st_sample_logits", logits.data_ptr(), kind, ld, B, V, u.data_ptr(), C.byref(s), ids.data_ptr(), _p(logp), _p(buf), nbytes)
@@ -412,7 +411,7 @@ def sample_decode(ae, latent, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
     B, T, dev = latent.shape[0], max_len - 1, latent.device
     _on(latent, "latent", torch.float32, (B, 256))
     _on(u, "u", torch.float32, (B, T), dev)
-    if head is not None and (not isinstance(head, Q4Weight) or (head.N, head.K) != (ae.vocab, 256) or head.device != dev):
+    if head is not None and (not isinstance(head, Q4Weight) or (head.N, head.K) != (ae.vocab, 256) or head.image.device != dev):
         raise ValueError("head: expected a Q4Weight [%d, 256] on %s" % (ae.vocab, dev))
     s = _sample_settings(B, dev, temperature, top_k, top_p, min_p)
     ids = torch.empty(B, T, dtype=torch.int32, device=dev)
