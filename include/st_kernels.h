@@ -439,7 +439,8 @@ long long st_format_attack_log(const char* vocab_bytes, const int64_t* vocab_off
  *   scales  f16 [N, ceil(K / group)]       zeros  u8 [N, ceil(K / group)] (0..15; the upper bits are ignored) or NULL: 8
  *   group   32, 64 or 128; the last group of a row may be short
  * st_quantize_weight_q4 makes codes, scales (and zeros, when not NULL) of an f32 matrix [N, K]: scale = max |w| / 7, or
- * (max - min) / 15 with 0 in the range, rounded to f16; a code is the nearest one under the rounded scale.
+ * (max - min) / 15 with 0 in the range, rounded to f16; a code is the nearest one under the rounded scale.  A group that holds a
+ * NaN or an infinity, or whose scale is beyond f16, gets a scale that is not finite, and so does what is multiplied with it.
  * st_pack_weight_q4 lays them out for the product (once per weight); the image takes st_q4_packed_bytes and must lie on 16
  * bytes.  st_gemm_q4: x [M, K] and y [M, N] of `type` (ST_TYPE_*), rows ldx and ldy values apart (any alignment of whole
  * values); bias f32 [N] or NULL.  Sums are held in f32, one rounding to y's type at the end; the codes enter the product as they

@@ -73,7 +73,8 @@ __global__ __launch_bounds__(256) void q4_pack_kernel(const uint8_t* __restrict_
 
 // ---- codes of an f32 matrix ------------------------------------------------------------------------------------------------
 // One wave a (row, group).  Without zero codes: s = max |w| / 7 and z = 8; with them the range [min(w, 0), max(w, 0)] is cut into
-// 15 steps and z is 0's place in it.  s is rounded to f16 first, the codes go by the rounded one.
+// 15 steps and z is 0's place in it.  s is rounded to f16 first, the codes go by the rounded one.  A group with a NaN or an infinity
+// has s NaN, one whose s is beyond f16 has s infinite, with the codes of 0: neither is taken for ordinary weights.
 __global__ __launch_bounds__(256) void q4_quantize_kernel(const float* __restrict__ W, int N, int K, int group, uint8_t* __restrict__ codes,
                                                           _Float16* __restrict__ scales, uint8_t* __restrict__ zeros) {
   const int groups = (K + group - 1) / group, lane = threadIdx.x & 63;
@@ -84,8 +85,9 @@ __global__ __launch_bounds__(256) void q4_quantize_kernel(const float* __restric
   const bool in0 = 2 * lane < group && k < K, in1 = 2 * lane < group && k + 1 < K;
   const float a = in0 ? W[(size_t)n * K + k] : 0.0f, b = in1 ? W[(size_t)n * K + k + 1] : 0.0f;
   const float hi = wave_max(fmaxf(fmaxf(a, b), 0.0f)), lo = -wave_max(fmaxf(fmaxf(-a, -b), 0.0f));
-  const float step = zeros ? (hi - lo) / 15.0f : fmaxf(hi, -lo) / 7.0f;
-  const _Float16 s16 = (_Float16)fminf(step, 65504.0f);
+  const bool finite = !__any(!(fabsf(a) < INFINITY && fabsf(b) < INFINITY));
+  const float step = !finite ? NAN : zeros ? (hi - lo) / 15.0f : fmaxf(hi, -lo) / 7.0f;
+  const _Float16 s16 = (_Float16)step;
   const float s = (float)s16;
   const int z = zeros ? (s > 0.0f ? min(15, max(0, (int)rintf(-lo / s))) : 0) : 8;
   const int c0 = s > 0.0f ? min(15, max(0, (int)fminf(fmaxf(rintf(a / s), -16.0f), 16.0f) + z)) : z;

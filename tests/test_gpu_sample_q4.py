@@ -394,6 +394,24 @@ def test_quantize_weight_q4(dev, group, zeros):
     check_product(W[:9], w, None, y, "f32")
 
 
+@pytest.mark.parametrize("m", [1, 40])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_quantize_weight_q4_not_finite(dev, zeros, m):
+    """a weight that 4 bits and an f16 scale cannot hold is seen in the product, in its row alone"""
+    from style_transfer_amd import ops
+    g = torch.Generator(device=dev).manual_seed(5)
+    W = torch.randn(12, 96, generator=g, device=dev)
+    W[1, 40], W[4, 0], W[5, 95], W[7, 33], W[9, 64] = float("nan"), float("inf"), -float("inf"), 2.0e6, -3.0e38
+    W[9, 65] = 3.0e38                      # the range itself is beyond f32
+    codes, scales, z = ops.quantize_weight_q4(W, 32, zeros)
+    x = torch.randn(m, 96, generator=g, device=dev)
+    y = ops.gemm_q4(x, ops.pack_weight_q4(codes, scales, z, group=32))
+    bad = [1, 4, 5, 7, 9]
+    good = [i for i in range(12) if i not in bad]
+    assert not torch.isfinite(y[:, bad]).any()
+    check_product(x, weight_of(codes[good], scales[good], None if z is None else z[good], 96, 32), None, y[:, good], "f32")
+
+
 def test_gemm_q4_graph_and_stream(dev):
     from style_transfer_amd import ops
     codes, scales, z, g = some_weight(dev, 1000, 512, 64, True, 4)
