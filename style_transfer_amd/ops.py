@@ -320,9 +320,25 @@ def pack_weight_q4(codes, scales, zeros=None, k=None, group=128):
     return Q4Weight(image, N, K, group, zeros is not None)
 
 
+def _share_values(a, b):
+    """whether two 2-d tensors of one type, the values of a row contiguous, have a byte in common; columns of one buffer, side by
+    side, have none"""
+    if 0 in a.shape or 0 in b.shape:
+        return False
+    size, (p, q) = a.element_size(), (a.data_ptr(), b.data_ptr())
+    end = lambda t: t.data_ptr() + size * ((t.shape[0] - 1) * t.stride(0) + t.shape[1])   # noqa: E731
+    if end(a) <= q or end(b) <= p:
+        return False
+    row = a.stride(0) * size
+    if row != b.stride(0) * size or row == 0:
+        return True
+    off = (q - p) % row
+    return not (off >= a.shape[1] * size and off + b.shape[1] * size <= row)
+
+
 def gemm_q4(x, weight, bias=None, out=None):
     """x [M, K] (f32, bf16 or f16; rows may be strided) times a Q4Weight's transpose, plus bias f32 [N] -> [M, N] of x's type
-    (written into `out` when given: same type, rows may be strided)."""
+    (written into `out` when given: same type, rows may be strided, no value of x's).  Has no gradient."""
     kind, ldx = _rows_of(x, "x")
     M, dev = x.shape[0], x.device
     if x.shape[1] != weight.K:
@@ -337,6 +353,8 @@ def gemm_q4(x, weight, bias=None, out=None):
         ldy = _rows_of(out, "out")[1]
         if out.dtype != x.dtype or tuple(out.shape) != (M, weight.N) or out.device != dev:
             raise ValueError("out: expected %s of shape %s on %s" % (x.dtype, (M, weight.N), dev))
+        if _share_values(x, out):
+            raise ValueError("out shares values with x")
     _call(dev, "st_gemm_q4", x.data_ptr(), kind, ldx, M, weight.ref, _p(bias), out.data_ptr(), ldy)
     return out
 

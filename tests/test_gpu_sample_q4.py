@@ -458,6 +458,19 @@ def test_q4_refusals(dev):
     assert ops.gemm_q4(x[:0], q).shape == (0, 40)
 
 
+def test_gemm_q4_out_and_x_in_one_buffer(dev):
+    from style_transfer_amd import ops
+    codes, scales, z, g = some_weight(dev, 128, 128, 64, True, 2)
+    q = ops.pack_weight_q4(codes, scales, z, group=64)
+    buf = torch.randn(40, 300, generator=g, device=dev)
+    want = ops.gemm_q4(buf[:, :128], q)
+    for a, b in ((buf[:, :128], buf[:, :128]), (buf[:, :128], buf[:, 100:228]), (buf[1:, :128], buf[:39, :128])):
+        with pytest.raises(ValueError, match="shares"):
+            ops.gemm_q4(a, q, out=b)
+    ops.gemm_q4(buf[:, :128], q, out=buf[:, 130:258])
+    assert torch.equal(buf[:, 130:258], want)
+
+
 # ---- in a row ---------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("rows", [1, 64, 200])

@@ -101,3 +101,19 @@ def test_callables_refuse_cpu_tensors():
         ops.quantize_weight_q4(x)
     with pytest.raises(ValueError):
         ops.pack_weight_q4(torch.zeros(2, 4, dtype=torch.uint8), torch.zeros(2, 1, dtype=torch.float16))
+
+
+def test_values_in_common():
+    """against the sets of addresses themselves"""
+    def addresses(t):
+        return {t.data_ptr() + 4 * (i * t.stride(0) + j) for i in range(t.shape[0]) for j in range(t.shape[1])}
+    buf = torch.zeros(400)
+    views = [buf.as_strided((m, n), (ld, 1), at) for m in (1, 3) for n, ld in ((5, 5), (5, 20), (12, 20), (7, 9)) for at in (0, 4, 5, 12, 26, 60)]
+    for a in views:
+        for b in views:
+            common = bool(addresses(a) & addresses(b))
+            got = ops._share_values(a, b)
+            assert got or not common
+    wide = torch.zeros(6, 20)
+    assert not ops._share_values(wide[:, :8], wide[:, 8:]) and not ops._share_values(wide[:, 8:], wide[:, :8])
+    assert ops._share_values(wide[:, :8], wide[:, 7:]) and ops._share_values(wide, wide) and not ops._share_values(wide[:0], wide)
