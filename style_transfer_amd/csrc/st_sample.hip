@@ -676,7 +676,7 @@ __device__ __forceinline__ bool by_list(const Settings& o, int chunks) { return 
 // One workgroup a row.  Dynamic shared memory: masses of the bins [nbin], a list of places [nbin / 2] (before that, counts).
 // LISTS: rows that a sorted list answers (greedy ones, short ones, a top_k that the threads' largest entries bound); BINS: any row.
 // With LISTS alone a row that needs the bins is marked TODO in ids, and BINS alone takes the marked ones (todo) or all.  Apart, the
-// lists' kernel needs 64 registers and the chip holds twice as many rows of it: 4096 x 9339 with top-k 79 us together, 57 apart.
+// lists' kernel needs 64 registers and the chip holds twice as many rows of it: 4096 x 9339 with top-k 79 us together, 59 apart.
 constexpr int TODO = -2;
 template <int TYPE, bool LISTS, bool BINS, int WAVES>
 __global__ __launch_bounds__(BINS ? 1024 : 512, WAVES) void sample_row_kernel(SampleArgs a, int nbin, int todo) {
