@@ -712,10 +712,9 @@ __global__ __launch_bounds__(BINS ? 1024 : 512, WAVES) void sample_row_kernel(Sa
     }
     const bool listed = by_list(o, r.chunks);
     if (listed || a.V <= (int)room) {
-      uint32_t n;
-      if (listed && a.V > 256) {
-        n = gather_top<4>(r, o.top_k, top, own_max, list, room, sh, [](int i) SM_INLINE { return i; });
-      } else {
+      uint32_t n = room + 1;
+      if (listed && a.V > 256) n = gather_top<4>(r, o.top_k, top, own_max, list, room, sh, [](int i) SM_INLINE { return i; });
+      if (n > room && a.V <= (int)room) {   // all entries, where they fit: also those of a row with fewer than top_k threads that have one
         if (tid == 0) sh.n = 0;
         __syncthreads();
         r.template each_if<2>([](float l) SM_INLINE { return l > -INFINITY; }, [&](float l, int i) SM_INLINE {
@@ -950,7 +949,8 @@ template <int TYPE> int launch_type(const SampleArgs& a, hipStream_t st) {
     if (lists && a.B >= 512) {
       hipLaunchKernelGGL((sample_row_kernel<TYPE, true, false, 8>), dim3(a.B), dim3(256), lds, st, a, nbin, 0);
       ST_LAUNCH_CHECK();
-      if (a.V > nbin / 2 && a.set.top_k != 1 && a.set.temperature > 0.0f)   // equal logits may not have fitted into a list
+      // rows marked: their equal logits did not fit into a list, or too few threads had an entry (a list of nbin / 2 takes any shorter row)
+      if (a.V > nbin / 2 && a.set.top_k != 1 && a.set.temperature > 0.0f)
         hipLaunchKernelGGL((sample_row_kernel<TYPE, false, true, 4>), dim3(a.B), dim3(threads), lds, st, a, nbin, 1);
     } else if (alike && !lists) {
       hipLaunchKernelGGL((sample_row_kernel<TYPE, false, true, 4>), dim3(a.B), dim3(threads), lds, st, a, nbin, 0);

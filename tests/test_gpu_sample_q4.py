@@ -616,3 +616,27 @@ def test_sample_decode_refusals(dev, ae, latents):
             ops.sample_decode(ae, a, b, **kw)
     ids, logp, steps = ops.sample_decode(ae, z[:0], u[:0])
     assert ids.shape == (0, 59) and steps == 0
+
+
+# ---- more rows, settings and inputs that the documentation allows -------------------------------------------------------
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("b", [511, 512, 513])
+@pytest.mark.parametrize("v", [257, 300, 777, 1000, 1024, 1025, 2600])
+def test_sample_many_short_rows_masked(dev, b, v, kind):
+    """many rows with a top_k, on both sides of every size at which another kernel takes them: rows with none, one, a few, top_k - 1,
+    top_k and all of their entries left, the entries side by side or spread out, and rows of ties; one setting for all and arrays"""
+    from style_transfer_amd import ops
+    logits, u, g = some_logits(dev, b, v, kind, b + v)
+    k = max(2, min(50, v // 12))
+    live = torch.tensor([0, 1, 3, k - 1, k, v], device=dev)[torch.arange(b, device=dev) % 6]
+    place = torch.arange(v, device=dev).repeat(b, 1)
+    place[b // 2:] = torch.rand(b - b // 2, v, generator=g, device=dev).argsort(1)
+    masked = torch.tensor([-math.inf, float("nan")], device=dev, dtype=logits.dtype)[torch.arange(b, device=dev) % 2][:, None]
+    logits = torch.where(place < live[:, None], logits, masked)
+    logits[5::12] = torch.randint(0, 3, (v,), generator=g, device=dev).to(logits.dtype)
+    ks = torch.tensor([k, 0, 1, k + 7, v], dtype=torch.int32, device=dev)[torch.randint(0, 5, (b,), generator=g, device=dev)]
+    for s in (dict(top_k=k, top_p=0.9), dict(top_k=k, min_p=0.01, temperature=1.4), dict(top_k=ks, temperature=0.8), dict(top_k=1)):
+        ids, logp = ops.sample_logits(logits, u, **s)
+        assert int(ids.min()) == -1
+        check_sample(logits, u, ids, logp, **s)
