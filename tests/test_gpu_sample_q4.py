@@ -640,3 +640,31 @@ def test_sample_many_short_rows_masked(dev, b, v, kind):
         ids, logp = ops.sample_logits(logits, u, **s)
         assert int(ids.min()) == -1
         check_sample(logits, u, ids, logp, **s)
+
+
+def rows_of_the_whole_range(dev, v, kind, seed):
+    """rows whose largest and smallest logits are farther apart than f32's largest number (f16's own range is 131008 wide)"""
+    g = torch.Generator(device=dev).manual_seed(seed)
+    most = torch.finfo(TYPES[kind]).max
+    at = torch.rand(12, v, generator=g, device=dev)
+    rows = at * 2 * (most / 2) - most / 2
+    rows[0:4] = torch.where(at[0:4] < 0.5, 0.88 * most, -0.88 * most)
+    rows[4:8] = torch.where(at[4:8] < 0.5, most, -most)
+    rows[8:10] *= 1.99
+    rows[10, ::3] = -math.inf
+    rows[11, ::3] = math.inf
+    u = torch.rand(12, generator=g, device=dev)
+    u[::2] = 1 - 2.0 ** -24               # among the last entries, far from the top
+    return rows.to(TYPES[kind]), u
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("v", [300, 3000, 9339, 40000])
+def test_sample_whole_range_of_logits(dev, v, kind):
+    """temperatures from which logits at both ends of the type share the mass"""
+    from style_transfer_amd import ops
+    logits, u = rows_of_the_whole_range(dev, v, kind, v)
+    for t in (3e4, 1.05e37, 1.07e37, 3e37, 1e38):
+        for s in (dict(), dict(top_k=700), dict(top_p=0.9), dict(top_k=20), dict(min_p=0.3)):
+            ids, logp = ops.sample_logits(logits, u, temperature=t, **s)
+            check_sample(logits, u, ids, logp, temperature=t, **s)
