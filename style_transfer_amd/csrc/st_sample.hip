@@ -404,9 +404,9 @@ __device__ __forceinline__ uint32_t gather_top(const Row<TYPE>& r, int k, float 
 // bins reach down to 32 temperatures under the top (e^-32 < 2^-45: no mass beyond), or to the lowest logit if that is nearer; the
 // largest f32 at most, so that no place is 0 x infinity (what is farther below the top lies in the last bin)
 __device__ __forceinline__ BinMap bins_of(const Settings& o, float top, float low, int nbin) {
-  return {top, (float)nbin / fmaxf(fminf(fminf(32.0f * fminf(o.temp, 3.4e38f), top + low), 3.4e38f), 1e-30f), (float)(nbin - 1)};
+  return {top, (float)nbin / fmaxf(fminf(fminf(32.0f * o.temp, top + low), 3.4e38f), 1e-30f), (float)(nbin - 1)};
 }
-__device__ __forceinline__ Scale scale_of(const Settings& o, float top) { return {top, 1.4426950408889634 / (double)fminf(o.temp, 3.4e38f)}; }
+__device__ __forceinline__ Scale scale_of(const Settings& o, float top) { return {top, 1.4426950408889634 / (double)o.temp}; }
 
 // masses (and counts, where a rank is asked for) of the bins; -> this thread's mass of the entries with w >= min_p
 template <int TYPE>

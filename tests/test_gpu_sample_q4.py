@@ -668,3 +668,17 @@ def test_sample_whole_range_of_logits(dev, v, kind):
         for s in (dict(), dict(top_k=700), dict(top_p=0.9), dict(top_k=20), dict(min_p=0.3)):
             ids, logp = ops.sample_logits(logits, u, temperature=t, **s)
             check_sample(logits, u, ids, logp, temperature=t, **s)
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("v", [300, 3000, 40000])
+def test_sample_largest_temperatures(dev, v, kind):
+    """f32's largest temperature, and an infinite one in an array: every finite logit has the same weight"""
+    from style_transfer_amd import ops
+    logits, u = rows_of_the_whole_range(dev, v, kind, v + 1)
+    logits = logits[:11]
+    u = u[:11].contiguous()
+    for t in (torch.finfo(torch.float32).max, torch.full((11,), torch.finfo(torch.float32).max, device=dev), torch.full((11,), math.inf, device=dev)):
+        for s in (dict(), dict(top_k=700), dict(top_p=0.9), dict(top_k=20), dict(min_p=0.3)):
+            ids, logp = ops.sample_logits(logits, u, temperature=t, **s)
+            check_sample(logits, u, ids, logp, temperature=t, **s)
