@@ -3,9 +3,10 @@
 // A weight is read as a code c in 0..15; c - z is a whole number in -15..15, which f16 holds exactly, so the matrix cores
 // multiply f16 images of x with f16 whole numbers (v_mfma_f32_16x16x32_f16, sums in f32) and the scale is applied in f32 once a
 // group: no weight is rounded.  x in f16 goes in as it is.  x in bf16 or f32 is first multiplied, row by row, with a power of
-// two that brings the row's largest value to [2^14, 2^15): a bf16 value then is an f16 value (8 significant bits of 11; what is
-// 2^-29 of the largest and less becomes an f16 subnormal, an error below 2^-39 of the largest), an f32 value is split into
-// hi + lo as in the f16x3 format (about 2^-22 of the value) and costs two products.
+// two that brings the row's largest value to [2^14, 2^15).  A bf16 value then is an f16 value (8 significant bits of 11); what is
+// below 2^-31 of the largest loses bits as an f16 subnormal, rounded to the nearest: an error of 2^-39 of the row's largest at
+// most.  An f32 value is split into hi + lo, each to the nearest, and costs two products: an error of 2^-23 of the value or 2^-39
+// of the row's largest, whichever is more.
 #include "st_common.h"
 
 namespace {
@@ -182,7 +183,7 @@ template <int TYPE> struct X8 {
     for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(value(i)));
     return m;
   }
-  // the values times 2^14 over the row's power of two as f16: rounded towards 0, and for f32 what that leaves, to the nearest
+  // the values times 2^14 over the row's power of two as f16, to the nearest, and for f32 what that leaves, to the nearest
   __device__ __forceinline__ void split(float shift, h8& hi, h8& lo) const {
     if constexpr (TYPE == ST_TYPE_F16) {
       hi = __builtin_bit_cast(h8, *(const u32x4*)w);
@@ -191,9 +192,9 @@ template <int TYPE> struct X8 {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float a = value(2 * i) * shift, b = value(2 * i + 1) * shift;
-        h[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+        const h2 q = {(_Float16)a, (_Float16)b};   // (one instruction)
+        h[i] = __builtin_bit_cast(uint32_t, q);
         if constexpr (TYPE == ST_TYPE_F32) {
-          const h2 q = __builtin_bit_cast(h2, h[i]);
           lo[2 * i] = (_Float16)fmaxf(a - (float)q[0], -65504.0f);        // an infinity: inf - inf is not wanted
           lo[2 * i + 1] = (_Float16)fmaxf(b - (float)q[1], -65504.0f);
         }

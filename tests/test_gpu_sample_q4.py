@@ -682,3 +682,36 @@ def test_sample_largest_temperatures(dev, v, kind):
         for s in (dict(), dict(top_k=700), dict(top_p=0.9), dict(top_k=20), dict(min_p=0.3)):
             ids, logp = ops.sample_logits(logits, u, temperature=t, **s)
             check_sample(logits, u, ids, logp, temperature=t, **s)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("m,n,k,outlier", [(47, 64, 90, 0), (47, 64, 90, 89), (47, 100, 700, 3), (47, 100, 1500, 1499), (256, 4100, 6200, 0), (256, 4100, 6200, 6199)])
+def test_gemm_q4_small_values_beside_an_outlier(dev, m, n, k, outlier, kind):
+    """one value of a row is far larger than the others and has weight 0 (its code is the zero code): what is left is the others'
+    product, each with an error of 2^-39 of the outlier at most, f32 ones of 2^-23 of themselves if that is more, beside the f32
+    sums' own (all x and w positive, so that errors of one direction add up, and mixed signs)"""
+    from style_transfer_amd import ops
+    g = torch.Generator(device=dev).manual_seed(m + k + outlier)
+    codes = torch.randint(0, 256, (n, k // 2), generator=g, device=dev, dtype=torch.uint8)
+    scales = (0.01 * (0.1 + torch.rand(n, -(-k // 64), generator=g, device=dev))).half()
+    for signs in (False, True):
+        c = codes if signs else codes | 0x88
+        at, keep = outlier // 2, 0xf0 if outlier % 2 == 0 else 0x0f
+        c = c.clone()
+        c[:, at] = (c[:, at] & keep) | (0x88 & ~keep)
+        far = 2.0 ** -(torch.arange(m, device=dev) % 47).float()[:, None]
+        x = far * (1 + torch.rand(m, k, generator=g, device=dev))
+        if signs:
+            x = torch.where(torch.rand(m, k, generator=g, device=dev) < 0.5, x, -x)
+        x[:, outlier] = 1.0
+        x = x.to(TYPES[kind])
+        y = ops.gemm_q4(x, ops.pack_weight_q4(c, scales, group=64), None).float().cpu().numpy().astype(np.float64)
+        w, x64 = weight_of(c, scales, None, k, 64), x.float().cpu().numpy().astype(np.float64)
+        assert (w[:, outlier] == 0).all()
+        want, a = x64 @ w.T, np.abs(w)
+        value = np.maximum((2.0 ** -23 if kind == "f32" else 0.0) * np.abs(x64), 2.0 ** -39 * np.abs(x64).max(1, keepdims=True))
+        tol = value @ a.T + (k + 64) * 2.0 ** -24 * (np.abs(x64) @ a.T)
+        tol += HALF_STEP[kind] * (np.abs(want) + tol)
+        over = np.abs(y - want) - tol
+        i = np.unravel_index(np.argmax(over), over.shape)
+        assert over[i] <= 0, "%s: %r, want %r, may differ by %.3g" % (i, y[i], want[i], tol[i])
