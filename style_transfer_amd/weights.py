@@ -98,7 +98,8 @@ class AEWeights(_Packed):
         self.dec.emb, self.dec.pe = self.emb_ptr, self.pe_ptr
         self.dec.lnf_a, self.dec.lnf_b = self.dev(sd["decoder.norm.a_2"]), self.dev(sd["decoder.norm.b_2"])
         self.dec.gen_w, self.dec.gen_b = self.packed(sd["generator.proj.weight"]), self.dev(sd["generator.proj.bias"])
-        self._generator = sd["generator.proj.weight"]
+        # for quantized_generator: a copy of its own (the caller may train on), in host memory (most users need no second image)
+        self._generator = sd["generator.proj.weight"].detach().to(device="cpu", dtype=torch.float32, copy=True)
         for l in range(self.n_layers):
             p = "decoder.layers.%d." % l
             y = self.dec.layer[l]
@@ -164,9 +165,10 @@ class AEWeights(_Packed):
 
 
     def quantized_generator(self, group=64, zero_points=False):
-        """the generator matrix [vocab, 256] in 4 bits with a scale per `group` columns (ops.Q4Weight): ops.sample_decode's head"""
+        """the generator matrix [vocab, 256], as it was given to this object, in 4 bits with a scale per `group` columns
+        (ops.Q4Weight): ops.sample_decode's head"""
         from . import ops
-        W = self._generator.detach().to(device=self.device, dtype=torch.float32).contiguous()
+        W = self._generator.to(self.device).contiguous()
         return ops.pack_weight_q4(*ops.quantize_weight_q4(W, group, zero_points), group=group)
 
 

@@ -715,3 +715,13 @@ def test_gemm_q4_small_values_beside_an_outlier(dev, m, n, k, outlier, kind):
         over = np.abs(y - want) - tol
         i = np.unravel_index(np.argmax(over), over.shape)
         assert over[i] <= 0, "%s: %r, want %r, may differ by %.3g" % (i, y[i], want[i], tol[i])
+
+
+def test_quantized_generator_of_weights_that_train_on(dev, ae_sd_torch):
+    """the 4-bit head is that of the weights that were packed, whatever the caller does with its tensors afterwards"""
+    from style_transfer_amd.weights import AEWeights
+    sd = {k: v.clone() for k, v in ae_sd_torch.items()}
+    want = AEWeights(ae_sd_torch, dev, l0_table=False).quantized_generator(32, True).image
+    ae = AEWeights(sd, dev, l0_table=False)
+    sd["generator.proj.weight"].mul_(3.0).add_(1.0)
+    assert torch.equal(ae.quantized_generator(32, True).image, want)
