@@ -338,7 +338,8 @@ def _share_values(a, b):
 
 def gemm_q4(x, weight, bias=None, out=None):
     """x [M, K] (f32, bf16 or f16; rows may be strided) times a Q4Weight's transpose, plus bias f32 [N] -> [M, N] of x's type
-    (written into `out` when given: same type, rows may be strided, no value of x's).  Has no gradient."""
+    (written into `out` when given: same type, rows may be strided, no value of x's).  Has no gradient: where one would be lost
+    (grad mode on, x or bias requires it) the call is refused."""
     kind, ldx = _rows_of(x, "x")
     M, dev = x.shape[0], x.device
     if x.shape[1] != weight.K:
@@ -347,6 +348,8 @@ def gemm_q4(x, weight, bias=None, out=None):
         raise ValueError("the weight is on %s, x on %s" % (weight.image.device, dev))
     if bias is not None:
         _on(bias, "bias", torch.float32, (weight.N,), dev)
+    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+        raise ValueError("gemm_q4 has no gradient: call it under torch.no_grad(), or with detached tensors")
     if out is None:
         out, ldy = torch.empty(M, weight.N, dtype=x.dtype, device=dev), weight.N
     else:
@@ -402,7 +405,8 @@ def _workspace(ws, nbytes, device):
 def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, want_logp=True, ws: DecodeWorkspace = None):
     """One token per row of logits [B, V] (f32, bf16 or f16; rows may be strided) from the uniform numbers u [B] (f32, in
     [0, 1)) -> (ids int32 [B], logp f32 [B] or None).  Filters in the order temperature, top_k (0: off), top_p (1: off),
-    min_p (0: off); each is a number or a tensor [B].  temperature 0: argmax.  A row of -inf / NaN alone: id -1, logp -inf."""
+    min_p (0: off); each is a number or a tensor [B].  temperature 0: argmax.  A row of -inf / NaN alone: id -1, logp -inf.
+    logp is a value: no gradient goes from it to the logits."""
     kind, ld = _rows_of(logits, "logits")
     B, V = logits.shape
     dev = logits.device

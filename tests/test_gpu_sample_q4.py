@@ -725,3 +725,20 @@ def test_quantized_generator_of_weights_that_train_on(dev, ae_sd_torch):
     ae = AEWeights(sd, dev, l0_table=False)
     sd["generator.proj.weight"].mul_(3.0).add_(1.0)
     assert torch.equal(ae.quantized_generator(32, True).image, want)
+
+
+def test_gemm_q4_refuses_to_lose_a_gradient(dev):
+    from style_transfer_amd import ops
+    codes, scales, z, g = some_weight(dev, 40, 128, 64, True, 1)
+    q = ops.pack_weight_q4(codes, scales, z, group=64)
+    x, bias = torch.randn(4, 128, generator=g, device=dev), torch.randn(40, generator=g, device=dev)
+    want = ops.gemm_q4(x, q, bias)
+    leaf, row = x.clone().requires_grad_(), bias.clone().requires_grad_()
+    for a, b in ((leaf, None), (leaf * 1.0, bias), (x, row)):
+        with pytest.raises(ValueError, match="gradient"):
+            ops.gemm_q4(a, q, b)
+    with torch.no_grad():
+        assert torch.equal(ops.gemm_q4(leaf, q, row), want)
+    with torch.inference_mode():
+        assert torch.equal(ops.gemm_q4(leaf, q, row), want)
+    assert torch.equal(ops.gemm_q4(leaf.detach(), q, bias), want)
