@@ -432,6 +432,8 @@ def sample_decode(ae, latent, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
         raise ValueError("latent: expected [B, 256]")
     B, T, dev = latent.shape[0], max_len - 1, latent.device
     _on(latent, "latent", torch.float32, (B, 256))
+    if ae.where != dev:
+        raise ValueError("the weights are on %s, latent on %s" % (ae.where, dev))
     _on(u, "u", torch.float32, (B, T), dev)
     if head is not None and (not isinstance(head, Q4Weight) or (head.N, head.K) != (ae.vocab, 256) or head.image.device != dev):
         raise ValueError("head: expected a Q4Weight [%d, 256] on %s" % (ae.vocab, dev))

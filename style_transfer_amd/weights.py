@@ -86,6 +86,7 @@ class AEWeights(_Packed):
         self.max_len = max_len
         pe = positional_encoding(max(max_len, 64), self.d_model)
         self.emb_ptr = self.dev(emb)
+        self.where = self._keep[-1].device   # `device` with its number
         self.pe_ptr = self.dev(pe)
         self.dec = _lib.StDecoderWeights()
         for s in (self.dec,):
@@ -168,7 +169,7 @@ class AEWeights(_Packed):
         """the generator matrix [vocab, 256], as it was given to this object, in 4 bits with a scale per `group` columns
         (ops.Q4Weight): ops.sample_decode's head"""
         from . import ops
-        W = self._generator.to(self.device).contiguous()
+        W = self._generator.to(self.where).contiguous()
         return ops.pack_weight_q4(*ops.quantize_weight_q4(W, group, zero_points), group=group)
 
 

@@ -742,3 +742,13 @@ def test_gemm_q4_refuses_to_lose_a_gradient(dev):
     with torch.inference_mode():
         assert torch.equal(ops.gemm_q4(leaf, q, row), want)
     assert torch.equal(ops.gemm_q4(leaf.detach(), q, bias), want)
+
+
+def test_sample_decode_refuses_weights_elsewhere(dev, ae, latents):
+    import copy
+    from style_transfer_amd import ops
+    assert ae.where == latents.device
+    other = copy.copy(ae)
+    other.where = torch.device("cuda", 1)
+    with pytest.raises(ValueError, match="weights are on"):
+        ops.sample_decode(other, latents[:2].contiguous(), torch.rand(2, 59, device=dev))
