@@ -1087,8 +1087,8 @@ static int decode_loop(const StDecoderWeights* w, const float* latent, int B, in
     ST_HIP(hipMemcpyAsync(&flag, ws.cnt + 3, sizeof(int), hipMemcpyDeviceToHost, st));
     ST_HIP(hipStreamSynchronize(st));
     if (flag) {
-      st_set_error("st_decode_greedy: an activation left the f16 range (|x| >= 65504 or NaN) in the f16x3 format; "
-                   "the decoded ids are invalid - pack the weights with ST_GEMM_F32");
+      st_set_error("%s: an activation left the f16 range (|x| >= 65504 or NaN) in the f16x3 format; "
+                   "the decoded ids are invalid - pack the weights with ST_GEMM_F32", sm ? "st_decode_sample" : "st_decode_greedy");
       return ST_ERANGE;
     }
   }

@@ -752,3 +752,18 @@ def test_sample_decode_refuses_weights_elsewhere(dev, ae, latents):
     other.where = torch.device("cuda", 1)
     with pytest.raises(ValueError, match="weights are on"):
         ops.sample_decode(other, latents[:2].contiguous(), torch.rand(2, 59, device=dev))
+
+
+@pytest.mark.parametrize("head_bits", [0, 4])
+def test_sample_decode_range_error_names_its_entry_point(dev, ae_sd_torch, head_bits):
+    from style_transfer_amd import _lib, ops
+    from style_transfer_amd.weights import AEWeights
+    sd = {k: v.clone() for k, v in ae_sd_torch.items()}
+    sd["decoder.layers.1.feed_forward.w_1.weight"] *= 3e4
+    ae = AEWeights(sd, dev, l0_table=False)
+    latent, u = torch.rand(48, 256, device=dev) * 8, torch.rand(48, 59, device=dev)
+    with pytest.raises(_lib.StError, match="f16 range") as e:
+        ops.sample_decode(ae, latent, u, head=ae.quantized_generator() if head_bits else None)
+    assert "st_decode_greedy" not in str(e.value)
+    with pytest.raises(_lib.StError, match="st_decode_greedy: an activation"):
+        ops.greedy_decode(ae, latent)
