@@ -739,9 +739,10 @@ struct DecodeWs {
   void* smp;       // the draw's own workspace
   size_t total;
 };
-// rows of logits that are held at a time: 256 MB of them, 64 rows at least
+// rows of logits that are held at a time: 256 MB of them, 64 rows at least, and no more than the 4-bit product takes in one call
 static int sample_rows(const StDecoderWeights* w, int B) {
-  const long r = ((256L << 20) / ((long)w->vocab * 4) + 63) / 64 * 64;
+  long r = ((256L << 20) / ((long)w->vocab * 4) + 63) / 64 * 64;
+  if (r > ST_Q4_MAX_ROWS) r = ST_Q4_MAX_ROWS / 64 * 64;
   return r < B ? (int)(r < 64 ? 64 : r) : B;
 }
 // what a sampled decode has beside a greedy one's arguments

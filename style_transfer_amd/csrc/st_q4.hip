@@ -588,7 +588,7 @@ extern "C" int st_gemm_q4(const void* x, int type, int64_t ldx, int M, const StQ
   ST_CHECK_ARG(w != nullptr, "weights struct is NULL");
   ST_TRY(check_q4_shape(w->N, w->K, w->group));
   ST_CHECK_ARG(type == ST_TYPE_F32 || type == ST_TYPE_BF16 || type == ST_TYPE_F16, "type=%d unknown", type);
-  ST_CHECK_ARG(M >= 0 && M <= 65535 * 16, "M=%d (0 .. %d)", M, 65535 * 16);
+  ST_CHECK_ARG(M >= 0 && M <= ST_Q4_MAX_ROWS, "M=%d (0 .. %d)", M, ST_Q4_MAX_ROWS);
   if (M == 0) return ST_OK;
   ST_CHECK_ARG(x && w->image && y, "NULL buffer");
   ST_CHECK_ARG(((size_t)w->image & 15) == 0, "the packed image must lie on 16 bytes");

@@ -117,3 +117,13 @@ def test_values_in_common():
     wide = torch.zeros(6, 20)
     assert not ops._share_values(wide[:, :8], wide[:, 8:]) and not ops._share_values(wide[:, 8:], wide[:, :8])
     assert ops._share_values(wide[:, :8], wide[:, 7:]) and ops._share_values(wide, wide) and not ops._share_values(wide[:0], wide)
+
+
+def test_sample_decode_holds_as_many_rows_as_the_product_takes(L):
+    """a small vocabulary and very many sentences: the logits held at a time are rows that st_gemm_q4 takes in one call"""
+    up = lambda v: (v + 255) // 256 * 256  # noqa: E731
+    for vocab, B, rows in ((60, 1100000, 65535 * 16 // 64 * 64), (60, 4096, 4096), (9339, 20000, 7232), (1, 1 << 21, 65535 * 16 // 64 * 64)):
+        w = _lib.StDecoderWeights()
+        w.d_model, w.n_heads, w.d_ff, w.n_layers, w.vocab, w.pe_rows = 256, 4, 1024, 2, vocab, 64
+        more = L.st_decode_sample_workspace_bytes(C.byref(w), B, 2, 4) - L.st_decode_workspace_bytes_opt(C.byref(w), B, 2, 4)
+        assert more == up(rows * vocab * 4) + 2 * up(B * 4)
