@@ -478,7 +478,8 @@ int st_gemm_q4(const void* x, int type, int64_t ldx, int M, const StQ4Weight* w,
  * finite, top_k < 0, top_p outside (0, 1], min_p outside [0, 1]); array values act as written above, with temperature <= 0 or
  * NaN greedy, an infinite one w = 1 for every finite logit, top_k <= 0 off, top_p <= 0 the first entry alone, top_p >= 1 or NaN off,
  * min_p <= 0 or NaN off, min_p > 1 the first alone.
- * u is clamped to [0, 1]; a NaN counts as 0.  V <= ST_SAMPLE_MAX_VOCAB.  B = 0 is a no-op.  Asynchronous, may be captured into
+ * u is clamped to [0, 1]; a NaN counts as 0.  V <= ST_SAMPLE_MAX_VOCAB.  B = 0 is a no-op; 4 194 303 rows are taken at any V, more at
+ * V <= 32768 (8 388 607) and V <= 2048 (16 777 215); ST_EINVAL beyond, one launch holds no more.  Asynchronous, may be captured into
  * a graph; calls that overlap need workspaces of their own (nothing in one has to be cleared).                              */
 #define ST_SAMPLE_MAX_VOCAB 524288
 typedef struct StSampleSettings {

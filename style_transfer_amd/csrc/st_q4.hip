@@ -512,7 +512,7 @@ template <int TYPE, int GPB, int MT, int NT, int WM, int WN> int launch_tile(con
   constexpr int lds = 2 * PARTS * ROWS * 256 + 2 * ROWS * 4 + 16;
   const int tiles_m = (a.M + ROWS - 1) / ROWS, tiles_n = (a.nb + COLS - 1) / COLS;
   const long grid = (long)(tiles_n + 7) / 8 * 8 * tiles_m;
-  ST_CHECK_ARG(grid < (1L << 31), "M=%d N=%d: too large for one launch", a.M, a.N);
+  ST_CHECK_ARG(grid * 64 * WM * WN < (1L << 32), "M=%d N=%d: too large for one launch", a.M, a.N);
   ST_ENSURE_LDS((q4_tile_kernel<TYPE, GPB, MT, NT, WM, WN>), lds);
   hipLaunchKernelGGL((q4_tile_kernel<TYPE, GPB, MT, NT, WM, WN>), dim3((unsigned)grid), dim3(64 * WM * WN), lds, st, a, tiles_m, tiles_n);
   ST_LAUNCH_CHECK();

@@ -947,6 +947,8 @@ template <int TYPE> int launch_type(const SampleArgs& a, hipStream_t st) {
     const int threads = a.V <= 2048 ? 256 : a.V <= 32768 ? 512 : 1024;
     const bool alike = !a.set.temperature_rows && !a.set.top_k_rows;
     const bool lists = a.V <= nbin / 2 || (alike && (!(a.set.temperature > 0.0f) || (a.set.top_k > 0 && a.set.top_k <= 128)));
+    const long rows = ((1L << 32) - 1) / threads;   // a launch has fewer than 2^32 threads
+    ST_CHECK_ARG(a.B <= rows, "B=%d: at most %ld rows of %d values in one call", a.B, rows, a.V);
     if (lists && a.B >= 512) {
       hipLaunchKernelGGL((sample_row_kernel<TYPE, true, false, 8>), dim3(a.B), dim3(256), lds, st, a, nbin, 0);
       ST_LAUNCH_CHECK();

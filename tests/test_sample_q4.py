@@ -127,3 +127,14 @@ def test_sample_decode_holds_as_many_rows_as_the_product_takes(L):
         w.d_model, w.n_heads, w.d_ff, w.n_layers, w.vocab, w.pe_rows = 256, 4, 1024, 2, vocab, 64
         more = L.st_decode_sample_workspace_bytes(C.byref(w), B, 2, 4) - L.st_decode_workspace_bytes_opt(C.byref(w), B, 2, 4)
         assert more == up(rows * vocab * 4) + 2 * up(B * 4)
+
+
+def test_sample_rows_of_one_launch(L):
+    """more rows than a launch has threads for are refused before it (2^32 threads, 256 to 1024 of them a row)"""
+    buf = C.create_string_buffer(4096)
+    p = C.addressof(buf)
+    for V, most in ((1, (1 << 24) - 1), (2048, (1 << 24) - 1), (2049, (1 << 23) - 1), (32768, (1 << 23) - 1), (32769, (1 << 22) - 1), (524288, (1 << 22) - 1)):
+        for B in (most + 1, (1 << 31) - 1):
+            for kw in (dict(), dict(top_k=5), dict(temperature=0.0), dict(temperature_rows=p)):
+                s = settings(**kw)
+                refused(L, L.st_sample_logits(p, 1, 0, B, V, p, C.byref(s), p, None, None, 0, None), "at most %d rows" % most)
