@@ -22,6 +22,7 @@ ST_GEMM_F32, ST_GEMM_F16X3 = 0, 1
 GEMM_FORMATS = {"f32": ST_GEMM_F32, "f16x3": ST_GEMM_F16X3}
 ST_TYPE_F32, ST_TYPE_BF16, ST_TYPE_F16 = 0, 1, 2
 ST_SAMPLE_MAX_VOCAB = 524288
+ST_Q4_MAX_ROWS, ST_Q4_MAX_SIDE = 65535 * 16, 1 << 24
 ABI_VERSION = 9
 
 fp = C.c_void_p  # device pointers travel as integers

@@ -273,6 +273,12 @@ def _call(device, name, *args):
         check(rc, name)
 
 
+def _q4_sides(N, K):
+    """sizes that the library takes (and that its 32-bit arguments hold)"""
+    if max(N, K) > _lib.ST_Q4_MAX_SIDE:
+        raise ValueError("a [%d, %d] weight: at most %d rows and columns" % (N, K, _lib.ST_Q4_MAX_SIDE))
+
+
 class Q4Weight:
     """A packed [N, K] weight of 4-bit codes with a scale (and a zero code) per group of columns: st_pack_weight_q4's image
     and the struct that st_gemm_q4 takes."""
@@ -291,6 +297,7 @@ def quantize_weight_q4(W, group=128, zero_points=False):
     if group not in (32, 64, 128):
         raise ValueError("group %r: expected 32, 64 or 128" % (group,))
     N, K = W.shape
+    _q4_sides(N, K)
     g = -(-K // group)
     codes = torch.empty(N, (K + 1) // 2, dtype=torch.uint8, device=W.device)
     scales = torch.empty(N, g, dtype=torch.float16, device=W.device)
@@ -310,6 +317,7 @@ def pack_weight_q4(codes, scales, zeros=None, k=None, group=128):
     K = 2 * codes.shape[1] if k is None else int(k)
     if K < 1 or (K + 1) // 2 != codes.shape[1]:
         raise ValueError("codes: %d bytes a row do not hold k = %d columns" % (codes.shape[1], K))
+    _q4_sides(N, K)
     shape = (N, -(-K // group))
     _on(scales, "scales", torch.float16, shape, codes.device)
     if zeros is not None:
@@ -342,6 +350,8 @@ def gemm_q4(x, weight, bias=None, out=None):
     (grad mode on, x or bias requires it) the call is refused."""
     kind, ldx = _rows_of(x, "x")
     M, dev = x.shape[0], x.device
+    if M > _lib.ST_Q4_MAX_ROWS:
+        raise ValueError("x has %d rows: at most %d in one call" % (M, _lib.ST_Q4_MAX_ROWS))
     if x.shape[1] != weight.K:
         raise ValueError("x has %d columns, the weight %d" % (x.shape[1], weight.K))
     if weight.image.device != dev:
@@ -412,6 +422,8 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, wan
     dev = logits.device
     if V < 1 or V > _lib.ST_SAMPLE_MAX_VOCAB:
         raise ValueError("logits: rows of %d values (1 .. %d)" % (V, _lib.ST_SAMPLE_MAX_VOCAB))
+    if B >= 1 << 31:
+        raise ValueError("logits: %d rows do not fit into 32 bits" % B)
     _on(u, "u", torch.float32, (B,), dev)
     s = _sample_settings(B, dev, temperature, top_k, top_p, min_p)
     ids = torch.empty(B, dtype=torch.int32, device=dev)

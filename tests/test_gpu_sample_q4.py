@@ -767,3 +767,21 @@ def test_sample_decode_range_error_names_its_entry_point(dev, ae_sd_torch, head_
     assert "st_decode_greedy" not in str(e.value)
     with pytest.raises(_lib.StError, match="st_decode_greedy: an activation"):
         ops.greedy_decode(ae, latent)
+
+
+def test_sizes_beyond_32_bits_are_refused(dev):
+    """the C entry points take 32-bit sizes: 2^32 + 3 rows are not 3 rows"""
+    from style_transfer_amd import ops
+    far, u = (1 << 32) + 3, torch.rand(3, device=dev)
+    with pytest.raises(ValueError, match="32 bits"):
+        ops.sample_logits(torch.zeros(1, 1, device=dev).expand(far, 1), u)
+    q = ops.pack_weight_q4(*ops.quantize_weight_q4(torch.ones(4, 8, device=dev), 32), k=8, group=32)
+    for m in ((1 << 20), far):
+        with pytest.raises(ValueError, match="at most"):
+            ops.gemm_q4(torch.zeros(1, 8, device=dev).expand(m, 8), q)
+    with pytest.raises(ValueError, match="at most"):
+        ops.quantize_weight_q4(torch.empty(far, 1, device=dev), 32)
+    with pytest.raises(ValueError, match="at most"):
+        ops.quantize_weight_q4(torch.empty(1, (1 << 24) + 1, device=dev), 32)
+    with pytest.raises(ValueError, match="at most"):
+        ops.pack_weight_q4(torch.empty(far, 1, device=dev, dtype=torch.uint8), torch.empty(1, 1, device=dev, dtype=torch.float16).expand(far, 1), group=32)
