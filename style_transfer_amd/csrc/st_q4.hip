@@ -46,29 +46,32 @@ int check_q4_shape(int N, int K, int group) {
 // codes (bytes) lie block by block, [16 l][4 t][groups of the block]: a lane reads those of its four rows at once.  Rows from N on
 // and groups from K on have scale 0.
 __global__ __launch_bounds__(256) void q4_pack_kernel(const uint8_t* __restrict__ codes, const uint16_t* __restrict__ scales,
-                                                      const uint8_t* __restrict__ zeros, int N, int K, int group, int kb_n,
+                                                      const uint8_t* __restrict__ zeros, int N, int K, int group, int kb_n, size_t tiles,
                                                       uint32_t* __restrict__ out, uint16_t* __restrict__ out_s, uint8_t* __restrict__ out_z) {
   const int row_bytes = (K + 1) / 2, groups = (K + group - 1) / group, gpb = KB / group;
-  const int t = blockIdx.x & 3, j = threadIdx.x & 3, lane = threadIdx.x >> 2;   // one workgroup a tile, a thread a word
-  const size_t b = blockIdx.x >> 2;
-  const int kb = (int)(b % kb_n), n = (int)(b / kb_n) * 64 + 16 * t + (lane & 15);
-  const int k0 = kb * KB + 32 * j + 8 * (lane >> 4);
-  uint32_t w = 0;
-  if (n < N)
-    for (int i = 0; i < 8; ++i) {
-      const int k = k0 + i;
-      if (k < K) {
-        const uint32_t c = (codes[(size_t)n * row_bytes + (k >> 1)] >> (4 * (k & 1))) & 15u;
-        w |= c << (4 * ((i >> 1) + 4 * (i & 1)));
+  const int j = threadIdx.x & 3, lane = threadIdx.x >> 2;   // a workgroup a tile at a time, a thread a word
+  for (size_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const int t = (int)(tile & 3);
+    const size_t b = tile >> 2;
+    const int kb = (int)(b % kb_n), n = (int)(b / kb_n) * 64 + 16 * t + (lane & 15);
+    const int k0 = kb * KB + 32 * j + 8 * (lane >> 4);
+    uint32_t w = 0;
+    if (n < N)
+      for (int i = 0; i < 8; ++i) {
+        const int k = k0 + i;
+        if (k < K) {
+          const uint32_t c = (codes[(size_t)n * row_bytes + (k >> 1)] >> (4 * (k & 1))) & 15u;
+          w |= c << (4 * ((i >> 1) + 4 * (i & 1)));
+        }
       }
+    out[tile * 256 + threadIdx.x] = w;
+    if (threadIdx.x < 16 * gpb) {
+      const int l = threadIdx.x / gpb, i = threadIdx.x % gpb, row = (int)(b / kb_n) * 64 + 16 * t + l, g = kb * gpb + i;
+      const size_t at = ((b * 16 + l) * 4 + t) * gpb + i;
+      const bool in = row < N && g < groups;
+      out_s[at] = in ? scales[(size_t)row * groups + g] : (uint16_t)0;
+      if (out_z) out_z[at] = in ? (uint8_t)(zeros[(size_t)row * groups + g] & 15) : (uint8_t)0;
     }
-  out[(size_t)blockIdx.x * 256 + threadIdx.x] = w;
-  if (threadIdx.x < 16 * gpb) {
-    const int l = threadIdx.x / gpb, i = threadIdx.x % gpb, row = (int)(b / kb_n) * 64 + 16 * t + l, g = kb * gpb + i;
-    const size_t at = ((b * 16 + l) * 4 + t) * gpb + i;
-    const bool in = row < N && g < groups;
-    out_s[at] = in ? scales[(size_t)row * groups + g] : (uint16_t)0;
-    if (out_z) out_z[at] = in ? (uint8_t)(zeros[(size_t)row * groups + g] & 15) : (uint8_t)0;
   }
 }
 
@@ -79,24 +82,24 @@ __global__ __launch_bounds__(256) void q4_pack_kernel(const uint8_t* __restrict_
 __global__ __launch_bounds__(256) void q4_quantize_kernel(const float* __restrict__ W, int N, int K, int group, uint8_t* __restrict__ codes,
                                                           _Float16* __restrict__ scales, uint8_t* __restrict__ zeros) {
   const int groups = (K + group - 1) / group, lane = threadIdx.x & 63;
-  const size_t wv = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (wv >= (size_t)N * groups) return;
-  const int n = (int)(wv / groups), g = (int)(wv % groups);
-  const int k = g * group + 2 * lane;                 // lanes 0 .. group / 2 - 1 have two columns each
-  const bool in0 = 2 * lane < group && k < K, in1 = 2 * lane < group && k + 1 < K;
-  const float a = in0 ? W[(size_t)n * K + k] : 0.0f, b = in1 ? W[(size_t)n * K + k + 1] : 0.0f;
-  const float hi = wave_max(fmaxf(fmaxf(a, b), 0.0f)), lo = -wave_max(fmaxf(fmaxf(-a, -b), 0.0f));
-  const bool finite = !__any(!(fabsf(a) < INFINITY && fabsf(b) < INFINITY));
-  const float step = !finite ? NAN : zeros ? (hi - lo) / 15.0f : fmaxf(hi, -lo) / 7.0f;
-  const _Float16 s16 = (_Float16)step;
-  const float s = (float)s16;
-  const int z = zeros ? (s > 0.0f ? min(15, max(0, (int)rintf(-lo / s))) : 0) : 8;
-  const int c0 = s > 0.0f ? min(15, max(0, (int)fminf(fmaxf(rintf(a / s), -16.0f), 16.0f) + z)) : z;
-  const int c1 = s > 0.0f ? min(15, max(0, (int)fminf(fmaxf(rintf(b / s), -16.0f), 16.0f) + z)) : z;
-  if (in0) codes[(size_t)n * ((K + 1) / 2) + (k >> 1)] = (uint8_t)(c0 | (in1 ? c1 << 4 : 0));
-  if (lane == 0) {
-    scales[wv] = s16;
-    if (zeros) zeros[wv] = (uint8_t)z;
+  for (size_t wv = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6); wv < (size_t)N * groups; wv += (size_t)gridDim.x * 4) {
+    const int n = (int)(wv / groups), g = (int)(wv % groups);
+    const int k = g * group + 2 * lane;                 // lanes 0 .. group / 2 - 1 have two columns each
+    const bool in0 = 2 * lane < group && k < K, in1 = 2 * lane < group && k + 1 < K;
+    const float a = in0 ? W[(size_t)n * K + k] : 0.0f, b = in1 ? W[(size_t)n * K + k + 1] : 0.0f;
+    const float hi = wave_max(fmaxf(fmaxf(a, b), 0.0f)), lo = -wave_max(fmaxf(fmaxf(-a, -b), 0.0f));
+    const bool finite = !__any(!(fabsf(a) < INFINITY && fabsf(b) < INFINITY));
+    const float step = !finite ? NAN : zeros ? (hi - lo) / 15.0f : fmaxf(hi, -lo) / 7.0f;
+    const _Float16 s16 = (_Float16)step;
+    const float s = (float)s16;
+    const int z = zeros ? (s > 0.0f ? min(15, max(0, (int)rintf(-lo / s))) : 0) : 8;
+    const int c0 = s > 0.0f ? min(15, max(0, (int)fminf(fmaxf(rintf(a / s), -16.0f), 16.0f) + z)) : z;
+    const int c1 = s > 0.0f ? min(15, max(0, (int)fminf(fmaxf(rintf(b / s), -16.0f), 16.0f) + z)) : z;
+    if (in0) codes[(size_t)n * ((K + 1) / 2) + (k >> 1)] = (uint8_t)(c0 | (in1 ? c1 << 4 : 0));
+    if (lane == 0) {
+      scales[wv] = s16;
+      if (zeros) zeros[wv] = (uint8_t)z;
+    }
   }
 }
 
@@ -557,6 +560,9 @@ extern "C" size_t st_q4_packed_bytes(int N, int K, int group, int has_zeros) {
   return q4_layout(N, K, group, has_zeros).total;
 }
 
+// workgroups of 256 threads for so many pieces of a weight: a launch has fewer than 2^32 threads, beyond 2^23 a workgroup takes several
+static unsigned weight_blocks(size_t pieces) { return (unsigned)(pieces < (1u << 23) ? pieces : 1u << 23); }
+
 extern "C" int st_pack_weight_q4(const uint8_t* codes, const void* scales, const uint8_t* zeros, int N, int K, int group, void* out_packed,
                                  void* stream) {
   ST_TRY(check_q4_shape(N, K, group));
@@ -564,10 +570,9 @@ extern "C" int st_pack_weight_q4(const uint8_t* codes, const void* scales, const
   ST_CHECK_ARG(((size_t)out_packed & 15) == 0, "the packed image must lie on 16 bytes");
   const Q4Layout y = q4_layout(N, K, group, zeros != nullptr);
   const size_t tiles = (size_t)y.sb * y.kb * 4;
-  ST_CHECK_ARG(tiles < (1ull << 31), "N=%d K=%d: too large for one launch", N, K);
   char* out = (char*)out_packed;
-  hipLaunchKernelGGL(q4_pack_kernel, dim3((unsigned)tiles), dim3(256), 0, (hipStream_t)stream, codes, (const uint16_t*)scales,
-                     zeros, N, K, group, y.kb, (uint32_t*)out, (uint16_t*)(out + y.scales), zeros ? (uint8_t*)(out + y.zeros) : nullptr);
+  hipLaunchKernelGGL(q4_pack_kernel, dim3(weight_blocks(tiles)), dim3(256), 0, (hipStream_t)stream, codes, (const uint16_t*)scales,
+                     zeros, N, K, group, y.kb, tiles, (uint32_t*)out, (uint16_t*)(out + y.scales), zeros ? (uint8_t*)(out + y.zeros) : nullptr);
   ST_LAUNCH_CHECK();
   return ST_OK;
 }
@@ -576,8 +581,7 @@ extern "C" int st_quantize_weight_q4(const float* W, int N, int K, int group, ui
   ST_TRY(check_q4_shape(N, K, group));
   ST_CHECK_ARG(W && codes && scales, "NULL buffer");
   const size_t waves = (size_t)N * ((K + group - 1) / group);
-  ST_CHECK_ARG(waves / 4 < (1ull << 31) - 1, "N=%d K=%d: too large for one launch", N, K);
-  hipLaunchKernelGGL(q4_quantize_kernel, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, (hipStream_t)stream, W, N, K, group, codes,
+  hipLaunchKernelGGL(q4_quantize_kernel, dim3(weight_blocks((waves + 3) / 4)), dim3(256), 0, (hipStream_t)stream, W, N, K, group, codes,
                      (_Float16*)scales, zeros);
   ST_LAUNCH_CHECK();
   return ST_OK;

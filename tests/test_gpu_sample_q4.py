@@ -785,3 +785,31 @@ def test_sizes_beyond_32_bits_are_refused(dev):
         ops.quantize_weight_q4(torch.empty(1, (1 << 24) + 1, device=dev), 32)
     with pytest.raises(ValueError, match="at most"):
         ops.pack_weight_q4(torch.empty(far, 1, device=dev, dtype=torch.uint8), torch.empty(1, 1, device=dev, dtype=torch.float16).expand(far, 1), group=32)
+
+
+def test_quantize_weight_q4_of_2_32_values(dev):
+    """more groups than a launch has waves for: rows from all over against the same rows by themselves"""
+    from style_transfer_amd import ops
+    n, k = 262144 + 3, 16384
+    W = torch.empty(n, k, device=dev)
+    for i in range(0, n, 32768):
+        W[i:i + 32768].normal_(0, 0.1, generator=torch.Generator(device=dev).manual_seed(i))
+    codes, scales, zeros = ops.quantize_weight_q4(W, 32, True)
+    for part in (slice(0, 50), slice(n // 4 - 25, n // 4 + 25), slice(n // 2 - 25, n // 2 + 25), slice(n - 50, n)):
+        c, s, z = ops.quantize_weight_q4(W[part].clone(), 32, True)
+        assert torch.equal(c, codes[part]) and torch.equal(s, scales[part]) and torch.equal(z, zeros[part])
+
+
+def test_pack_weight_q4_of_2_35_codes(dev):
+    """an image of 2^34 bytes and more: its first, middle and last rows in a product"""
+    from style_transfer_amd import ops
+    n, k = (1 << 20) + 5, 32768
+    g = torch.Generator(device=dev).manual_seed(3)
+    codes = torch.empty(n, k // 2, dtype=torch.uint8, device=dev)
+    for i in range(0, n, 131072):
+        codes[i:i + 131072] = torch.randint(0, 256, codes[i:i + 131072].shape, generator=g, device=dev, dtype=torch.uint8)
+    scales = (0.01 * (0.1 + torch.rand(n, k // 128, generator=g, device=dev))).half()
+    x = torch.randn(2, k, generator=g, device=dev).half()
+    y = ops.gemm_q4(x, ops.pack_weight_q4(codes, scales))
+    for part in (slice(0, 40), slice(n // 2 - 20, n // 2 + 20), slice(n - 40, n)):
+        check_product(x, weight_of(codes[part], scales[part], None, k, 128), None, y[:, part], "f16")
