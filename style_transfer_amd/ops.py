@@ -329,25 +329,25 @@ def pack_weight_q4(codes, scales, zeros=None, k=None, group=128):
 
 
 def _share_values(a, b):
-    """whether two 2-d tensors of one type, the values of a row contiguous, have a byte in common; columns of one buffer, side by
-    side, have none"""
+    """whether two 2-d tensors, the values of a row contiguous, have a byte in common; columns of one buffer, side by side, have none"""
     if 0 in a.shape or 0 in b.shape:
         return False
-    size, (p, q) = a.element_size(), (a.data_ptr(), b.data_ptr())
-    end = lambda t: t.data_ptr() + size * ((t.shape[0] - 1) * t.stride(0) + t.shape[1])   # noqa: E731
-    if end(a) <= q or end(b) <= p:
+    p, q, wide_a, wide_b = a.data_ptr(), b.data_ptr(), a.shape[1] * a.element_size(), b.shape[1] * b.element_size()
+    row, row_b = a.stride(0) * a.element_size(), b.stride(0) * b.element_size()
+    if p + (a.shape[0] - 1) * row + wide_a <= q or q + (b.shape[0] - 1) * row_b + wide_b <= p:
         return False
-    row = a.stride(0) * size
-    if row != b.stride(0) * size or row == 0:
+    if b.shape[0] == 1:
+        row_b = row
+    if row != row_b or row == 0:
         return True
     off = (q - p) % row
-    return not (off >= a.shape[1] * size and off + b.shape[1] * size <= row)
+    return not (off >= wide_a and off + wide_b <= row)
 
 
 def gemm_q4(x, weight, bias=None, out=None):
     """x [M, K] (f32, bf16 or f16; rows may be strided) times a Q4Weight's transpose, plus bias f32 [N] -> [M, N] of x's type
-    (written into `out` when given: same type, rows may be strided, no value of x's).  Has no gradient: where one would be lost
-    (grad mode on, x or bias requires it) the call is refused."""
+    (written into `out` when given: same type, rows may be strided, no value of x's or the bias's).  Has no gradient: where one
+    would be lost (grad mode on, x or bias requires it) the call is refused."""
     kind, ldx = _rows_of(x, "x")
     M, dev = x.shape[0], x.device
     if M > _lib.ST_Q4_MAX_ROWS:
@@ -368,6 +368,8 @@ def gemm_q4(x, weight, bias=None, out=None):
             raise ValueError("out: expected %s of shape %s on %s" % (x.dtype, (M, weight.N), dev))
         if _share_values(x, out):
             raise ValueError("out shares values with x")
+        if bias is not None and _share_values(out, bias[None]):
+            raise ValueError("out shares values with bias")
     _call(dev, "st_gemm_q4", x.data_ptr(), kind, ldx, M, weight.ref, _p(bias), out.data_ptr(), ldy)
     return out
 

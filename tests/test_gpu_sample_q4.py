@@ -813,3 +813,18 @@ def test_pack_weight_q4_of_2_35_codes(dev):
     y = ops.gemm_q4(x, ops.pack_weight_q4(codes, scales))
     for part in (slice(0, 40), slice(n // 2 - 20, n // 2 + 20), slice(n - 40, n)):
         check_product(x, weight_of(codes[part], scales[part], None, k, 128), None, y[:, part], "f16")
+
+
+def test_gemm_q4_out_and_bias_in_one_buffer(dev):
+    from style_transfer_amd import ops
+    codes, scales, z, g = some_weight(dev, 128, 128, 64, True, 2)
+    q = ops.pack_weight_q4(codes, scales, z, group=64)
+    x, buf = torch.randn(40, 128, generator=g, device=dev), torch.randn(40, 300, generator=g, device=dev)
+    want = ops.gemm_q4(x, q, buf[3, 150:278].clone())
+    for bias in (buf[3, :128], buf[0, 100:228], buf[39, 127:255]):
+        with pytest.raises(ValueError, match="shares values with bias"):
+            ops.gemm_q4(x, q, bias, out=buf[:, :128])
+    with pytest.raises(ValueError, match="shares values with bias"):
+        ops.gemm_q4(x[:1].bfloat16(), q, buf[3, :128], out=buf.view(torch.bfloat16)[3:4, 254:382])
+    ops.gemm_q4(x, q, buf[3, 150:278], out=buf[:, :128])       # beside the columns that are written
+    assert torch.equal(buf[:, :128], want)

@@ -138,3 +138,19 @@ def test_sample_rows_of_one_launch(L):
             for kw in (dict(), dict(top_k=5), dict(temperature=0.0), dict(temperature_rows=p)):
                 s = settings(**kw)
                 refused(L, L.st_sample_logits(p, 1, 0, B, V, p, C.byref(s), p, None, None, 0, None), "at most %d rows" % most)
+
+
+def test_values_in_common_of_two_types():
+    """a row and a strided tensor of another type in one buffer, against the sets of bytes themselves"""
+    def of(t):
+        return {t.data_ptr() + t.element_size() * (i * t.stride(0) + j) + b for i in range(t.shape[0]) for j in range(t.shape[1]) for b in range(t.element_size())}
+    buf = torch.zeros(200)
+    half = buf.view(torch.bfloat16)
+    rows = [buf.as_strided((1, n), (n, 1), at) for n in (3, 9) for at in (0, 4, 7, 20, 33)]
+    for t in [half.as_strided((m, n), (ld, 1), at) for m in (1, 4) for n, ld in ((6, 6), (6, 20), (12, 44)) for at in (0, 7, 13)]:
+        for r in rows:
+            common = bool(of(t) & of(r))
+            got = ops._share_values(t, r)
+            assert got or not common
+    wide = torch.zeros(6, 40).view(torch.bfloat16)
+    assert not ops._share_values(wide[:, :40], wide.view(torch.float32)[2:3, 20:]) and ops._share_values(wide[:, :41], wide.view(torch.float32)[2:3, 20:])
