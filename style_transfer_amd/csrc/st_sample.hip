@@ -33,10 +33,6 @@ template <int TYPE> __device__ __forceinline__ float logit(typename LOf<TYPE>::t
   else f = (float)v;
   return f == f ? f : -INFINITY;
 }
-template <int TYPE> __device__ __forceinline__ typename LOf<TYPE>::t no_entry() {
-  if constexpr (TYPE == ST_TYPE_BF16) return 0xff80;
-  else return (typename LOf<TYPE>::t)-INFINITY;
-}
 
 // ascending keys are descending logits; -0 and 0 are one value.  An entry's place in the walk is (key, index) in one number.
 __device__ __forceinline__ uint32_t key_of(float l) {
@@ -173,7 +169,7 @@ struct Shared {
 
 // Sums over the lanes up to this one, by row shifts and row broadcasts: no way through shared memory
 #define SM_DPP(v, ctrl, rows) __builtin_amdgcn_update_dpp(0, (int)(v), ctrl, rows, 0xf, false)
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v, int) {
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
   v += SM_DPP(v, 0x111, 0xf);   // row_shr:1, 2, 4, 8 (lanes from outside a row of 16 count 0)
   v += SM_DPP(v, 0x112, 0xf);
   v += SM_DPP(v, 0x114, 0xf);
@@ -182,7 +178,7 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v, int) {
   v += SM_DPP(v, 0x143, 0xc);   // row_bcast:31 into rows 2 and 3
   return v;
 }
-__device__ __forceinline__ u64 wave_scan(u64 v, int) {
+__device__ __forceinline__ u64 wave_scan(u64 v) {
 #define SM_ADD(ctrl, rows) v += (u64)(uint32_t)SM_DPP(v >> 32, ctrl, rows) << 32 | (uint32_t)SM_DPP(v, ctrl, rows)
   SM_ADD(0x111, 0xf);
   SM_ADD(0x112, 0xf);
@@ -194,7 +190,7 @@ __device__ __forceinline__ u64 wave_scan(u64 v, int) {
   return v;
 }
 __device__ __forceinline__ u64 block_sum(u64 v, Shared& sh) {
-  v = wave_scan(v, 0);
+  v = wave_scan(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 63) sh.wave_u64[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -313,7 +309,7 @@ __device__ __forceinline__ void draw_from_sorted(const SampleArgs& a, int b, con
     if (w >= (double)o.min_p) over += m;
     cum[e] = sum;
   }
-  u64 base = wave_scan(sum, lane);
+  u64 base = wave_scan(sum);
   if (lane == 63) sh.wave_u64[wv] = base;
   base -= sum;
   __syncthreads();
@@ -379,7 +375,7 @@ __device__ __forceinline__ uint32_t gather_top(const Row<TYPE>& r, int k, float 
     uint32_t c[4], before = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) c[i] = sh.digit_count[4 * lane + i], before += c[i];
-    before = wave_scan(before, lane) - before;
+    before = wave_scan(before) - before;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (before < (uint32_t)k && (uint32_t)k <= before + c[i]) sh.found_bin = 4 * lane + i;
@@ -483,8 +479,8 @@ __device__ __forceinline__ void draw_from_bins(const SampleArgs& a, int b, const
   }
   const u64 own_mass = base_mass;
   const uint32_t own_count = base_count;
-  base_mass = wave_scan(base_mass, lane);
-  base_count = wave_scan(base_count, lane);
+  base_mass = wave_scan(base_mass);
+  base_count = wave_scan(base_count);
   if (lane == 63) sh.wave_u64[wv] = base_mass, sh.wave_u32[wv] = base_count;
   __syncthreads();
   base_mass -= own_mass;
@@ -551,7 +547,7 @@ __device__ __forceinline__ void draw_from_bins(const SampleArgs& a, int b, const
           from_at = ws.offset[(size_t)lane * OFFSETS + bin];
           n = ws.offset[(size_t)lane * OFFSETS + bin + 1] - from_at;
         }
-        const uint32_t end = wave_scan(n, lane);
+        const uint32_t end = wave_scan(n);
         if (lane < MAX_PARTS) sh.part_end[lane] = end, sh.part_at[lane] = from_at - (end - n);
         if (lane == 63) sh.n = end;
       }
@@ -648,8 +644,8 @@ __device__ __forceinline__ void draw_from_bins(const SampleArgs& a, int b, const
         u64 m[4], mt = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) c[i] = sh.digit_count[4 * lane + i], m[i] = sh.digit_mass[4 * lane + i], ct += c[i], mt += m[i];
-        ct = before_count + wave_scan(ct, lane) - ct;
-        mt = before_mass + wave_scan(mt, lane) - mt;
+        ct = before_count + wave_scan(ct) - ct;
+        mt = before_mass + wave_scan(mt) - mt;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if (by_count ? ct <= target && target < ct + c[i] : mt <= target && target < mt + m[i]) sh.found_bin = 4 * lane + i, sh.found_count = ct, sh.found_mass = mt;
@@ -840,7 +836,7 @@ template <int TYPE> __global__ __launch_bounds__(512) void sample_bins_kernel(Sa
 #pragma unroll
   for (int i = 0; i < PER; ++i) c[i] = count[tid * PER + i], before += c[i];
   const uint32_t own = before;
-  before = wave_scan(before, tid & 63);
+  before = wave_scan(before);
   if ((tid & 63) == 63) sh.wave_u32[tid >> 6] = before;
   __syncthreads();   // and nobody reads the counts any more
   before -= own;
