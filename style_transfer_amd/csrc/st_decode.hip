@@ -1022,47 +1022,47 @@ static int decode_loop(const StDecoderWeights* w, const float* latent, int B, in
                          n_dev, out_ids, sm->logp, T, pos, eos, pad, early, last, ws.idx[cur ^ 1], ws.cnt + (cur ^ 1));
       ST_LAUNCH_CHECK();
     } else {
-    GemmArgs gg = {};
-    gg.fmt = w->gemm_format; gg.range_flag = ws.cnt + 3;
-    gg.X = ws.x; gg.n_dev = n_dev; gg.n_host = n_bound; gg.ln_a = w->lnf_a; gg.ln_b = w->lnf_b;
-    gg.W = w->gen_w; gg.bias = w->gen_b; gg.N = w->vocab; gg.partial = ws.partial;
-    gg.colpad = w->gemm_format == ST_GEMM_F16X3 ? ws.colpad : nullptr;
-    // partial buffer: B * ST_GEN_SPLITS + 64 * ST_GEN_SPLITS_SMALL entries
-    const long room = ((long)B * ST_GEN_SPLITS + 64L * ST_GEN_SPLITS_SMALL) / n_bound;
-    const int gsplits = rp_splits(n_bound, w->vocab, (int)(room < ST_GEN_SPLITS_SMALL ? (room < ST_GEN_SPLITS ? ST_GEN_SPLITS : room) : ST_GEN_SPLITS_SMALL));
-    // (a vocabulary beyond 32768 would not fit the block number into the screening kernel's 8 key bits: no screening)
-    const bool screen = screen_ok && n_bound >= ST_SCREEN_MIN_ROWS && (w->vocab + 127) / 128 <= RS_MAX_BLOCKS;
-    ProfPair pp;
-    if (g_prof_on == ST_PROF_GENERATOR) ST_TRY(prof_begin(&pp, 2.0 * 256.0 * (double)w->vocab, n_dev, n_bound, st));
-    if (screen) {
-      // pass 1: one-product logits for every live row; rows with a clear winner are finished
-      // per-column bound (gen_w_norm): the screening kernel books upper bounds, finish_kernel uses the winner's own norm
-      const float cx_c = 1.25f * (1.0f / 1024.0f + 1.0f / 65536.0f);
-      const float* wnorm = (rp_screen_shape16 && w->gen_w_norm && !rp_screen_maxnorm) ? w->gen_w_norm : nullptr;
-      gg.wnorm = wnorm; gg.scale = cx_c;
-      ST_TRY(launch_rp_screen_pipelined(gg, n_bound, gsplits, st));  // bookkeeping interleaved with the next block's MFMAs
-      gg.wnorm = nullptr;
-      hipLaunchKernelGGL(finish_kernel, dim3((n_bound + FIN_THREADS - 1) / FIN_THREADS), dim3(FIN_THREADS), 0, st, ws.partial, gsplits, idx, n_dev,
-                         out_ids, (float*)nullptr, T, pos, eos, pad, early, last, ws.idx[cur ^ 1], ws.cnt + (cur ^ 1),
-                         (const int*)nullptr, margin_c, ws.amb, ws.cnt + 2, wnorm, cx_c);
-      ST_LAUNCH_CHECK();
-      // pass 2: the undecided rows again with the 3-product kernel (row gather through ws.amb; the grid covers
-      // the worst case, workgroups beyond the ambiguous count exit at once)
-      gg.xrows = ws.amb; gg.n_dev = ws.cnt + 2;
-      const int rsplits = rp_splits((n_bound + 15) / 16, w->vocab, ST_GEN_SPLITS);
-      ST_TRY(launch_rp<EPI_ARGMAX>(gg, n_bound, rsplits, st));
-      hipLaunchKernelGGL(finish_kernel, dim3((n_bound + FIN_THREADS - 1) / FIN_THREADS), dim3(FIN_THREADS), 0, st, ws.partial, rsplits, idx, ws.cnt + 2,
-                         out_ids, (float*)nullptr, T, pos, eos, pad, early, last, ws.idx[cur ^ 1], ws.cnt + (cur ^ 1),
-                         (const int*)ws.amb, -1.0f, (int*)nullptr, (int*)nullptr, (const float*)nullptr, 0.0f);
-      ST_LAUNCH_CHECK();
-    } else {
-      ST_TRY(launch_rp<EPI_ARGMAX>(gg, n_bound, gsplits, st));
-      hipLaunchKernelGGL(finish_kernel, dim3((n_bound + FIN_THREADS - 1) / FIN_THREADS), dim3(FIN_THREADS), 0, st, ws.partial, gsplits, idx, n_dev,
-                         out_ids, top2gap, T, pos, eos, pad, early, last, ws.idx[cur ^ 1], ws.cnt + (cur ^ 1),
-                         (const int*)nullptr, -1.0f, (int*)nullptr, (int*)nullptr, (const float*)nullptr, 0.0f);
-      ST_LAUNCH_CHECK();
-    }
-    if (g_prof_on == ST_PROF_GENERATOR) ST_TRY(prof_end(&pp, st));
+      GemmArgs gg = {};
+      gg.fmt = w->gemm_format; gg.range_flag = ws.cnt + 3;
+      gg.X = ws.x; gg.n_dev = n_dev; gg.n_host = n_bound; gg.ln_a = w->lnf_a; gg.ln_b = w->lnf_b;
+      gg.W = w->gen_w; gg.bias = w->gen_b; gg.N = w->vocab; gg.partial = ws.partial;
+      gg.colpad = w->gemm_format == ST_GEMM_F16X3 ? ws.colpad : nullptr;
+      // partial buffer: B * ST_GEN_SPLITS + 64 * ST_GEN_SPLITS_SMALL entries
+      const long room = ((long)B * ST_GEN_SPLITS + 64L * ST_GEN_SPLITS_SMALL) / n_bound;
+      const int gsplits = rp_splits(n_bound, w->vocab, (int)(room < ST_GEN_SPLITS_SMALL ? (room < ST_GEN_SPLITS ? ST_GEN_SPLITS : room) : ST_GEN_SPLITS_SMALL));
+      // (a vocabulary beyond 32768 would not fit the block number into the screening kernel's 8 key bits: no screening)
+      const bool screen = screen_ok && n_bound >= ST_SCREEN_MIN_ROWS && (w->vocab + 127) / 128 <= RS_MAX_BLOCKS;
+      ProfPair pp;
+      if (g_prof_on == ST_PROF_GENERATOR) ST_TRY(prof_begin(&pp, 2.0 * 256.0 * (double)w->vocab, n_dev, n_bound, st));
+      if (screen) {
+        // pass 1: one-product logits for every live row; rows with a clear winner are finished
+        // per-column bound (gen_w_norm): the screening kernel books upper bounds, finish_kernel uses the winner's own norm
+        const float cx_c = 1.25f * (1.0f / 1024.0f + 1.0f / 65536.0f);
+        const float* wnorm = (rp_screen_shape16 && w->gen_w_norm && !rp_screen_maxnorm) ? w->gen_w_norm : nullptr;
+        gg.wnorm = wnorm; gg.scale = cx_c;
+        ST_TRY(launch_rp_screen_pipelined(gg, n_bound, gsplits, st));  // bookkeeping interleaved with the next block's MFMAs
+        gg.wnorm = nullptr;
+        hipLaunchKernelGGL(finish_kernel, dim3((n_bound + FIN_THREADS - 1) / FIN_THREADS), dim3(FIN_THREADS), 0, st, ws.partial, gsplits, idx, n_dev,
+                           out_ids, (float*)nullptr, T, pos, eos, pad, early, last, ws.idx[cur ^ 1], ws.cnt + (cur ^ 1),
+                           (const int*)nullptr, margin_c, ws.amb, ws.cnt + 2, wnorm, cx_c);
+        ST_LAUNCH_CHECK();
+        // pass 2: the undecided rows again with the 3-product kernel (row gather through ws.amb; the grid covers
+        // the worst case, workgroups beyond the ambiguous count exit at once)
+        gg.xrows = ws.amb; gg.n_dev = ws.cnt + 2;
+        const int rsplits = rp_splits((n_bound + 15) / 16, w->vocab, ST_GEN_SPLITS);
+        ST_TRY(launch_rp<EPI_ARGMAX>(gg, n_bound, rsplits, st));
+        hipLaunchKernelGGL(finish_kernel, dim3((n_bound + FIN_THREADS - 1) / FIN_THREADS), dim3(FIN_THREADS), 0, st, ws.partial, rsplits, idx, ws.cnt + 2,
+                           out_ids, (float*)nullptr, T, pos, eos, pad, early, last, ws.idx[cur ^ 1], ws.cnt + (cur ^ 1),
+                           (const int*)ws.amb, -1.0f, (int*)nullptr, (int*)nullptr, (const float*)nullptr, 0.0f);
+        ST_LAUNCH_CHECK();
+      } else {
+        ST_TRY(launch_rp<EPI_ARGMAX>(gg, n_bound, gsplits, st));
+        hipLaunchKernelGGL(finish_kernel, dim3((n_bound + FIN_THREADS - 1) / FIN_THREADS), dim3(FIN_THREADS), 0, st, ws.partial, gsplits, idx, n_dev,
+                           out_ids, top2gap, T, pos, eos, pad, early, last, ws.idx[cur ^ 1], ws.cnt + (cur ^ 1),
+                           (const int*)nullptr, -1.0f, (int*)nullptr, (int*)nullptr, (const float*)nullptr, 0.0f);
+        ST_LAUNCH_CHECK();
+      }
+      if (g_prof_on == ST_PROF_GENERATOR) ST_TRY(prof_end(&pp, st));
     }
     cur ^= 1;
     ++steps;
