@@ -828,3 +828,33 @@ def test_gemm_q4_out_and_bias_in_one_buffer(dev):
         ops.gemm_q4(x[:1].bfloat16(), q, buf[3, :128], out=buf.view(torch.bfloat16)[3:4, 254:382])
     ops.gemm_q4(x, q, buf[3, 150:278], out=buf[:, :128])       # beside the columns that are written
     assert torch.equal(buf[:, :128], want)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_quantize_weight_q4_codes(dev, group, zeros):
+    """scales, zero codes and codes equal to the definition's: the scale in f32 and then f16, a code the nearest whole number of
+    scales above the zero code, 0 to 15, ties to even (f32 quotients, as the definition has them); odd columns and a short last group"""
+    from style_transfer_amd import ops
+    n, k = 29, 301
+    g = torch.Generator(device=dev).manual_seed(group + zeros)
+    W = torch.randn(n, k, generator=g, device=dev) * torch.exp(3 * torch.randn(n, 1, generator=g, device=dev))
+    W[3], W[4], W[5], W[6] = 0, 0.7, W[5].abs() + 1.0, -W[6].abs() - 1.0
+    W[7], W[8] = W[7] * 1e-7, W[8] * 1e-12             # scales that are f16 subnormals, or 0
+    W[9] = torch.randint(-7, 8, (k,), generator=g, device=dev).float() * 0.5   # ties and exact codes
+    codes, scales, z = ops.quantize_weight_q4(W, group, zeros)
+    w, got = W.cpu().numpy(), codes_of(codes, k)
+    f = np.float32
+    for i in range(n):
+        for j in range(0, k, group):
+            v = w[i, j:j + group]
+            hi, lo = f(max(v.max(), 0)), f(min(v.min(), 0))
+            step = (f(hi - lo) / f(15) if zeros else max(hi, -lo) / f(7)).astype(np.float16)
+            s, at = f(step), j // group
+            assert scales[i, at].cpu().numpy() == step, (i, j)
+            zero = 8
+            if zeros:
+                zero = int(np.clip(np.rint(-lo / s), 0, 15)) if s > 0 else 0
+                assert int(z[i, at]) == zero, (i, j)
+            want = np.clip(np.clip(np.rint(v / s), -16, 16) + zero, 0, 15) if s > 0 else np.full(len(v), zero)
+            assert np.array_equal(got[i, j:j + group], want), (i, j)
