@@ -405,8 +405,9 @@ def _sample_settings(B, dev, temperature, top_k, top_p, min_p):
 
 
 def _workspace(ws, nbytes, device):
-    """a DecodeWorkspace's buffer, or one for this call alone"""
-    if ws is None:
+    """a DecodeWorkspace's buffer, or one for this call alone.  A graph that is being captured gets one from its own pool: the
+    DecodeWorkspace's may be replaced by a larger one, or serve another graph, before the replay."""
+    if ws is None or torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
     buf = ws.get(nbytes)
     if buf.device != device:

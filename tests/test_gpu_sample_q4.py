@@ -858,3 +858,35 @@ def test_quantize_weight_q4_codes(dev, group, zeros):
                 assert int(z[i, at]) == zero, (i, j)
             want = np.clip(np.clip(np.rint(v / s), -16, 16) + zero, 0, 15) if s > 0 else np.full(len(v), zero)
             assert np.array_equal(got[i, j:j + group], want), (i, j)
+
+
+def test_sample_workspace_in_graphs(dev):
+    """two graphs captured with one DecodeWorkspace, which a larger call replaces before they are replayed, side by side"""
+    from style_transfer_amd import ops
+    ws, s = ops.DecodeWorkspace(dev), dict(top_p=0.95)
+    sets = [some_logits(dev, 40, 30001, "f32", i)[:2] for i in (1, 2)]
+    want = [ops.sample_logits(l, u, ws=ws, **s) for l, u in sets]
+    first = ws.buf.data_ptr(), ws.buf.numel()
+    graphs, outs = [], []
+    for l, u in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(ops.sample_logits(l, u, ws=ws, **s))
+    big = some_logits(dev, 2, 400000, "bf16", 3)[:2]
+    assert ws.buf.data_ptr() == first[0]
+    ws.get(first[1] + (8 << 20))
+    other = torch.full((first[1],), 7, dtype=torch.uint8, device=dev)      # where the first one was
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        for o in outs:
+            o[0].fill_(-9)
+        side.wait_stream(torch.cuda.current_stream())
+        graphs[0].replay()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+        ids, logp = ops.sample_logits(*big, ws=ws, **s)
+        torch.cuda.synchronize()
+        check_sample(*big, ids, logp, **s)
+        for o, w in zip(outs, want):
+            assert torch.equal(o[0], w[0]) and torch.equal(o[1], w[1])
+    assert bool((other == 7).all())
