@@ -412,6 +412,7 @@ def _workspace(ws, nbytes, device):
     buf = ws.get(nbytes)
     if buf.device != device:
         raise ValueError("ws is on %s, not on %s" % (buf.device, device))
+    buf.record_stream(torch.cuda.current_stream(device))   # a larger one may replace it while this call still runs
     return buf
 
 
@@ -419,7 +420,7 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, wan
     """One token per row of logits [B, V] (f32, bf16 or f16; rows may be strided) from the uniform numbers u [B] (f32, in
     [0, 1)) -> (ids int32 [B], logp f32 [B] or None).  Filters in the order temperature, top_k (0: off), top_p (1: off),
     min_p (0: off); each is a number or a tensor [B].  temperature 0: argmax.  A row of -inf / NaN alone: id -1, logp -inf.
-    logp is a value: no gradient goes from it to the logits."""
+    logp is a value: no gradient goes from it to the logits.  Calls that may run at the same time need a ws each, or none."""
     kind, ld = _rows_of(logits, "logits")
     B, V = logits.shape
     dev = logits.device

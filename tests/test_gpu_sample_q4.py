@@ -890,3 +890,21 @@ def test_sample_workspace_in_graphs(dev):
         for o, w in zip(outs, want):
             assert torch.equal(o[0], w[0]) and torch.equal(o[1], w[1])
     assert bool((other == 7).all())
+
+
+def test_sample_workspace_replaced_while_another_stream_uses_it(dev):
+    from style_transfer_amd import ops
+    logits, u, _ = some_logits(dev, 40, 30001, "f32", 1)
+    want = ops.sample_logits(logits, u, top_p=0.95)
+    ws = ops.DecodeWorkspace(dev)
+    at, n = ws.get(ops.lib().st_sample_workspace_bytes(40, 30001)).data_ptr(), ws.buf.numel()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)                      # about a tenth of a second before the draw starts
+        got = ops.sample_logits(logits, u, top_p=0.95, ws=ws)
+    ws.get(n + (8 << 20))
+    other = torch.empty(n, dtype=torch.uint8, device=dev)
+    assert not side.query() and other.data_ptr() != at      # the old buffer still belongs to the draw
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
