@@ -445,7 +445,7 @@ long long st_format_attack_log(const char* vocab_bytes, const int64_t* vocab_off
  * bytes.  st_gemm_q4: x [M, K] and y [M, N] of `type` (ST_TYPE_*), rows ldx and ldy values apart (any alignment of whole
  * values; y shares no value with x or bias); bias f32 [N] or NULL.  Sums are held in f32, one rounding to y's type at the end; the codes
  * enter the product as they are, and so does an f16 x.  A bf16 or f32 value of x enters with an error of 2^-39 of its row's largest
- * value at most (f32: or of 2^-23 of itself, if that is more).  A row of x with an infinity or a NaN gives values that are not finite.
+ * value at most (f32: or of 2^-22 of itself, if that is more).  A row of x with an infinity or a NaN gives values that are not finite.
  * M = 0 is a no-op.  N and K up to 2^24, M up to ST_Q4_MAX_ROWS (ST_EINVAL beyond).  Asynchronous, needs no workspace, may be
  * captured into a graph.                                                                                                   */
 #define ST_Q4_MAX_ROWS (65535 * 16)

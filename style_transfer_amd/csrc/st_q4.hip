@@ -5,8 +5,8 @@
 // group: no weight is rounded.  x in f16 goes in as it is.  x in bf16 or f32 is first multiplied, row by row, with a power of
 // two that brings the row's largest value to [2^14, 2^15).  A bf16 value then is an f16 value (8 significant bits of 11); what is
 // below 2^-31 of the largest loses bits as an f16 subnormal, rounded to the nearest: an error of 2^-39 of the row's largest at
-// most.  An f32 value is split into hi + lo, each to the nearest, and costs two products: an error of 2^-23 of the value or 2^-39
-// of the row's largest, whichever is more.
+// most.  An f32 value is split into hi + lo and costs two products: hi is cut to 11 bits, what is left (below 2^-10 of the value's
+// power of two) is rounded to the nearest of 11 bits: an error of 2^-22 of the value or, in subnormals, 2^-39 of the row's largest.
 #include "st_common.h"
 
 namespace {
@@ -186,7 +186,7 @@ template <int TYPE> struct X8 {
     for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(value(i)));
     return m;
   }
-  // the values times 2^14 over the row's power of two as f16, to the nearest, and for f32 what that leaves, to the nearest
+  // the values times 2^14 over the row's power of two as f16, and for f32 what that leaves
   __device__ __forceinline__ void split(float shift, h8& hi, h8& lo) const {
     if constexpr (TYPE == ST_TYPE_F16) {
       hi = __builtin_bit_cast(h8, *(const u32x4*)w);
@@ -195,7 +195,8 @@ template <int TYPE> struct X8 {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float a = value(2 * i) * shift, b = value(2 * i + 1) * shift;
-        const h2 q = {(_Float16)a, (_Float16)b};   // (one instruction)
+        // f32: towards 0, what that leaves is kept in lo (to the nearest here takes 7 x 4751 x 2119 from 8.5 to 9.4 us)
+        const h2 q = TYPE == ST_TYPE_F32 ? __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(a, b)) : h2{(_Float16)a, (_Float16)b};
         h[i] = __builtin_bit_cast(uint32_t, q);
         if constexpr (TYPE == ST_TYPE_F32) {
           lo[2 * i] = (_Float16)fmaxf(a - (float)q[0], -65504.0f);        // an infinity: inf - inf is not wanted
