@@ -563,7 +563,9 @@ __device__ __forceinline__ void draw_from_bins(const SampleArgs& a, int b, const
     __syncthreads();
     const uint32_t n_bin = sh.n;
     __syncthreads();
-    // more of the row in one bin than the list holds (equal logits, mostly): the rounds below go over the row itself
+    // More of the row in one bin than the list holds (equal logits, mostly): the rounds below go over the row itself, twice a round, and
+    // that takes its time.  us, as in text / three values / one value: 4096 x 9339 top_p 0.9 150 / 665 / 815, with top_k 50 57 / 1057 /
+    // 1372; 1 x 131072 24 / 376 / 1051, 27 / 568 / 1665.
     const bool from_row = n_bin > room;
     auto walk = [&](auto f) SM_INLINE {   // f(place) for this thread's share of the bin
       if (SPLIT || !from_row) {
@@ -937,6 +939,12 @@ template <int TYPE> int launch_type(const SampleArgs& a, hipStream_t st) {
   int len = 0;
   const int parts = parts_of(a.B, a.V, &len);
   if (parts == 1) {
+    // Bins, and half as many places in the list.  Up to 1024 entries the list takes any row, so that no row is marked and one launch is
+    // enough: with 1024 / 2048 bins 4096 x 777 settings by row 31.6 / 28.4 us, 600 x 777 top_k 50 10.8 / 9.2; unfiltered draws pay for
+    // it, they sort the list where bins would do: 4096 x 777 40 / 99 us, 1 x 777 8.9 / 23.  Beyond, with 1024 / 2048 / 4096 bins, us:
+    // 128 x 9339 15.3 / 15.3 / 16.3, 1024 x 9339 top_k 400 42.9 / 44.0 / 48.5; 1024 x 19724 62.7 / 59.6 / 61.1, top_p 0.9 73.5 / 71.4 /
+    // 73.4, top_k 400 70.4 / 71.4 / 74.9; 200 x 50001 top_k 400 45.2 / 45.3 / 46.2, unfiltered 46.8 / 45.9 / 39.4; 256 x 131072 190 /
+    // 104 / 103, top_p 0.9 126 / 122 / 117.
     const int nbin = a.V <= 1024 ? 2048 : a.V <= 16384 ? 1024 : a.V <= 65536 ? 2048 : 4096;
     const size_t lds = (size_t)nbin * 12;
     // 256 x 131072 bf16: 151 us with 1024, 189 with 512; 128 x 9339: 16.0 and 14.5
@@ -945,6 +953,10 @@ template <int TYPE> int launch_type(const SampleArgs& a, hipStream_t st) {
     const bool lists = a.V <= nbin / 2 || (alike && (!(a.set.temperature > 0.0f) || (a.set.top_k > 0 && a.set.top_k <= 128)));
     const long rows = ((1L << 32) - 1) / threads;   // a launch has fewer than 2^32 threads
     ST_CHECK_ARG(a.B <= rows, "B=%d: at most %ld rows of %d values in one call", a.B, rows, a.V);
+    // Lists by a kernel of their own / by the one that has both, top_k 50, us.  9339 entries: 64 rows 13.1 / 9.6, 512 rows 14.1 / 11.9,
+    // 1024 rows 20.6 / 22.0, 4096 rows 56.8 / 74.8; 3000: 512 rows 10.8 / 9.9, 1024 rows 13.0 / 16.7; 50001: 256 rows 31.8 / 23.5, 512
+    // rows 38.9 / 41.4.  (With settings by row, longer rows than the list take the kernel that has both: 4096 x 9339 76 us where one
+    // setting for all takes 57.)
     if (lists && a.B >= 512) {
       hipLaunchKernelGGL((sample_row_kernel<TYPE, true, false, 8>), dim3(a.B), dim3(256), lds, st, a, nbin, 0);
       ST_LAUNCH_CHECK();

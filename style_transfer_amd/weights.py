@@ -167,7 +167,8 @@ class AEWeights(_Packed):
 
     def quantized_generator(self, group=64, zero_points=False):
         """the generator matrix [vocab, 256], as it was given to this object, in 4 bits with a scale per `group` columns
-        (ops.Q4Weight): ops.sample_decode's head"""
+        (ops.Q4Weight): ops.sample_decode's head.  For the tests' two models 2.5 to 5.4 in 100 greedy tokens then differ from those of
+        the f32 matrix after the same tokens (groups of 32 to 128, with and without zero_points)."""
         from . import ops
         W = self._generator.to(self.where).contiguous()
         return ops.pack_weight_q4(*ops.quantize_weight_q4(W, group, zero_points), group=group)
